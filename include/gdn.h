@@ -398,6 +398,86 @@ int gdn_attn_fwd(const void* q, const void* qg, int64_t qg_ld, const void* k_cac
                  int64_t Hkv, int64_t D, int64_t cap, int64_t kv_len_max, int64_t n_split,
                  void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------------
+ * The attention layers' cache in blocks, for batches whose rows share a long
+ * prefix: pools of keys and values [n_blocks, Hkv, block, D] bf16, and per row
+ * a table of the blocks its positions lie in (position p is row p % block of
+ * block table[b][p / block]; slot = block id * block + p % block).
+ * --------------------------------------------------------------------- */
+
+/*
+ * Block tables, slots and the free list for T new tokens per row (n_new[b] of
+ * them where n_new [B] is given, clamped to [0, T]):
+ *   need[b] = max(ceil((lengths[b] + new) / block), shared) blocks
+ *   held[b]  blocks the row's table lists now.  A row with more than it needs
+ *            gives the last ones back: they go onto the end of the stack
+ *            free_blocks[0 .. n_free[0]), in row order, each row's ascending.
+ *            Then a row with fewer takes blocks from the stack's end, in row
+ *            order.  A row that does not get all it asks for gets none, nor does
+ *            any row after it that asks; a row that needs more blocks than its
+ *            table is wide keeps what it holds.
+ *   slots    [B, T]: slot of the row's token t at position lengths[b] + t; -1
+ *            past new, and for every token of a row that did not get its blocks
+ *   held_out [B], n_free_out [1]: the counts afterwards; they may be held and
+ *            n_free (in place).  Otherwise the same call can be made again: table
+ *            and free_blocks are written past held and n_free only.
+ * All int32.  The first `shared` blocks of a row are never given back.
+ * block: a power of two up to 2^20; table rows are table_ld apart; free_blocks
+ * has room for n_blocks; B <= 4096; B * T and n_blocks * block below 2^31.
+ */
+int gdn_paged_tables(const int32_t* lengths, const int32_t* n_new, int32_t* table, int64_t table_ld,
+                     const int32_t* held, int32_t* free_blocks, const int32_t* n_free, int32_t* held_out,
+                     int32_t* n_free_out, int32_t* slots, int64_t B, int64_t T, int64_t block,
+                     int64_t shared, int64_t n_blocks, void* stream);
+
+/*
+ * q/k norm, rotary positions and cache append, like gdn_attn_qk, with
+ *   qg       heads q_head elements apart (2D: q then its gate; D: no gate)
+ *   q_norm_w, k_norm_w  or both NULL: no norm
+ *   turns    [rot/2] uint64: turns (of 2 pi) of pair i per position, as a
+ *            fraction of 2^64: the angle of a far position is as exact as a near
+ *            one's
+ *   factor   multiplies the rotated dims (1, or a long-context scaling's)
+ *   interleaved  pairs (2i, 2i + 1); otherwise (i, i + rot/2)
+ *   slots    [B,T] int32 slots of gdn_paged_tables; a token whose slot is not in
+ *            [0, n_blocks * block) is padding: its q is zeros, its k and v go
+ *            nowhere.  NULL: row b's own block b (n_blocks == B), at pos0[b] + t
+ *            clamped as in gdn_attn_qk: the dense cache [B,Hkv,cap,D].
+ * Norm and rotation are in fp32 and rounded once.  D in {128, 256}; rot even, and
+ * a multiple of D/32 for pairs (i, i + rot/2).  Slots are below 2^31.
+ */
+int gdn_attn_rope(const void* qg, int64_t qg_ld, int64_t q_head, const void* k_new, const void* v_new,
+                  int64_t kv_ld, const void* q_norm_w, const void* k_norm_w, int w_dtype, float eps,
+                  const int32_t* pos0, const int32_t* slots, const uint64_t* turns, float factor,
+                  int interleaved, void* q_out, void* keys, void* values, int64_t B, int64_t T,
+                  int64_t Hq, int64_t Hkv, int64_t D, int64_t n_blocks, int64_t block, int64_t rot,
+                  void* stream);
+
+/* Workspace bytes gdn_paged_attn needs for n_ranges = n_prefix + n_own key
+ * ranges (0 for one). */
+size_t gdn_paged_attn_workspace_bytes(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
+                                      int64_t n_ranges);
+
+/*
+ * gdn_attn_fwd over block tables: token t < n_new[b] (all T where n_new is NULL)
+ * of row b sees keys 0 .. pos0[b] + t; other tokens' outputs are zeros.
+ *   table    [B, table_ld] int32; entries are read as if clamped to the pool
+ *   shared   blocks at the start of every row's table that are the same (and
+ *            full) in all rows; pos0[b] is read as at least shared * block
+ *   n_prefix > 0: the shared keys are read once for all rows of the batch, in
+ *            n_prefix ranges, apart from each row's own; 0: with the row's own
+ *   n_own    key ranges of a row's own keys
+ *   kv_len_max  host bound of pos0[b] + n_new[b], in [shared * block + T (0 where
+ *            n_new is given), table_ld * block]
+ * block: a power of two from 64 on.  Other arguments as in gdn_attn_fwd.
+ */
+int gdn_paged_attn(const void* q, const void* qg, int64_t qg_ld, const void* keys, const void* values,
+                   const int32_t* table, int64_t table_ld, const int32_t* pos0, const int32_t* n_new,
+                   void* out, float scale, int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
+                   int64_t n_blocks, int64_t block, int64_t kv_len_max, int64_t shared,
+                   int64_t n_prefix, int64_t n_own, void* workspace, size_t workspace_bytes,
+                   void* stream);
+
 /* RMSNorm of bf16 rows (mlx nn.RMSNorm): y = h / sqrt(mean(h^2) + eps) * w
  * with h = x, or h = bf16(x + res) when res is not NULL (a residual add
  * fused in front; h is written to h_out when not NULL, which may alias x).

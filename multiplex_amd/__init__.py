@@ -30,6 +30,8 @@ from .linear import DecodeWorkspace, gated_norm_linear_decode, linear_decode
 from .mixer import GatedDeltaNet, commit_verified
 from .mixed_step import MixedStep
 from .attention import Attention, AttentionArgs, DecoderLayer, KVCache, MTPHead
+from .paged import BlockPool, PagedKVCache, paged_attn, paged_tables
+from .rotary import Rotary, attn_rope
 
 __all__ = [
     "Attention",
@@ -37,6 +39,12 @@ __all__ = [
     "DecoderLayer",
     "KVCache",
     "MTPHead",
+    "BlockPool",
+    "PagedKVCache",
+    "paged_attn",
+    "paged_tables",
+    "Rotary",
+    "attn_rope",
     "ArraysCache",
     "DecodeWorkspace",
     "GatedDeltaNet",

@@ -53,6 +53,10 @@ EXPORTS = (
     "gdn_attn_qk",
     "gdn_attn_workspace_bytes",
     "gdn_attn_fwd",
+    "gdn_paged_tables",
+    "gdn_attn_rope",
+    "gdn_paged_attn_workspace_bytes",
+    "gdn_paged_attn",
     "gdn_rms_norm",
     "gdn_pos_add",
     "gdn_silu_mul",
@@ -191,6 +195,21 @@ _SIGNATURES = {
     "gdn_attn_fwd": (
         c_int,
         [_P, _P, _I64, _P, _P, _P, _P, c_float, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P, c_size_t, _P],
+    ),
+    "gdn_paged_tables": (
+        c_int,
+        [_P, _P, _P, _I64, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _P],
+    ),
+    "gdn_attn_rope": (
+        c_int,
+        [_P, _I64, _I64, _P, _P, _I64, _P, _P, c_int, c_float, _P, _P, _P, c_float, c_int, _P, _P, _P,
+         _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P],
+    ),
+    "gdn_paged_attn_workspace_bytes": (c_size_t, [_I64, _I64, _I64, _I64, _I64, _I64]),
+    "gdn_paged_attn": (
+        c_int,
+        [_P, _P, _I64, _P, _P, _P, _I64, _P, _P, _P, c_float, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
+         _I64, _I64, _P, c_size_t, _P],
     ),
     "gdn_rms_norm": (c_int, [_P, _P, _P, _P, c_int, _P, _I64, _I64, _I64, c_float, _P]),
     "gdn_pos_add": (c_int, [_P, _I64, c_int32, c_int32, _P]),

@@ -38,6 +38,7 @@ import torch
 from . import _lib
 from .gated_delta import _dtype_code, _ptr, _require_device, _stream
 from .linear import linear
+from .rotary import Rotary, attn_rope
 
 __all__ = [
     "AttentionArgs",
@@ -66,6 +67,9 @@ class AttentionArgs:
     rms_norm_eps: float = 1e-6
     partial_rotary_factor: float = 0.25
     rope_theta: float = 10_000_000.0
+    # a long context's scaling and neighbouring pairs (mlx's ``traditional``): see :class:`Rotary`
+    rope_scaling: Optional[dict] = None
+    rope_traditional: bool = False
 
     @property
     def rot(self) -> int:
@@ -443,6 +447,8 @@ class Attention(torch.nn.Module):
         self.q_norm = RMSNorm(D, args.rms_norm_eps, device)
         self.k_norm = RMSNorm(D, args.rms_norm_eps, device)
         self.scale = D ** -0.5
+        self.rotary = Rotary(args.rot, args.rope_theta, interleaved=args.rope_traditional, scaling=args.rope_scaling,
+                             device=device)
         self.n_split = n_split
         self._cus = None
 
@@ -507,14 +513,35 @@ class Attention(torch.nn.Module):
         partials = 4e-6 * B * self.Hkv * rows * ranges * self.D  # MB
         return ranges if block_us * (blocks - of_range) > 3.5 + mb_us * partials else 1
 
-    def forward(self, x: torch.Tensor, cache: KVCache) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, cache: "KVCache | PagedKVCache",
+                n_new: Optional[Sequence[int]] = None) -> torch.Tensor:
+        """The layer's output for T new tokens a row, appended to ``cache``.  With
+        a :class:`PagedKVCache`, ``n_new`` (host counts) says how many of the T a
+        row has; the rest is padding, whose outputs are unspecified."""
         B, T, _ = x.shape
         Hq, Hkv, D = self.Hq, self.Hkv, self.D
+        pool = getattr(cache, "pool", None)
+        if pool is None and n_new is not None:
+            raise ValueError("n_new needs a PagedKVCache")
         qkv = linear(x, self.qkv_proj)
         qg, k, v = qkv.split((2 * Hq * D, Hkv * D, Hkv * D), -1)
+        if pool is not None:
+            counts = None if n_new is None else cache.counts(n_new)
+            slots = cache.reserve(T, n_new, counts)
+            q = attn_rope(qg, k, v, self.q_norm.weight, self.k_norm.weight, self.args.rms_norm_eps, cache.pos0,
+                          pool.keys, pool.values, self.rotary, slots=slots)
+            L = max((n + m for n, m in zip(cache.lengths, n_new or [T] * B)), default=T)
+            o = paged_attn(q, pool.keys, pool.values, cache.table, cache.pos0, L, n_new=counts, shared=cache.shared,
+                           gate=qg, scale=self.scale)
+            cache.advance(T, n_new, counts)
+            return linear(o.view(B, T, Hq * D), self.o_proj)
         cache.reserve(T)
-        q = attn_qk(qg, k, v, self.q_norm.weight, self.k_norm.weight, self.args.rms_norm_eps, cache.pos0,
-                    cache.keys, cache.values, self.args.rot, self.args.rope_theta)
+        if self.rotary.plain:
+            q = attn_qk(qg, k, v, self.q_norm.weight, self.k_norm.weight, self.args.rms_norm_eps, cache.pos0,
+                        cache.keys, cache.values, self.args.rot, self.args.rope_theta)
+        else:
+            q = attn_rope(qg, k, v, self.q_norm.weight, self.k_norm.weight, self.args.rms_norm_eps, cache.pos0,
+                          cache.keys, cache.values, self.rotary)
         L = cache.offset + T
         o = attn_fwd(q, cache.keys, cache.values, cache.pos0, L, gate=qg, scale=self.scale,
                      n_split=self._splits(B, T, L))
@@ -549,11 +576,13 @@ class DecoderLayer(torch.nn.Module):
         self.input_layernorm = RMSNorm(args.hidden_size, args.rms_norm_eps, device)
         self.post_attention_layernorm = RMSNorm(args.hidden_size, args.rms_norm_eps, device)
 
-    def forward(self, x: torch.Tensor, cache: KVCache) -> torch.Tensor:
-        h, m = self.forward_parts(x, None, cache)
+    def forward(self, x: torch.Tensor, cache: "KVCache | PagedKVCache",
+                n_new: Optional[Sequence[int]] = None) -> torch.Tensor:
+        h, m = self.forward_parts(x, None, cache, n_new)
         return h + m
 
-    def forward_parts(self, x: torch.Tensor, residual: Optional[torch.Tensor], cache: KVCache):
+    def forward_parts(self, x: torch.Tensor, residual: Optional[torch.Tensor], cache: "KVCache | PagedKVCache",
+                      n_new: Optional[Sequence[int]] = None):
         """The layer on ``x + residual`` (or ``x``), returning ``(h, m)`` whose
         sum is its output: the caller adds them inside the next norm
         (``gdn_rms_norm`` with a residual, the same bf16 rounding point), so no
@@ -563,7 +592,7 @@ class DecoderLayer(torch.nn.Module):
         else:
             xin, y0 = self.input_layernorm(x, residual=residual)
         # the residual add in front of the second norm is fused into it
-        h, y = self.post_attention_layernorm(xin, residual=self.self_attn(y0, cache))
+        h, y = self.post_attention_layernorm(xin, residual=self.self_attn(y0, cache, n_new))
         return h, self.mlp(y)
 
 
@@ -587,7 +616,14 @@ class MTPHead(torch.nn.Module):
         a = self.args
         return [KVCache(batch, a.num_key_value_heads, a.head_dim, capacity, dev) for _ in self.layers]
 
-    def forward(self, embed: torch.Tensor, hidden: torch.Tensor, cache: Sequence[KVCache]) -> torch.Tensor:
+    def make_paged_cache(self, batch: int, n_blocks: int, block: int = 64, capacity: int = 256) -> "List[PagedKVCache]":
+        """Each draft layer's cache over a pool of ``n_blocks`` blocks of its own."""
+        dev, a = self.fc.device, self.args
+        return [PagedKVCache(BlockPool(n_blocks, a.num_key_value_heads, a.head_dim, block, dev), batch, capacity)
+                for _ in self.layers]
+
+    def forward(self, embed: torch.Tensor, hidden: torch.Tensor,
+                cache: "Sequence[KVCache | PagedKVCache]") -> torch.Tensor:
         """Post-norm hidden ``[B, L, H]``; each draft layer's cache advances by L."""
         if len(cache) != len(self.layers):
             raise ValueError(f"expected {len(self.layers)} draft caches, got {len(cache)}")
@@ -604,9 +640,13 @@ class MTPHead(torch.nn.Module):
         return self.norm(res, residual=x)[1]
 
     @staticmethod
-    def trim_cache_to(cache: Sequence[KVCache], size: int) -> None:
+    def trim_cache_to(cache: "Sequence[KVCache | PagedKVCache]", size: int) -> None:
         """``Drafter.trim_cache_to`` (mtp.py:497-503)."""
         target = max(0, int(size))
         for c in cache:
             if c.size() > target:
                 c.trim(c.size() - target)
+
+
+# the paged cache builds on this module's
+from .paged import BlockPool, PagedKVCache, paged_attn  # noqa: E402
