@@ -548,8 +548,8 @@ constexpr int kPrefillRows = 512;  // rows (tokens x heads of a group) per kv-he
 constexpr int PR = 128;            // rows per workgroup
 constexpr int VTP = KB;            // Vt row stride (bf16); 16-byte granules XOR-swizzled by (d & 7)
 
-template <int D, int KG>
-__global__ __launch_bounds__(256 * KG) void attn_prefill_kernel(const AttnParams p) {
+template <int D, int KG, class P = AttnParams>
+__global__ __launch_bounds__(256 * KG) void attn_prefill_kernel(const P p) {
   constexpr int NT = 256 * KG;                // threads
   constexpr int NS = D / 32;                  // k-steps of q . k
   constexpr int NJ = D / 16;                  // 16-wide d tiles of the output
@@ -567,23 +567,27 @@ __global__ __launch_bounds__(256 * KG) void attn_prefill_kernel(const AttnParams
   constexpr int kMl = KG == 2 ? 8 * 128 * 4 : 0;  // the waves' (m, l) for the merge
   __shared__ __align__(128) unsigned char smem[2 * (KSTAGE + VSTAGE) + kMl + 4 * 2 * QL * 1024];
 
-  const int b = blockIdx.z, split = blockIdx.y;
-  const int n_rb = gridDim.x / p.Hkv;
+  // The paged grid numbers (kv-head, range) pairs first, so that the row tiles that read a range's keys
+  // run on one XCD where the pairs are a multiple of the eight, and its L2 reads them once.
+  const int b = blockIdx.z, split = P::kPaged ? blockIdx.x / p.Hkv : blockIdx.y;
+  const int n_rb = P::kPaged ? gridDim.y : gridDim.x / p.Hkv;
   const int hkv = blockIdx.x % p.Hkv;
-  const int rb = n_rb - 1 - static_cast<int>(blockIdx.x) / p.Hkv;  // longest key ranges first
+  // longest key ranges first
+  const int rb = n_rb - 1 - static_cast<int>(P::kPaged ? blockIdx.y : blockIdx.x / p.Hkv);
   const int g = p.Hq / p.Hkv;
-  const int n_rows = p.T * g;
+  const int n_rows = tile_rows(p, g);
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int rg = wave & 3, kh = wave >> 2;  // the wave's 32 rows of the workgroup's, and its keys of each block
   const int lr = lane & 15, lq = lane >> 4;
-  const int p0 = first_pos(p.pos0, b, p.T, p.cap);
+  const int tokens = row_tokens(p, b);
+  const int p0 = row_start(p, b, tokens);
 
   const int row0 = rb * PR;
-  const int t_last = min((row0 + PR - 1) / g, p.T - 1);
-  const int k_lo = split * p.split_len;
-  const int k_hi = min(p0 + t_last + 1, k_lo + p.split_len);  // keys of this workgroup: [k_lo, k_hi)
-  const int k_free = min(p0 + row0 / g + 1, k_hi);             // keys below this are visible to every row
+  const int t_last = min((row0 + PR - 1) / g, tokens - 1);
+  const KeyRange keys = key_range(p, split, p0, t_last, row0 / g < tokens);
+  const int k_lo = keys.lo, k_hi = keys.hi;  // keys of this workgroup: [k_lo, k_hi)
+  const int k_free = prefix_of(p) ? k_hi : min(p0 + row0 / g + 1, k_hi);  // keys below this are visible to every row
   const int nblk = k_hi > k_lo ? (k_hi - k_lo + KB - 1) / KB : 0;
 
   // the wave's two 16-row tiles; rows past the end compute on q = 0 and are not stored.  The last QL
@@ -597,10 +601,11 @@ __global__ __launch_bounds__(256 * KG) void attn_prefill_kernel(const AttnParams
 #pragma unroll
   for (int rt = 0; rt < 2; ++rt) {
     const int r = row0 + 32 * rg + 16 * rt + lr;
-    const bool ok = r < n_rows;
-    const int t = ok ? r / g : p.T - 1, hq = hkv * g + (ok ? r % g : 0);
-    kmax[rt] = p0 + t;
-    const uint16_t* qrow = p.q + ((static_cast<int64_t>(b) * p.T + t) * p.Hq + hq) * D;
+    const RowAt at = row_at(p, b, hkv, g, min(r, n_rows - 1));
+    const bool ok = r < n_rows && (!P::kPaged || prefix_of(p) || at.t < tokens);
+    const int t = at.t, hq = P::kPaged || ok ? at.hq : hkv * g;
+    kmax[rt] = prefix_of(p) ? INT_MAX : p0 + t;
+    const uint16_t* qrow = p.q + ((static_cast<int64_t>(at.b) * p.T + t) * p.Hq + hq) * D;
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
       const u32x4 v = *reinterpret_cast<const u32x4*>(qrow + 32 * s + 8 * lq);
@@ -613,10 +618,26 @@ __global__ __launch_bounds__(256 * KG) void attn_prefill_kernel(const AttnParams
   // K and V blocks are read through descriptors that end at the range's last
   // key, so the lane offsets are constants and keys past the range (masked
   // below) read as zeros
-  const unsigned char* kc_head =
-      reinterpret_cast<const unsigned char*>(p.kc + (static_cast<int64_t>(b) * p.Hkv + hkv) * p.cap * D);
-  const unsigned char* vc_head =
-      reinterpret_cast<const unsigned char*>(p.vc + (static_cast<int64_t>(b) * p.Hkv + hkv) * p.cap * D);
+  const int64_t head = P::kPaged ? 0 : (static_cast<int64_t>(b) * p.Hkv + hkv) * p.cap * D;
+  const unsigned char* kc_head = reinterpret_cast<const unsigned char*>(p.kc + head);
+  const unsigned char* vc_head = reinterpret_cast<const unsigned char*>(p.vc + head);
+  // The paged cache's step i lies where the table says: lane l holds the block of step page0 + l, so that a
+  // step's is one lane's read, and no load for it is among the loop's.
+  int page0 = 0, pages = 0;
+  auto load_pages = [&](int blk) {
+    page0 = blk;
+    const int kb = min(k_lo + KB * (blk + lane), k_hi - 1);
+    pages = nblk > 0 ? block_of(p, b, kb) : 0;
+  };
+  // byte offset of the step of keys at kb (a whole number of steps past k_lo)
+  auto step_off = [&](int kb) -> int64_t {
+    if constexpr (P::kPaged) {
+      const int page = __builtin_amdgcn_readlane(pages, (kb - k_lo) / KB - page0);
+      return key_off<D>(p, b, hkv, kb, page) * 2;
+    } else {
+      return static_cast<int64_t>(kb) * (D * 2);
+    }
+  };
   auto block_bytes = [&](int kb) { return min(k_hi - kb, KB) * (D * 2); };
   // K block -> stage st: thread tid's load i fills physical granule i * NT + tid, which is row
   // i * KR + tid / KROW, granule (tid % KROW) ^ (row & 7) of the block (the swizzle does not depend on i)
@@ -627,9 +648,9 @@ __global__ __launch_bounds__(256 * KG) void attn_prefill_kernel(const AttnParams
   // LDS address of the wave's 1 KB slice of load 0 in stage 0
   const uint32_t k_lds = __builtin_amdgcn_readfirstlane(
       static_cast<uint32_t>(reinterpret_cast<uintptr_t>(smem)) + wave * 1024);
-  auto k_dma = [&](int kb, int bytes, int st, int i) {  // the block's bytes from load i's first row on
+  auto k_dma = [&](int64_t off, int bytes, int st, int i) {  // the block's bytes from load i's first row on
     constexpr int kLoad = KR * D * 2;
-    lds_dma16(buf_words(kc_head + static_cast<int64_t>(kb) * (D * 2) + i * kLoad, max(bytes - i * kLoad, 0)), k_off,
+    lds_dma16(buf_words(kc_head + off + i * kLoad, max(bytes - i * kLoad, 0)), k_off,
               k_lds + st * KSTAGE + i * (NT * 16));
   };
   // V block -> registers: pair i is key quad tid % 16 (4 rows) x d octet i * NT / 16 + tid / 16
@@ -679,12 +700,14 @@ __global__ __launch_bounds__(256 * KG) void attn_prefill_kernel(const AttnParams
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(4 * VPAIRS) : "memory");
   };
   if (nblk > 0) {
+    if constexpr (P::kPaged) load_pages(0);
     const int nb = block_bytes(k_lo);
     const int k1 = nblk > 1 ? k_lo + KB : k_lo;
-    const __amdgpu_buffer_rsrc_t vrs = buf_rsrc(vc_head + static_cast<int64_t>(k_lo) * (D * 2), nb);
-    const __amdgpu_buffer_rsrc_t vrs1 = buf_rsrc(vc_head + static_cast<int64_t>(k1) * (D * 2), block_bytes(k1));
+    const int64_t off0 = step_off(k_lo);
+    const __amdgpu_buffer_rsrc_t vrs = buf_rsrc(vc_head + off0, nb);
+    const __amdgpu_buffer_rsrc_t vrs1 = buf_rsrc(vc_head + step_off(k1), block_bytes(k1));
 #pragma unroll
-    for (int i = 0; i < KDMA; ++i) k_dma(k_lo, nb, 0, i);
+    for (int i = 0; i < KDMA; ++i) k_dma(off0, nb, 0, i);
 #pragma unroll
     for (int i = 0; i < VPAIRS; ++i) {
 #pragma unroll
@@ -706,7 +729,11 @@ __global__ __launch_bounds__(256 * KG) void attn_prefill_kernel(const AttnParams
     // last block (never used), so that none sits behind a branch.
     const int kb1 = blk + 1 < nblk ? kb + KB : kb, kb2 = blk + 2 < nblk ? kb + 2 * KB : kb1;
     const int nb1 = block_bytes(kb1);
-    const __amdgpu_buffer_rsrc_t vrs = buf_rsrc(vc_head + static_cast<int64_t>(kb2) * (D * 2), block_bytes(kb2));
+    if constexpr (P::kPaged) {
+      if (blk - page0 >= 32) load_pages(blk);  // steps blk + 1 and blk + 2 are always among the lanes'
+    }
+    const int64_t off1 = step_off(kb1);
+    const __amdgpu_buffer_rsrc_t vrs = buf_rsrc(vc_head + step_off(kb2), block_bytes(kb2));
 
     // S^T = K Q^T: lane (r, q) holds keys 16 kt + 4q + i of row r, for both row tiles
     const unsigned char* Ks = smem + st * KSTAGE;
@@ -726,7 +753,7 @@ __global__ __launch_bounds__(256 * KG) void attn_prefill_kernel(const AttnParams
       const int s = f / KTW, kt = f % KTW;
       const bf16x8 a = kf[f % KPF];
       if (f + KPF < NS * KTW) kf[f % KPF] = k_frag((f + KPF) / KTW, (f + KPF) % KTW);
-      if (kt == 0 && s < KDMA) k_dma(kb1, nb1, st ^ 1, s);
+      if (kt == 0 && s < KDMA) k_dma(off1, nb1, st ^ 1, s);
       const bool in_regs = s < NS - QL;
       sc[0][kt] = mfma16(a, in_regs ? qf[0][in_regs ? s : 0] : *q_lds(0, s), sc[0][kt]);
       sc[1][kt] = mfma16(a, in_regs ? qf[1][in_regs ? s : 0] : *q_lds(1, s), sc[1][kt]);
@@ -839,13 +866,23 @@ __global__ __launch_bounds__(256 * KG) void attn_prefill_kernel(const AttnParams
     constexpr int rt = decltype(rtc)::value;
     const int r = row0 + 32 * rg + 16 * rt + lr;
     if (r >= n_rows) return;
+    const RowAt at = row_at(p, b, hkv, g, r);
+    if constexpr (P::kPaged) {
+      if (!prefix_of(p) && at.t >= tokens) {  // a padded token
+        if (p.n_split == 1) {
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) store_zero4<D>(p, b, at.t, at.hq, 16 * j + 4 * lq);
+        }
+        return;
+      }
+    }
     if (p.n_split == 1) {
       const float inv_l = 1.0f / lt[rt];  // (l = 0: every score is -inf, whose softmax is NaN)
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) store_out4<D>(p, b, r / g, hkv * g + r % g, 16 * j + 4 * lq, o[rt][j], inv_l);
+      for (int j = 0; j < NJ; ++j) store_out4<D>(p, b, at.t, at.hq, 16 * j + 4 * lq, o[rt][j], inv_l);
       return;
     }
-    const int64_t pr = part_row(p, b, hkv, r) + split;
+    const int64_t pr = part_row(p, at.b, hkv, at.row) + split_at(p, split);
     const int64_t n_part = static_cast<int64_t>(p.B) * p.Hkv * p.rows_pad * p.n_split;
     if (lq == 0) {
       p.part[n_part * D + pr] = m[rt];

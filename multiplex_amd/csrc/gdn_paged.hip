@@ -465,7 +465,7 @@ extern "C" int gdn_paged_attn(const void* q, const void* qg, int64_t qg_ld, cons
       !gdn_host::aligned(out, 8) || (qg && (!gdn_host::aligned(qg, 8) || qg_ld % 4 != 0)))
     return fail(GDN_ERR_INVALID, "gdn_paged_attn: misaligned pointer");
   const int64_t g = Hq / Hkv, rows = T * g, n_split = n_prefix + n_own;
-  if (B > 65535 || B * rows > INT32_MAX / 2 || Hkv * ((B * rows + 15) / 16) > INT32_MAX ||
+  if (B > 65535 || Hkv > 65535 || (B * rows + PR - 1) / PR > 65535 || Hkv * n_split > INT32_MAX ||
       B * Hkv * rows * n_split * (D + 2) > (int64_t(1) << 40))
     return fail(GDN_ERR_UNSUPPORTED, "gdn_paged_attn: problem too large");
   const size_t need = gdn_paged_attn_workspace_bytes(B, T, Hq, Hkv, D, n_split);
@@ -500,16 +500,15 @@ extern "C" int gdn_paged_attn(const void* q, const void* qg, int64_t qg_ld, cons
     p.prefix = n_prefix > 0 && split0 == 0;
     p.split0 = static_cast<int>(split0);
     p.split_len = static_cast<int>(((keys_hi - keys_lo + n - 1) / n + KB - 1) / KB * KB);
-    const int rt = tile_rows <= 16 ? 1 : 4;
-    const int64_t y = Hkv * ((tile_rows + 16 * rt - 1) / (16 * rt));
-    if (y > 65535) return fail(GDN_ERR_UNSUPPORTED, "gdn_paged_attn: problem too large");
-    const dim3 grid(static_cast<unsigned>(n), static_cast<unsigned>(y), static_cast<unsigned>(batch));
-    if (D == 256) {
-      if (rt == 4) hipLaunchKernelGGL((attn_fwd_kernel<256, 4, PagedParams>), grid, dim3(256), 0, st, p);
-      else hipLaunchKernelGGL((attn_fwd_kernel<256, 1, PagedParams>), grid, dim3(256), 0, st, p);
-    } else {
-      if (rt == 4) hipLaunchKernelGGL((attn_fwd_kernel<128, 4, PagedParams>), grid, dim3(256), 0, st, p);
+    if (tile_rows <= 16) {
+      const dim3 grid(static_cast<unsigned>(n), static_cast<unsigned>(Hkv), static_cast<unsigned>(batch));
+      if (D == 256) hipLaunchKernelGGL((attn_fwd_kernel<256, 1, PagedParams>), grid, dim3(256), 0, st, p);
       else hipLaunchKernelGGL((attn_fwd_kernel<128, 1, PagedParams>), grid, dim3(256), 0, st, p);
+    } else {
+      const int64_t tiles = (tile_rows + PR - 1) / PR;
+      const dim3 grid(static_cast<unsigned>(Hkv * n), static_cast<unsigned>(tiles), static_cast<unsigned>(batch));
+      if (D == 256) hipLaunchKernelGGL((attn_prefill_kernel<256, 2, PagedParams>), grid, dim3(512), 0, st, p);
+      else hipLaunchKernelGGL((attn_prefill_kernel<128, 1, PagedParams>), grid, dim3(256), 0, st, p);
     }
     return gdn_host::check_launch("gdn_paged_attn");
   };

@@ -104,13 +104,13 @@ def _ranges(cus: int, B: int, T: int, Hq: int, Hkv: int, prefix: int, own: int) 
     """``(n_prefix, n_own)``: key ranges of the shared prefix (0: read with each
     row's own keys) and of a row's own keys, for workgroups enough."""
     rows = T * (Hq // Hkv)
-    if prefix and (B == 1 or rows >= 64):
+    if prefix and (B == 1 or rows >= 128):
         prefix, own = 0, own + prefix
-    tiles = -(-rows // (16 if rows <= 16 else 64))
+    tiles = -(-rows // (16 if rows <= 16 else 128))
     n_own = max(1, min(cus // max(B * Hkv * tiles, 1), own // 128))
     if not prefix:
         return 0, n_own
-    tiles = -(-B * rows // (16 if B * rows <= 16 else 64))
+    tiles = -(-B * rows // (16 if B * rows <= 16 else 128))
     return max(1, min(cus // (Hkv * tiles), prefix // 128)), n_own
 
 
