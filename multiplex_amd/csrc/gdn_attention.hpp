@@ -75,6 +75,7 @@ struct PagedParams : AttnParams {
   const int32_t* n_new;  // [B] or null: T
   int table_ld, lg, n_blocks, key0, prefix;
   int split0;  // the launch's first key range of the row's n_split
+  int reread;  // rows' own keys start with the shared ones: other rows read them too
 };
 
 // A value that no kernel of this library's call writes, by a scalar load where
@@ -186,14 +187,44 @@ __device__ __forceinline__ void store_out4(const AttnParams& p, int b, int t, in
   *reinterpret_cast<u32x2*>(p.out + row * D + d) = u32x2{pk_bf16(y[0], y[1]), pk_bf16(y[2], y[3])};
 }
 
+// A lane's N pieces of 4 of one output row, STEP columns apart: o / l times the gate, whose loads are all
+// issued before the first is used.  (l = 0: every score is -inf, whose softmax is NaN.)
+template <int D, int N, int STEP>
+__device__ __forceinline__ void store_row(const AttnParams& p, const RowAt& at, int d, const f32x4* o, float l) {
+  const int64_t bt = static_cast<int64_t>(at.b) * p.T + at.t;
+  uint16_t* out = p.out + (bt * p.Hq + at.hq) * D + d;
+  const float inv_l = 1.0f / l;
+  if (p.qg == nullptr) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const f32x4 y = o[n] * inv_l;
+      *reinterpret_cast<u32x2*>(out + STEP * n) = u32x2{pk_bf16(y[0], y[1]), pk_bf16(y[2], y[3])};
+    }
+    return;
+  }
+  u32x2 gate[N];
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+    gate[n] = *reinterpret_cast<const u32x2*>(p.qg + bt * p.qg_ld + at.hq * 2 * D + D + d + STEP * n);
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    f32x4 y = o[n] * inv_l;
+    y[0] *= sigmoid(__uint_as_float(gate[n].x << 16));
+    y[1] *= sigmoid(__uint_as_float(gate[n].x & 0xffff0000u));
+    y[2] *= sigmoid(__uint_as_float(gate[n].y << 16));
+    y[3] *= sigmoid(__uint_as_float(gate[n].y & 0xffff0000u));
+    *reinterpret_cast<u32x2*>(out + STEP * n) = u32x2{pk_bf16(y[0], y[1]), pk_bf16(y[2], y[3])};
+  }
+}
+
 // A padded token's output.
 template <int D>
 __device__ __forceinline__ void store_zero4(const AttnParams& p, int b, int t, int hq, int d) {
   *reinterpret_cast<u32x2*>(p.out + ((static_cast<int64_t>(b) * p.T + t) * p.Hq + hq) * D + d) = u32x2{0u, 0u};
 }
 
-template <int D, int RT, class P = AttnParams>
-__global__ __launch_bounds__(256) void attn_fwd_kernel(const P p) {
+template <int D, int RT>
+__global__ __launch_bounds__(256) void attn_fwd_kernel(const AttnParams p) {
   constexpr int KP = D + 8;   // K row stride (bf16): 16-byte fragment reads of 16 rows hit distinct banks
   constexpr int VP = D + 16;  // V row stride: the transposed reads of 4 rows hit distinct banks
   constexpr int KT = RT == 4 ? 4 : 1;  // 16-key tiles per wave and block
@@ -205,29 +236,28 @@ __global__ __launch_bounds__(256) void attn_fwd_kernel(const P p) {
   const int hkv = blockIdx.y % p.Hkv, rb = blockIdx.y / p.Hkv;
   const int split = blockIdx.x;
   const int g = p.Hq / p.Hkv;
-  const int n_rows = tile_rows(p, g);
+  const int n_rows = p.T * g;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lr = lane & 15, lq = lane >> 4;
-  const int tokens = row_tokens(p, b);
-  const int p0 = row_start(p, b, tokens);
+  const int p0 = first_pos(p.pos0, b, p.T, p.cap);
 
   const int row0 = rb * 16 * RT;
-  const int t_last = min((row0 + 16 * RT - 1) / g, tokens - 1);
-  const KeyRange keys = key_range(p, split, p0, t_last, row0 / g < tokens);
-  const int k_lo = keys.lo, k_hi = keys.hi;  // keys of this workgroup: [k_lo, k_hi)
+  const int t_last = min((row0 + 16 * RT - 1) / g, p.T - 1);
+  const int k_lo = split * p.split_len;
+  const int k_hi = min(p0 + t_last + 1, k_lo + p.split_len);  // keys of this workgroup: [k_lo, k_hi)
   const int rt = RT == 4 ? wave : 0;
   const int sub = RT == 4 ? 0 : wave;  // first 16-key tile of this wave in each block
 
   // this wave's 16 rows (lane lr's row): Q as the B operand of S^T = K Q^T
   const int r = row0 + 16 * rt + lr;
-  const RowAt at = row_at(p, b, hkv, g, r < n_rows ? r : 0);
-  const int t = at.t, hq = at.hq;
-  const bool row_ok = r < n_rows && !(P::kPaged && !prefix_of(p) && t >= tokens);
-  const int kmax = prefix_of(p) ? INT_MAX : p0 + t;  // last key row r may see
+  const bool row_ok = r < n_rows;
+  const int t = row_ok ? r / g : 0;
+  const int hq = hkv * g + (row_ok ? r % g : 0);
+  const int kmax = p0 + t;  // last key row r may see
   bf16x8 qf[NS];
   {
-    const uint16_t* qrow = p.q + ((static_cast<int64_t>(at.b) * p.T + t) * p.Hq + hq) * D;
+    const uint16_t* qrow = p.q + ((static_cast<int64_t>(b) * p.T + t) * p.Hq + hq) * D;
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
       const u32x4 v = *reinterpret_cast<const u32x4*>(qrow + 32 * s + 8 * lq);
@@ -246,14 +276,13 @@ __global__ __launch_bounds__(256) void attn_fwd_kernel(const P p) {
   // 152.8 us at B=64).
   u32x4 kr[CPT], vr[CPT];
   const int64_t head_base = (static_cast<int64_t>(b) * p.Hkv + hkv) * p.cap * D;
-  auto load_blk = [&](int kb, int page) {
-    const int64_t base = P::kPaged ? key_off<D>(p, b, hkv, kb, page) - static_cast<int64_t>(kb) * D : head_base;
+  auto load_blk = [&](int kb) {
 #pragma unroll
     for (int i = 0; i < CPT; ++i) {
       const int c = tid + 256 * i;
       const int row = c / (D / 8), col = (c % (D / 8)) * 8;
       const int key = kb + row;
-      const int64_t off = base + static_cast<int64_t>(min(key, k_hi - 1)) * D + col;  // in bounds: k_hi <= cap
+      const int64_t off = head_base + static_cast<int64_t>(min(key, k_hi - 1)) * D + col;  // in bounds: k_hi <= cap
       kr[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p.kc + off));
       vr[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p.vc + off));
     }
@@ -276,19 +305,13 @@ __global__ __launch_bounds__(256) void attn_fwd_kernel(const P p) {
   for (int j = 0; j < NJ; ++j) o[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
   const int nblk = k_hi > k_lo ? (k_hi - k_lo + KB - 1) / KB : 0;
-  // the block after the next one's table entry, read a step before its keys are
-  int page = nblk > 0 ? block_of(p, b, k_lo) : 0;
-  if (nblk > 0) load_blk(k_lo, page);
-  if (nblk > 1) page = block_of(p, b, k_lo + KB);
+  if (nblk > 0) load_blk(k_lo);
   for (int blk = 0; blk < nblk; ++blk) {
     const int kb = k_lo + KB * blk;
     __syncthreads();  // the previous block's reads are done
     store_blk(kb);
     __syncthreads();
-    if (blk + 1 < nblk) {
-      load_blk(kb + KB, page);
-      if (blk + 2 < nblk) page = block_of(p, b, kb + 2 * KB);
-    }
+    if (blk + 1 < nblk) load_blk(kb + KB);
 
     // S^T = K Q^T for this wave's key tiles: lane (r, q) holds keys 16 kt + 4q + i of row r
     f32x4 sc[KT];
@@ -362,19 +385,9 @@ __global__ __launch_bounds__(256) void attn_fwd_kernel(const P p) {
   const bool split_out = p.n_split > 1;
   if constexpr (RT == 4) {
     // lane (r, q) holds O[row r][16 j + 4 q + i]
-    if constexpr (P::kPaged) {
-      if (!row_ok) {
-        if (r < n_rows && !split_out) {
-#pragma unroll
-          for (int j = 0; j < NJ; ++j) store_zero4<D>(p, b, t, hq, 16 * j + 4 * lq);
-        }
-        return;
-      }
-    } else {
-      if (!row_ok) return;
-    }
+    if (!row_ok) return;
     if (split_out) {
-      const int64_t pr = part_row(p, at.b, hkv, at.row) + split_at(p, split);
+      const int64_t pr = part_row(p, b, hkv, r) + split;
       float* po = p.part + pr * D;
 #pragma unroll
       for (int j = 0; j < NJ; ++j) *reinterpret_cast<f32x4*>(po + 16 * j + 4 * lq) = o[j];
@@ -386,7 +399,7 @@ __global__ __launch_bounds__(256) void attn_fwd_kernel(const P p) {
       }
       return;
     }
-    const float inv_l = P::kPaged || l > 0.0f ? 1.0f / l : 0.0f;
+    const float inv_l = l > 0.0f ? 1.0f / l : 0.0f;
 #pragma unroll
     for (int j = 0; j < NJ; ++j) store_out4<D>(p, b, t, hq, 16 * j + 4 * lq, o[j], inv_l);
   } else {
@@ -408,17 +421,6 @@ __global__ __launch_bounds__(256) void attn_fwd_kernel(const P p) {
     const int mr = tid >> 4, c0 = (tid & 15) * CW;
     const int rr = row0 + mr;
     if (rr >= n_rows) return;
-    const RowAt mat = row_at(p, b, hkv, g, rr);
-    const int tt = mat.t, hh = mat.hq;
-    if constexpr (P::kPaged) {
-      if (!prefix_of(p) && tt >= tokens) {
-        if (!split_out) {
-#pragma unroll
-          for (int c = 0; c < CW; c += 4) store_zero4<D>(p, b, tt, hh, c0 + c);
-        }
-        return;
-      }
-    }
     float mw[4], ms = -INFINITY;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
@@ -433,7 +435,7 @@ __global__ __launch_bounds__(256) void attn_fwd_kernel(const P p) {
       lsum += sw[w] * Ls[w * 16 + mr];
     }
     if (split_out) {
-      const int64_t pr = part_row(p, mat.b, hkv, mat.row) + split_at(p, split);
+      const int64_t pr = part_row(p, b, hkv, rr) + split;
       float* po = p.part + pr * D;
 #pragma unroll
       for (int c = 0; c < CW; c += 4) {
@@ -450,7 +452,8 @@ __global__ __launch_bounds__(256) void attn_fwd_kernel(const P p) {
       }
       return;
     }
-    const float inv_l = P::kPaged || lsum > 0.0f ? 1.0f / lsum : 0.0f;
+    const float inv_l = lsum > 0.0f ? 1.0f / lsum : 0.0f;
+    const int tt = rr / g, hh = hkv * g + rr % g;
 #pragma unroll
     for (int c = 0; c < CW; c += 4) {
       f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -518,6 +521,13 @@ __device__ __forceinline__ void lds_dma16(u32x4 rsrc, uint32_t voff, uint32_t ld
                : "v"(voff), "s"(rsrc), "s"(lds_base)
                : "memory", "m0");
 }
+// The same for bytes that are read once: not kept in the caches.
+__device__ __forceinline__ void lds_dma16_once(u32x4 rsrc, uint32_t voff, uint32_t lds_base) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen nt lds"
+               :
+               : "v"(voff), "s"(rsrc), "s"(lds_base)
+               : "memory", "m0");
+}
 
 // Max / sum over the four 16-lane rows of a wave (lanes r, r + 16, r + 32, r + 48), by the
 // gfx950 row-swap moves (VALU, no LDS round trip): permlane16_swap(x, x) yields the even and the
@@ -548,8 +558,18 @@ constexpr int kPrefillRows = 512;  // rows (tokens x heads of a group) per kv-he
 constexpr int PR = 128;            // rows per workgroup
 constexpr int VTP = KB;            // Vt row stride (bf16); 16-byte granules XOR-swizzled by (d & 7)
 
-template <int D, int KG, class P = AttnParams>
-__global__ __launch_bounds__(256 * KG) void attn_prefill_kernel(const P p) {
+// k-steps of q kept in LDS: as many as leave the loop without a spill
+template <int KG, class P>
+constexpr int q_lds_steps() { return KG == 2 ? (P::kPaged ? 3 : 2) : 0; }
+template <int D, int KG, class P>
+constexpr int tile_lds() {
+  return 2 * (KB * D * 2 + D * VTP * 2) + (KG == 2 ? 8 * 128 * 4 : 0) + 4 * 2 * q_lds_steps<KG, P>() * 1024;
+}
+
+// Tile rb of kv-head hkv's rows of batch entry b over key range `split`, by 256 * KG threads with
+// tile_lds<D, KG, P>() bytes of LDS.
+template <int D, int KG, class P>
+__device__ __forceinline__ void attn_tile(const P& p, unsigned char* smem, int b, int hkv, int rb, int split) {
   constexpr int NT = 256 * KG;                // threads
   constexpr int NS = D / 32;                  // k-steps of q . k
   constexpr int NJ = D / 16;                  // 16-wide d tiles of the output
@@ -563,17 +583,10 @@ __global__ __launch_bounds__(256 * KG) void attn_prefill_kernel(const P p) {
   static_assert(KDMA * NT == KB * KROW && VPAIRS * NT == (KB / 4) * KROW, "block must split evenly over the threads");
   static_assert(KDMA <= NS && 4 * VPAIRS <= NS, "at most one K and one V load per k-step");
 
-  constexpr int QL = KG == 2 ? 2 : 0;         // k-steps of q kept in LDS
+  constexpr int QL = q_lds_steps<KG, P>();
   constexpr int kMl = KG == 2 ? 8 * 128 * 4 : 0;  // the waves' (m, l) for the merge
-  __shared__ __align__(128) unsigned char smem[2 * (KSTAGE + VSTAGE) + kMl + 4 * 2 * QL * 1024];
+  static_assert(tile_lds<D, KG, P>() == 2 * (KSTAGE + VSTAGE) + kMl + 4 * 2 * QL * 1024, "LDS layout");
 
-  // The paged grid numbers (kv-head, range) pairs first, so that the row tiles that read a range's keys
-  // run on one XCD where the pairs are a multiple of the eight, and its L2 reads them once.
-  const int b = blockIdx.z, split = P::kPaged ? blockIdx.x / p.Hkv : blockIdx.y;
-  const int n_rb = P::kPaged ? gridDim.y : gridDim.x / p.Hkv;
-  const int hkv = blockIdx.x % p.Hkv;
-  // longest key ranges first
-  const int rb = n_rb - 1 - static_cast<int>(P::kPaged ? blockIdx.y : blockIdx.x / p.Hkv);
   const int g = p.Hq / p.Hkv;
   const int n_rows = tile_rows(p, g);
   const int tid = threadIdx.x, lane = tid & 63;
@@ -598,22 +611,30 @@ __global__ __launch_bounds__(256 * KG) void attn_prefill_kernel(const P p) {
   };
   int kmax[2];
   bf16x8 qf[2][NS - QL];
+  auto load_q = [&]() {
+    u32x4 v[2][NS];
+    bool ok[2];
 #pragma unroll
-  for (int rt = 0; rt < 2; ++rt) {
-    const int r = row0 + 32 * rg + 16 * rt + lr;
-    const RowAt at = row_at(p, b, hkv, g, min(r, n_rows - 1));
-    const bool ok = r < n_rows && (!P::kPaged || prefix_of(p) || at.t < tokens);
-    const int t = at.t, hq = P::kPaged || ok ? at.hq : hkv * g;
-    kmax[rt] = prefix_of(p) ? INT_MAX : p0 + t;
-    const uint16_t* qrow = p.q + ((static_cast<int64_t>(at.b) * p.T + t) * p.Hq + hq) * D;
+    for (int rt = 0; rt < 2; ++rt) {
+      const int r = row0 + 32 * rg + 16 * rt + lr;
+      const RowAt at = row_at(p, b, hkv, g, min(r, n_rows - 1));
+      ok[rt] = r < n_rows && (!P::kPaged || prefix_of(p) || at.t < tokens);
+      const int hq = P::kPaged || ok[rt] ? at.hq : hkv * g;
+      kmax[rt] = prefix_of(p) ? INT_MAX : p0 + at.t;
+      const uint16_t* qrow = p.q + ((static_cast<int64_t>(at.b) * p.T + at.t) * p.Hq + hq) * D;
 #pragma unroll
-    for (int s = 0; s < NS; ++s) {
-      const u32x4 v = *reinterpret_cast<const u32x4*>(qrow + 32 * s + 8 * lq);
-      const bf16x8 f = __builtin_bit_cast(bf16x8, ok ? v : u32x4{0u, 0u, 0u, 0u});
-      if (s < NS - QL) qf[rt][s] = f;
-      else if (kh == 0) *q_lds(rt, s) = f;
+      for (int s = 0; s < NS; ++s) v[rt][s] = *reinterpret_cast<const u32x4*>(qrow + 32 * s + 8 * lq);
     }
-  }
+#pragma unroll
+    for (int rt = 0; rt < 2; ++rt)
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        const bf16x8 f = __builtin_bit_cast(bf16x8, ok[rt] ? v[rt][s] : u32x4{0u, 0u, 0u, 0u});
+        if (s < NS - QL) qf[rt][s] = f;
+        else if (kh == 0) *q_lds(rt, s) = f;
+      }
+  };
+  if constexpr (!P::kPaged) load_q();
 
   // K and V blocks are read through descriptors that end at the range's last
   // key, so the lane offsets are constants and keys past the range (masked
@@ -713,6 +734,7 @@ __global__ __launch_bounds__(256 * KG) void attn_prefill_kernel(const P p) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) v_load(vrs, i, e);
     }
+    if constexpr (P::kPaged) load_q();  // behind the first keys' loads: one latency for both
 #pragma unroll
     for (int i = 0; i < VPAIRS; ++i) {
 #pragma unroll
@@ -728,12 +750,14 @@ __global__ __launch_bounds__(256 * KG) void attn_prefill_kernel(const P p) {
     // transposed, during O^T, and the registers take the block after it.  Past the end the loads re-read the
     // last block (never used), so that none sits behind a branch.
     const int kb1 = blk + 1 < nblk ? kb + KB : kb, kb2 = blk + 2 < nblk ? kb + 2 * KB : kb1;
-    const int nb1 = block_bytes(kb1);
+    // (the paged form reads nothing past the end: its descriptors there are empty)
+    const int nb1 = P::kPaged && blk + 1 >= nblk ? 0 : block_bytes(kb1);
     if constexpr (P::kPaged) {
       if (blk - page0 >= 32) load_pages(blk);  // steps blk + 1 and blk + 2 are always among the lanes'
     }
     const int64_t off1 = step_off(kb1);
-    const __amdgpu_buffer_rsrc_t vrs = buf_rsrc(vc_head + step_off(kb2), block_bytes(kb2));
+    const __amdgpu_buffer_rsrc_t vrs =
+        buf_rsrc(vc_head + step_off(kb2), P::kPaged && blk + 2 >= nblk ? 0 : block_bytes(kb2));
 
     // S^T = K Q^T: lane (r, q) holds keys 16 kt + 4q + i of row r, for both row tiles
     const unsigned char* Ks = smem + st * KSTAGE;
@@ -876,6 +900,10 @@ __global__ __launch_bounds__(256 * KG) void attn_prefill_kernel(const P p) {
         return;
       }
     }
+    if (P::kPaged && p.n_split == 1) {
+      store_row<D, NJ, 16>(p, at, 4 * lq, o[rt], lt[rt]);
+      return;
+    }
     if (p.n_split == 1) {
       const float inv_l = 1.0f / lt[rt];  // (l = 0: every score is -inf, whose softmax is NaN)
 #pragma unroll
@@ -888,11 +916,46 @@ __global__ __launch_bounds__(256 * KG) void attn_prefill_kernel(const P p) {
       p.part[n_part * D + pr] = m[rt];
       p.part[n_part * (D + 1) + pr] = lt[rt];
     }
-    if (nblk == 0) return;  // the combine does not read the O of a range without keys (l = 0)
+    if (nblk == 0) return;  // the combine does not use the O of a range without keys (l = 0)
 #pragma unroll
     for (int j = 0; j < NJ; ++j) *reinterpret_cast<f32x4*>(p.part + pr * D + 16 * j + 4 * lq) = o[rt][j];
   };
+  // The paged form's partial results go out in whole rows, through the wave's 64 D bytes of LDS at `at`: the
+  // accumulators' own layout would write 64 bytes of a row at a time, at a fifth of the rate (128 rows of 256:
+  // TODO against TODO us).
+  auto store_part = [&](auto rtc, unsigned char* buf) {
+    constexpr int rt = decltype(rtc)::value;
+    constexpr int G = D / 4;  // 16-byte granules of a row, XOR-swizzled by the row
+    const int r = row0 + 32 * rg + 16 * rt + lr;
+    const RowAt at = row_at(p, b, hkv, g, min(r, n_rows - 1));
+    const bool ok = r < n_rows && (prefix_of(p) || at.t < tokens);
+    const int64_t pr = part_row(p, at.b, hkv, at.row) + split_at(p, split);
+    if (ok && lq == 0) {
+      const int64_t n_part = static_cast<int64_t>(p.B) * p.Hkv * p.rows_pad * p.n_split;
+      p.part[n_part * D + pr] = m[rt];
+      p.part[n_part * (D + 1) + pr] = lt[rt];
+    }
+    if (nblk == 0) return;  // the combine does not use the O of a range without keys (l = 0)
+    f32x4* cell = reinterpret_cast<f32x4*>(buf);
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) cell[lr * G + ((4 * j + lq) ^ lr)] = o[rt][j];
+    const uint64_t rows = __builtin_amdgcn_ballot_w64(ok);
+#pragma unroll
+    for (int n = 0; n < 16; n += 64 / G) {
+      const int row = n + lane / G, col = lane % G;
+      const f32x4 x = cell[row * G + (col ^ row)];
+      const int64_t at_row = static_cast<int64_t>(__shfl(static_cast<int>(pr >> 32), row, 64)) << 32 |
+                             static_cast<uint32_t>(__shfl(static_cast<int>(pr), row, 64));
+      if ((rows >> row) & 1) *reinterpret_cast<f32x4*>(p.part + at_row * D + 4 * col) = x;
+    }
+  };
   if constexpr (KG == 1) {
+    if (P::kPaged && p.n_split > 1) {
+      __syncthreads();  // the stages are free
+      store_part(std::integral_constant<int, 0>{}, smem + wave * 64 * D);
+      store_part(std::integral_constant<int, 1>{}, smem + wave * 64 * D);
+      return;
+    }
     store_tile(std::integral_constant<int, 0>{});
     store_tile(std::integral_constant<int, 1>{});
   } else {
@@ -920,7 +983,8 @@ __global__ __launch_bounds__(256 * KG) void attn_prefill_kernel(const P p) {
 #pragma unroll
       for (int j = 0; j < NJ; ++j)
         o[rt][j] = a1 * o[rt][j] + a2 * *reinterpret_cast<const f32x4*>(xo + ((w * NJ + j) * 64 + lane) * 4);
-      store_tile(rtc);
+      if (P::kPaged && p.n_split > 1) store_part(rtc, smem + w * NJ * 1024);  // over what it has just read
+      else store_tile(rtc);
     };
     if (kh == 0) hand_over(std::integral_constant<int, 1>{});
     else hand_over(std::integral_constant<int, 0>{});
@@ -930,13 +994,21 @@ __global__ __launch_bounds__(256 * KG) void attn_prefill_kernel(const P p) {
   }
 }
 
+template <int D, int KG>
+__global__ __launch_bounds__(256 * KG) void attn_prefill_kernel(const AttnParams p) {
+  __shared__ __align__(128) unsigned char smem[tile_lds<D, KG, AttnParams>()];
+  const int n_rb = gridDim.x / p.Hkv;
+  // longest key ranges first
+  attn_tile<D, KG>(p, smem, blockIdx.z, blockIdx.x % p.Hkv, n_rb - 1 - static_cast<int>(blockIdx.x) / p.Hkv, blockIdx.y);
+}
+
 // One wave per (row, kv-head, batch row): the split partials of a row merged.
 // A range without keys of the row (l = 0) may have left its O unwritten: it is
 // skipped, its loads read the row's first range with keys instead.
 // Lane s takes range s's m and l (64 ranges a pass), and eight ranges' O are
 // in flight at a time.
-template <int D, class P = AttnParams>
-__global__ __launch_bounds__(256) void attn_combine_kernel(const P p) {
+template <int D>
+__global__ __launch_bounds__(256) void attn_combine_kernel(const AttnParams p) {
   const int lane = threadIdx.x & 63;
   const int g = p.Hq / p.Hkv;
   const int n_rows = p.T * g;
@@ -946,19 +1018,11 @@ __global__ __launch_bounds__(256) void attn_combine_kernel(const P p) {
   const int r = static_cast<int>(item % n_rows);
   const int hkv = static_cast<int>((item / n_rows) % p.Hkv);
   const int b = static_cast<int>(item / (static_cast<int64_t>(n_rows) * p.Hkv));
-  constexpr int EPL = D / 64, NB = 8;
-  const int t = r / g, hq = hkv * g + r % g;
-  if constexpr (P::kPaged) {
-    if (t >= row_tokens(p, b)) {  // a padded token
-      if constexpr (EPL == 4) store_zero4<D>(p, b, t, hq, EPL * lane);
-      else *reinterpret_cast<uint32_t*>(p.out + ((static_cast<int64_t>(b) * p.T + t) * p.Hq + hq) * D + EPL * lane) = 0u;
-      return;
-    }
-  }
   const int64_t n_part = static_cast<int64_t>(p.B) * p.Hkv * p.rows_pad * p.n_split;
   const int64_t pr = part_row(p, b, hkv, r);
   const float* pm = p.part + n_part * D + pr;
   const float* pl = p.part + n_part * (D + 1) + pr;
+  constexpr int EPL = D / 64, NB = 8;
   typedef float vec __attribute__((ext_vector_type(EPL)));
   vec acc = {};
   float m = -FLT_MAX, lsum = 0.0f;
@@ -992,7 +1056,8 @@ __global__ __launch_bounds__(256) void attn_combine_kernel(const P p) {
     }
   }
   // l = 0: every score is -inf, whose softmax is NaN (zeros in the kernel of fewer rows)
-  const float inv_l = P::kPaged || n_rows >= kPrefillRows || lsum > 0.0f ? 1.0f / lsum : 0.0f;
+  const float inv_l = n_rows >= kPrefillRows || lsum > 0.0f ? 1.0f / lsum : 0.0f;
+  const int t = r / g, hq = hkv * g + r % g;
   if constexpr (EPL == 4) {
     store_out4<D>(p, b, t, hq, EPL * lane, acc, inv_l);
   } else {
@@ -1008,4 +1073,5 @@ __global__ __launch_bounds__(256) void attn_combine_kernel(const P p) {
     *reinterpret_cast<uint32_t*>(p.out + row * D + d) = pk_bf16(y0, y1);
   }
 }
+
 }  // namespace

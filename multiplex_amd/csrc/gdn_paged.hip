@@ -324,6 +324,316 @@ __global__ __launch_bounds__(256) void attn_rope_kernel(const RopeParams p) {
   }
 }
 
+// ------------------------------------------------------------ attention
+
+// One launch covers a step: the workgroups of the shared prefix first (all rows
+// of the batch, read once per row tile), then each row's own keys.
+struct StepParams : PagedParams {
+  int n_prefix, n_own;        // key ranges
+  int len_prefix, len_own;    // keys of a range
+  int prefix_tiles, own_tiles;  // row tiles; 0: the rows fit the 16 of attn_rows
+};
+
+// Up to 16 rows of kv-head hkv (of batch entry b, or of the whole batch) over key
+// range `split`, by W waves.  Every wave takes 16 KT keys of a step of 16 KT W and
+// keeps a softmax state of its own; nothing in the loop waits for another wave.
+// K and V go to the wave's own 16 KB of LDS by direct loads of whole rows (K as
+// fragments from memory, 64 bytes of a row at a time, took the cold cache's read
+// from TODO to TODO TB/s), their 16-byte granules swizzled on the way: K's by
+// (key & 7), so that 16-byte fragment reads of 8 keys hit distinct banks, V's by
+// 2 (key & 7), so that its transposed reads of 4 x 4 keys do.  K of the next step
+// is asked for as soon as this one's scores are formed, V as soon as its products
+// are: a CU has up to 128 KB in flight.
+template <int D, int W>
+constexpr int rows_lds() {
+  constexpr int kv = W * 2 * 256 * 16 * 2, merge = W * 16 * D * 4 + 2 * W * 16 * 4;
+  return kv > merge ? kv : merge;
+}
+template <int D, int W>
+__device__ __forceinline__ void attn_rows(const PagedParams& p, unsigned char* smem, int b, int hkv, int split) {
+  constexpr int KT = 256 / D;         // 16-key tiles per wave and step
+  constexpr int KW = 16 * KT;         // keys per wave and step
+  constexpr int KS = KW * W;          // keys per step
+  constexpr int NS = D / 32, NJ = D / 16;
+  constexpr int KROW = D / 8;         // 16-byte granules per row
+  constexpr int LD = KW * KROW / 64;  // direct loads of 1 KB per wave, step and operand
+  constexpr int STAGE = KW * D * 2;   // bytes
+  const int g = p.Hq / p.Hkv;
+  const int n_rows = tile_rows(p, g);
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lr = lane & 15, lq = lane >> 4;
+  const int tokens = row_tokens(p, b);
+  const int p0 = row_start(p, b, tokens);
+  const KeyRange range = key_range(p, split, p0, tokens - 1, tokens > 0);
+  const int k_lo = range.lo + KW * wave, k_hi = range.hi;  // this wave's keys: KW from k_lo, k_lo + KS, ..
+  const int n_step = k_hi > k_lo ? (k_hi - k_lo + KS - 1) / KS : 0;
+
+  // lane l holds the block of the wave's step page0 + l
+  int page0 = 0, pages = 0;
+  auto load_pages = [&](int i) {
+    page0 = i;
+    pages = block_of(p, b, min(k_lo + KS * (i + lane), k_hi - 1));
+  };
+  // the wave's keys of step i: rows past the range read as zeros
+  unsigned char* ks = smem + wave * (2 * STAGE);
+  const unsigned char* vs = ks + STAGE;
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(ks)));
+  const int row0 = lane / KROW, gran = lane % KROW;
+  static_assert(64 % KROW == 0, "whole rows per load");
+  constexpr int RL = 64 / KROW;  // rows per load
+  // a row's own keys are read by one workgroup
+  const bool once = !prefix_of(p) && !p.reread;
+  auto load = [&](const uint16_t* pool, int i, uint32_t lds, int twist) {
+    const int kb = k_lo + KS * i;
+    const int64_t off = key_off<D>(p, b, hkv, kb, __builtin_amdgcn_readlane(pages, i - page0)) * 2;
+    const u32x4 rsrc = buf_words(reinterpret_cast<const unsigned char*>(pool) + off, min(k_hi - kb, KW) * (D * 2));
+#pragma unroll
+    for (int c = 0; c < LD; ++c) {
+      const int row = c * RL + row0;
+      const uint32_t off = row * (D * 2) + (gran ^ (twist * (row & 7))) * 16;
+      if (once) lds_dma16_once(rsrc, off, lds + c * 1024);
+      else lds_dma16(rsrc, off, lds + c * 1024);
+    }
+  };
+
+  if (n_step > 0) {
+    load_pages(0);
+    load(p.kc, 0, lds0, 1);
+  }
+  // lane lr's row: Q as the B operand of S^T = K Q^T
+  const RowAt at = row_at(p, b, hkv, g, lr < n_rows ? lr : 0);
+  const bool row_ok = lr < n_rows && (prefix_of(p) || at.t < tokens);
+  const int kmax = prefix_of(p) ? INT_MAX : p0 + at.t;  // last key the row may see
+  u32x4 qr[NS];
+  {
+    const uint16_t* qrow = p.q + ((static_cast<int64_t>(at.b) * p.T + at.t) * p.Hq + at.hq) * D;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) qr[s] = *reinterpret_cast<const u32x4*>(qrow + 32 * s + 8 * lq);
+  }
+  if (n_step > 0) load(p.vc, 0, lds0 + STAGE, 2);
+  bf16x8 qf[NS];
+#pragma unroll
+  for (int s = 0; s < NS; ++s) qf[s] = __builtin_bit_cast(bf16x8, row_ok ? qr[s] : u32x4{0u, 0u, 0u, 0u});
+
+  float m = -FLT_MAX, l = 0.0f;  // running max (log2 units) and this lane's share of the sum
+  f32x4 o[NJ];
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) o[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int i = 0; i < n_step; ++i) {
+    const int kb = k_lo + KS * i;
+    const bool more = i + 1 < n_step;
+    if (more && i + 1 - page0 >= 64) load_pages(i + 1);
+    asm volatile("s_waitcnt vmcnt(%0)" : : "n"(LD) : "memory");  // K is there, V may be on its way
+    // S^T = K Q^T: lane (r, q) holds keys 16 kt + 4 q + e of row r
+    f32x4 sc[KT];
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) {
+      f32x4 a = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int s = 0; s < NS; ++s)
+        a = mfma16(*reinterpret_cast<const bf16x8*>(ks + (16 * kt + lr) * (D * 2) + ((4 * s + lq) ^ (lr & 7)) * 16), qf[s], a);
+      sc[kt] = a;
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");  // K is read
+    if (more) load(p.kc, i + 1, lds0, 1);
+
+    float mb = -INFINITY;
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int key = kb + 16 * kt + 4 * lq + e;
+        if (!(key <= kmax && key < k_hi)) sc[kt][e] = -INFINITY;
+        mb = fmaxf(mb, sc[kt][e]);
+      }
+    mb = rows_max(mb) * p.scale_log2;
+    // the max is raised only when a row's grows by more than 8 (P stays below 2^8): most steps rescale nothing
+    if (__builtin_amdgcn_ballot_w64(mb > m + 8.0f) != 0) {
+      const float m_new = fmaxf(m, mb);
+      const float alpha = __builtin_amdgcn_exp2f(m - m_new);
+      m = m_new;
+      l *= alpha;
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) o[j] *= alpha;
+    }
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        sc[kt][e] = __builtin_amdgcn_exp2f(fmaf(sc[kt][e], p.scale_log2, -m));
+        l += sc[kt][e];
+      }
+    if (more) asm volatile("s_waitcnt vmcnt(%0)" : : "n"(LD) : "memory");  // V is there, the next K on its way
+    else asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+    // O^T += V^T P^T: P (as bf16) in the accumulators' own lanes, V^T by transposed LDS reads of
+    // keys 4 q .. 4 q + 3 (lane r: key 4 q + r / 4, dims 16 j + 4 (r % 4) ..)
+    const int key = 4 * lq + (lr >> 2);
+    const unsigned char* va = vs + key * (D * 2) + 16 * ((lr & 3) >> 1) + 8 * (lr & 1);
+    const int twist = 32 * (key & 7);
+    auto v_read = [&](int j, int kt) {
+      return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(va + kt * 16 * (D * 2) + ((32 * j) ^ twist)));
+    };
+    if constexpr (KT == 1) {
+      const i16x4 pb = __builtin_bit_cast(i16x4, u32x2{pk_bf16(sc[0][0], sc[0][1]), pk_bf16(sc[0][2], sc[0][3])});
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) o[j] = mfma16k16(v_read(j, 0), pb, o[j]);
+    } else {
+      const bf16x8 pb = __builtin_bit_cast(bf16x8, u32x4{pk_bf16(sc[0][0], sc[0][1]), pk_bf16(sc[0][2], sc[0][3]),
+                                                         pk_bf16(sc[1][0], sc[1][1]), pk_bf16(sc[1][2], sc[1][3])});
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+        o[j] = mfma16(__builtin_bit_cast(bf16x8, i16x8(__builtin_shufflevector(v_read(j, 0), v_read(j, 1), 0, 1, 2, 3, 4, 5, 6, 7))),
+                      pb, o[j]);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");  // V is read
+    if (more) load(p.vc, i + 1, lds0 + STAGE, 2);
+  }
+  l = rows_sum(l);
+
+  // the waves' states merge: thread (row, column piece)
+  __syncthreads();
+  float* Os = reinterpret_cast<float*>(smem);  // [W][16][D]
+  float* Ms = Os + W * 16 * D;                 // [W][16]
+  float* Ls = Ms + W * 16;
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) *reinterpret_cast<f32x4*>(&Os[(wave * 16 + lr) * D + 16 * j + 4 * lq]) = o[j];
+  if (lq == 0) {
+    Ms[wave * 16 + lr] = m;
+    Ls[wave * 16 + lr] = l;
+  }
+  __syncthreads();
+  constexpr int CW = D / (4 * W);  // columns per thread, in pieces of 4, 16 W apart
+  static_assert(CW % 4 == 0, "whole pieces");
+  const int mr = threadIdx.x / (4 * W), c0 = (threadIdx.x % (4 * W)) * 4;
+  if (mr >= n_rows) return;
+  const RowAt mat = row_at(p, b, hkv, g, mr);
+  if (!prefix_of(p) && mat.t >= tokens) {  // a padded token
+    if (p.n_split == 1) {
+#pragma unroll
+      for (int c = 0; c < CW / 4; ++c) store_zero4<D>(p, mat.b, mat.t, mat.hq, c0 + 16 * W * c);
+    }
+    return;
+  }
+  float ms = -FLT_MAX, mw[W], ls = 0.0f;
+#pragma unroll
+  for (int w = 0; w < W; ++w) ms = fmaxf(ms, Ms[w * 16 + mr]);
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    mw[w] = __builtin_amdgcn_exp2f(Ms[w * 16 + mr] - ms);
+    ls += mw[w] * Ls[w * 16 + mr];
+  }
+  f32x4 acc[CW / 4];
+#pragma unroll
+  for (int c = 0; c < CW / 4; ++c) {
+    acc[c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int w = 0; w < W; ++w)
+      acc[c] += mw[w] * *reinterpret_cast<const f32x4*>(&Os[(w * 16 + mr) * D + c0 + 16 * W * c]);
+  }
+  if (p.n_split == 1) {
+    store_row<D, CW / 4, 16 * W>(p, mat, c0, acc, ls);
+    return;
+  }
+  const int64_t pr = part_row(p, mat.b, hkv, mat.row) + split_at(p, split);
+#pragma unroll
+  for (int c = 0; c < CW / 4; ++c) *reinterpret_cast<f32x4*>(p.part + pr * D + c0 + 16 * W * c) = acc[c];
+  if (c0 == 0) {
+    const int64_t n_part = static_cast<int64_t>(p.B) * p.Hkv * p.rows_pad * p.n_split;
+    p.part[n_part * D + pr] = ms;
+    p.part[n_part * (D + 1) + pr] = ls;
+  }
+}
+
+template <int D>
+constexpr int step_threads() { return D == 256 ? 512 : 256; }
+
+template <int D>
+__global__ __launch_bounds__(step_threads<D>()) void attn_step_kernel(const StepParams p) {
+  constexpr int KG = D == 256 ? 2 : 1, W = step_threads<D>() / 64;
+  constexpr int kTile = tile_lds<D, KG, PagedParams>(), kRows = rows_lds<D, W>();
+  __shared__ __align__(128) unsigned char smem[kTile > kRows ? kTile : kRows];
+  // (kv-head, range) pairs run fastest, so that the row tiles that read a range's keys run on one XCD where
+  // the pairs are a multiple of the eight, and its L2 reads them once
+  PagedParams r = p;
+  int i = blockIdx.x;
+  const int n_prefix = p.Hkv * p.n_prefix * max(p.prefix_tiles, 1);
+  r.prefix = i < n_prefix;
+  if (!r.prefix) i -= n_prefix;
+  r.split0 = r.prefix ? 0 : p.n_prefix;
+  r.split_len = r.prefix ? p.len_prefix : p.len_own;
+  const int tiles = r.prefix ? p.prefix_tiles : p.own_tiles;
+  const int pairs = p.Hkv * (r.prefix ? p.n_prefix : p.n_own);
+  const int tb = i / pairs, hs = i - tb * pairs;
+  const int split = hs / p.Hkv, hkv = hs - split * p.Hkv;
+  const int batch = r.prefix ? 1 : p.B;
+  const int tile = tb / batch, b = tb - tile * batch;
+  if (tiles == 0) attn_rows<D, W>(r, smem, b, hkv, split);
+  else attn_tile<D, KG>(r, smem, b, hkv, tiles - 1 - tile, split);  // longest key ranges first
+}
+
+// One wave per (token, q-head): its ranges' partial results merged, as
+// attn_combine_kernel does, and a padded token's zeros.  The first NB ranges'
+// sums, the gate and all maxima are loaded before any is used: the launch is a
+// few memory latencies long.  A range without a key of the row (l = 0) may not
+// have written its sums: they are loaded all the same and dropped.
+template <int D>
+__global__ __launch_bounds__(256) void step_combine_kernel(const PagedParams p) {
+  constexpr int EPL = D / 64, NB = 8;
+  typedef float vec __attribute__((ext_vector_type(EPL)));
+  typedef uint16_t hvec __attribute__((ext_vector_type(EPL)));
+  const int lane = threadIdx.x & 63;
+  const int item = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  const int g = p.Hq / p.Hkv;
+  const int bt = item / p.Hq, hq = item - bt * p.Hq;
+  const int b = bt / p.T, t = bt - b * p.T;
+  if (b >= p.B) return;
+  const int64_t n_part = static_cast<int64_t>(p.B) * p.Hkv * p.rows_pad * p.n_split;
+  const int64_t pr = part_row(p, b, hq / g, t * g + hq % g);
+  const float* pm = p.part + n_part * D + pr;
+  const float* pl = p.part + n_part * (D + 1) + pr;
+  uint16_t* out = p.out + (static_cast<int64_t>(bt) * p.Hq + hq) * D + EPL * lane;
+  hvec gate = {};
+  if (p.qg != nullptr) gate = *reinterpret_cast<const hvec*>(p.qg + bt * p.qg_ld + hq * 2 * D + D + EPL * lane);
+  const int tokens = row_tokens(p, b);
+  vec acc = {}, v[NB];
+  float m = -FLT_MAX, lsum = 0.0f;
+  for (int s0 = 0; s0 < p.n_split; s0 += 64) {
+    const int n = min(64, p.n_split - s0);
+    const float ls = pl[s0 + min(lane, n - 1)], ms = pm[s0 + min(lane, n - 1)];
+    auto load = [&](int s) {
+#pragma unroll
+      for (int i = 0; i < NB; ++i)
+        v[i] = *reinterpret_cast<const vec*>(p.part + (pr + s0 + min(s + i, n - 1)) * D + EPL * lane);
+    };
+    load(0);
+    const bool has = lane < n && ls != 0.0f;
+    const float m_new = fmaxf(m, wave_max(has ? ms : -FLT_MAX));
+    const float keep = __builtin_amdgcn_exp2f(m - m_new);
+    m = m_new;
+    const float w = has ? __builtin_amdgcn_exp2f(ms - m) : 0.0f;  // the lane's range
+    acc *= keep;
+    lsum = lsum * keep + wave_sum(has ? w * ls : 0.0f);
+    for (int s = 0; s < n; s += NB) {
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        const float wi = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), min(s + i, 63)));
+        if (s + i < n && wi != 0.0f) acc += wi * v[i];  // wave-uniform
+      }
+      if (s + NB < n) load(s + NB);
+    }
+  }
+  const float inv_l = 1.0f / lsum;  // (0: every score is -inf, whose softmax is NaN)
+  hvec y;
+#pragma unroll
+  for (int e = 0; e < EPL; ++e) {
+    float x = lsum == 0.0f ? __builtin_nanf("") : acc[e] * inv_l;
+    if (p.qg != nullptr) x *= sigmoid(bf16_to_f32(gate[e]));
+    y[e] = f32_to_bf16(x);
+  }
+  *reinterpret_cast<hvec*>(out) = t < tokens ? y : hvec{};
+}
+
 int lg2(int64_t x) {  // of a power of two, else -1
   return x > 0 && (x & (x - 1)) == 0 ? __builtin_ctzll(static_cast<uint64_t>(x)) : -1;
 }
@@ -465,14 +775,14 @@ extern "C" int gdn_paged_attn(const void* q, const void* qg, int64_t qg_ld, cons
       !gdn_host::aligned(out, 8) || (qg && (!gdn_host::aligned(qg, 8) || qg_ld % 4 != 0)))
     return fail(GDN_ERR_INVALID, "gdn_paged_attn: misaligned pointer");
   const int64_t g = Hq / Hkv, rows = T * g, n_split = n_prefix + n_own;
-  if (B > 65535 || Hkv > 65535 || (B * rows + PR - 1) / PR > 65535 || Hkv * n_split > INT32_MAX ||
+  if (B > 65535 || B * T * Hq > INT32_MAX / 2 || Hkv * n_split > INT32_MAX ||
       B * Hkv * rows * n_split * (D + 2) > (int64_t(1) << 40))
     return fail(GDN_ERR_UNSUPPORTED, "gdn_paged_attn: problem too large");
   const size_t need = gdn_paged_attn_workspace_bytes(B, T, Hq, Hkv, D, n_split);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need || !gdn_host::aligned(workspace, 16)))
     return fail(GDN_ERR_INVALID, "gdn_paged_attn: workspace of %zu bytes is below the %zu needed for %lld key ranges",
                 workspace_bytes, need, (long long)n_split);
-  PagedParams p;
+  StepParams p;
   p.q = static_cast<const uint16_t*>(q);
   p.qg = static_cast<const uint16_t*>(qg);
   p.qg_ld = qg_ld;
@@ -495,32 +805,25 @@ extern "C" int gdn_paged_attn(const void* q, const void* qg, int64_t qg_ld, cons
   p.lg = lg;
   p.n_blocks = static_cast<int>(n_blocks);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  auto launch = [&](int64_t tile_rows, int64_t batch, int64_t keys_lo, int64_t keys_hi, int64_t n, int64_t split0) {
-    p.key0 = static_cast<int>(n_prefix > 0 ? shared * block : 0);
-    p.prefix = n_prefix > 0 && split0 == 0;
-    p.split0 = static_cast<int>(split0);
-    p.split_len = static_cast<int>(((keys_hi - keys_lo + n - 1) / n + KB - 1) / KB * KB);
-    if (tile_rows <= 16) {
-      const dim3 grid(static_cast<unsigned>(n), static_cast<unsigned>(Hkv), static_cast<unsigned>(batch));
-      if (D == 256) hipLaunchKernelGGL((attn_fwd_kernel<256, 1, PagedParams>), grid, dim3(256), 0, st, p);
-      else hipLaunchKernelGGL((attn_fwd_kernel<128, 1, PagedParams>), grid, dim3(256), 0, st, p);
-    } else {
-      const int64_t tiles = (tile_rows + PR - 1) / PR;
-      const dim3 grid(static_cast<unsigned>(Hkv * n), static_cast<unsigned>(tiles), static_cast<unsigned>(batch));
-      if (D == 256) hipLaunchKernelGGL((attn_prefill_kernel<256, 2, PagedParams>), grid, dim3(512), 0, st, p);
-      else hipLaunchKernelGGL((attn_prefill_kernel<128, 1, PagedParams>), grid, dim3(256), 0, st, p);
-    }
-    return gdn_host::check_launch("gdn_paged_attn");
-  };
-  const int64_t key0 = n_prefix > 0 ? shared * block : 0;
-  if (n_prefix > 0) {
-    const int rc = launch(B * rows, 1, 0, key0, n_prefix, 0);
-    if (rc != GDN_OK) return rc;
-  }
-  const int rc = launch(rows, B, key0, kv_len_max, n_own, n_prefix);
+  p.key0 = static_cast<int>(n_prefix > 0 ? shared * block : 0);
+  p.reread = n_prefix == 0 && shared > 0;
+  auto range_len = [](int64_t keys, int64_t n) { return static_cast<int>(((keys + n - 1) / n + KB - 1) / KB * KB); };
+  p.n_prefix = static_cast<int>(n_prefix);
+  p.n_own = static_cast<int>(n_own);
+  p.len_prefix = n_prefix > 0 ? range_len(p.key0, n_prefix) : 0;
+  p.len_own = range_len(kv_len_max - p.key0, n_own);
+  auto tiles_of = [](int64_t n) { return static_cast<int>(n <= 16 ? 0 : (n + PR - 1) / PR); };
+  p.prefix_tiles = n_prefix > 0 ? tiles_of(B * rows) : 0;
+  p.own_tiles = tiles_of(rows);
+  const int64_t groups = Hkv * (n_prefix * (p.prefix_tiles > 1 ? p.prefix_tiles : 1) +
+                                B * n_own * (p.own_tiles > 1 ? p.own_tiles : 1));
+  if (groups > INT32_MAX) return fail(GDN_ERR_UNSUPPORTED, "gdn_paged_attn: problem too large");
+  if (D == 256) hipLaunchKernelGGL(attn_step_kernel<256>, dim3(static_cast<unsigned>(groups)), dim3(512), 0, st, p);
+  else hipLaunchKernelGGL(attn_step_kernel<128>, dim3(static_cast<unsigned>(groups)), dim3(256), 0, st, p);
+  const int rc = gdn_host::check_launch("gdn_paged_attn");
   if (rc != GDN_OK || n_split == 1) return rc;
-  const dim3 cgrid(static_cast<unsigned>((B * Hkv * rows + 3) / 4));
-  if (D == 256) hipLaunchKernelGGL((attn_combine_kernel<256, PagedParams>), cgrid, dim3(256), 0, st, p);
-  else hipLaunchKernelGGL((attn_combine_kernel<128, PagedParams>), cgrid, dim3(256), 0, st, p);
+  const dim3 cgrid(static_cast<unsigned>((B * T * Hq + 3) / 4));
+  if (D == 256) hipLaunchKernelGGL(step_combine_kernel<256>, cgrid, dim3(256), 0, st, p);
+  else hipLaunchKernelGGL(step_combine_kernel<128>, cgrid, dim3(256), 0, st, p);
   return gdn_host::check_launch("gdn_paged_attn/combine");
 }
