@@ -189,10 +189,10 @@ __device__ __forceinline__ void store_out4(const AttnParams& p, int b, int t, in
 
 // A lane's N pieces of 4 of one output row, STEP columns apart: o / l times the gate, whose loads are all
 // issued before the first is used.  (l = 0: every score is -inf, whose softmax is NaN.)
+// `row` is the row of out: token times Hq plus head.
 template <int D, int N, int STEP>
-__device__ __forceinline__ void store_row(const AttnParams& p, const RowAt& at, int d, const f32x4* o, float l) {
-  const int64_t bt = static_cast<int64_t>(at.b) * p.T + at.t;
-  uint16_t* out = p.out + (bt * p.Hq + at.hq) * D + d;
+__device__ __forceinline__ void store_row(const AttnParams& p, int row, int d, const f32x4* o, float l) {
+  uint16_t* out = p.out + static_cast<int64_t>(row) * D + d;
   const float inv_l = 1.0f / l;
   if (p.qg == nullptr) {
 #pragma unroll
@@ -202,10 +202,11 @@ __device__ __forceinline__ void store_row(const AttnParams& p, const RowAt& at, 
     }
     return;
   }
+  const int bt = row / p.Hq, hq = row - bt * p.Hq;
+  const uint16_t* qg = p.qg + bt * p.qg_ld + hq * 2 * D + D + d;
   u32x2 gate[N];
 #pragma unroll
-  for (int n = 0; n < N; ++n)
-    gate[n] = *reinterpret_cast<const u32x2*>(p.qg + bt * p.qg_ld + at.hq * 2 * D + D + d + STEP * n);
+  for (int n = 0; n < N; ++n) gate[n] = *reinterpret_cast<const u32x2*>(qg + STEP * n);
 #pragma unroll
   for (int n = 0; n < N; ++n) {
     f32x4 y = o[n] * inv_l;
@@ -563,7 +564,8 @@ template <int KG, class P>
 constexpr int q_lds_steps() { return KG == 2 ? (P::kPaged ? 3 : 2) : 0; }
 template <int D, int KG, class P>
 constexpr int tile_lds() {
-  return 2 * (KB * D * 2 + D * VTP * 2) + (KG == 2 ? 8 * 128 * 4 : 0) + 4 * 2 * q_lds_steps<KG, P>() * 1024;
+  return 2 * (KB * D * 2 + D * VTP * 2) + (KG == 2 ? 8 * 128 * 4 : 0) + 4 * 2 * q_lds_steps<KG, P>() * 1024 +
+         (P::kPaged ? 3 * PR * 4 : 0);
 }
 
 // Tile rb of kv-head hkv's rows of batch entry b over key range `split`, by 256 * KG threads with
@@ -585,7 +587,8 @@ __device__ __forceinline__ void attn_tile(const P& p, unsigned char* smem, int b
 
   constexpr int QL = q_lds_steps<KG, P>();
   constexpr int kMl = KG == 2 ? 8 * 128 * 4 : 0;  // the waves' (m, l) for the merge
-  static_assert(tile_lds<D, KG, P>() == 2 * (KSTAGE + VSTAGE) + kMl + 4 * 2 * QL * 1024, "LDS layout");
+  static_assert(tile_lds<D, KG, P>() == 2 * (KSTAGE + VSTAGE) + kMl + 4 * 2 * QL * 1024 + (P::kPaged ? 3 * PR * 4 : 0),
+                "LDS layout");
 
   const int g = p.Hq / p.Hkv;
   const int n_rows = tile_rows(p, g);
@@ -611,17 +614,39 @@ __device__ __forceinline__ void attn_tile(const P& p, unsigned char* smem, int b
   };
   int kmax[2];
   bf16x8 qf[2][NS - QL];
+  // The paged form's rows, once per workgroup (several divisions each): their row of q and out (-1: none), the
+  // last key they may see (-1: none, a padded token) and their row of the partial results.
+  int* row_out = reinterpret_cast<int*>(smem + tile_lds<D, KG, P>()) - 3 * PR;
+  int* row_kmax = row_out + PR;
+  int* row_part = row_kmax + PR;
+  auto find_rows = [&]() {
+    if (tid < PR) {
+      const int r = row0 + tid;
+      const RowAt at = row_at(p, b, hkv, g, min(r, n_rows - 1));
+      row_out[tid] = r < n_rows ? (at.b * p.T + at.t) * p.Hq + at.hq : -1;
+      row_kmax[tid] = r < n_rows && (prefix_of(p) || at.t < tokens) ? (prefix_of(p) ? INT_MAX : p0 + at.t) : -1;
+      row_part[tid] = (at.b * p.Hkv + hkv) * p.rows_pad + at.row;
+    }
+  };
   auto load_q = [&]() {
     u32x4 v[2][NS];
     bool ok[2];
 #pragma unroll
     for (int rt = 0; rt < 2; ++rt) {
-      const int r = row0 + 32 * rg + 16 * rt + lr;
-      const RowAt at = row_at(p, b, hkv, g, min(r, n_rows - 1));
-      ok[rt] = r < n_rows && (!P::kPaged || prefix_of(p) || at.t < tokens);
-      const int hq = P::kPaged || ok[rt] ? at.hq : hkv * g;
-      kmax[rt] = prefix_of(p) ? INT_MAX : p0 + at.t;
-      const uint16_t* qrow = p.q + ((static_cast<int64_t>(at.b) * p.T + at.t) * p.Hq + hq) * D;
+      const uint16_t* qrow;
+      if constexpr (P::kPaged) {
+        const int r = 32 * rg + 16 * rt + lr;
+        kmax[rt] = row_kmax[r];
+        ok[rt] = kmax[rt] >= 0;
+        qrow = p.q + static_cast<int64_t>(max(row_out[r], 0)) * D;
+      } else {
+        const int r = row0 + 32 * rg + 16 * rt + lr;
+        const RowAt at = row_at(p, b, hkv, g, min(r, n_rows - 1));
+        ok[rt] = r < n_rows;
+        const int hq = ok[rt] ? at.hq : hkv * g;
+        kmax[rt] = p0 + at.t;
+        qrow = p.q + ((static_cast<int64_t>(at.b) * p.T + at.t) * p.Hq + hq) * D;
+      }
 #pragma unroll
       for (int s = 0; s < NS; ++s) v[rt][s] = *reinterpret_cast<const u32x4*>(qrow + 32 * s + 8 * lq);
     }
@@ -720,6 +745,10 @@ __device__ __forceinline__ void attn_tile(const P& p, unsigned char* smem, int b
   auto publish = [&]() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(4 * VPAIRS) : "memory");
   };
+  if (P::kPaged && nblk == 0) {
+    find_rows();
+    __syncthreads();
+  }
   if (nblk > 0) {
     if constexpr (P::kPaged) load_pages(0);
     const int nb = block_bytes(k_lo);
@@ -734,7 +763,11 @@ __device__ __forceinline__ void attn_tile(const P& p, unsigned char* smem, int b
 #pragma unroll
       for (int e = 0; e < 4; ++e) v_load(vrs, i, e);
     }
-    if constexpr (P::kPaged) load_q();  // behind the first keys' loads: one latency for both
+    if constexpr (P::kPaged) {  // behind the first keys' loads: one latency for both
+      find_rows();
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory");
+      load_q();
+    }
 #pragma unroll
     for (int i = 0; i < VPAIRS; ++i) {
 #pragma unroll
@@ -888,29 +921,28 @@ __device__ __forceinline__ void attn_tile(const P& p, unsigned char* smem, int b
   // row tile rt's state (lane (r, q): O[row r][16 j + 4 q + i]) to the output, or to the split's partials
   auto store_tile = [&](auto rtc) {
     constexpr int rt = decltype(rtc)::value;
+    if constexpr (P::kPaged) {
+      const int r = 32 * rg + 16 * rt + lr;
+      if (row_out[r] < 0) return;
+      if (row_kmax[r] >= 0) {
+        store_row<D, NJ, 16>(p, row_out[r], 4 * lq, o[rt], lt[rt]);
+      } else {  // a padded token
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+          *reinterpret_cast<u32x2*>(p.out + static_cast<int64_t>(row_out[r]) * D + 16 * j + 4 * lq) = u32x2{0u, 0u};
+      }
+      return;
+    }
     const int r = row0 + 32 * rg + 16 * rt + lr;
     if (r >= n_rows) return;
     const RowAt at = row_at(p, b, hkv, g, r);
-    if constexpr (P::kPaged) {
-      if (!prefix_of(p) && at.t >= tokens) {  // a padded token
-        if (p.n_split == 1) {
-#pragma unroll
-          for (int j = 0; j < NJ; ++j) store_zero4<D>(p, b, at.t, at.hq, 16 * j + 4 * lq);
-        }
-        return;
-      }
-    }
-    if (P::kPaged && p.n_split == 1) {
-      store_row<D, NJ, 16>(p, at, 4 * lq, o[rt], lt[rt]);
-      return;
-    }
     if (p.n_split == 1) {
       const float inv_l = 1.0f / lt[rt];  // (l = 0: every score is -inf, whose softmax is NaN)
 #pragma unroll
       for (int j = 0; j < NJ; ++j) store_out4<D>(p, b, at.t, at.hq, 16 * j + 4 * lq, o[rt][j], inv_l);
       return;
     }
-    const int64_t pr = part_row(p, at.b, hkv, at.row) + split_at(p, split);
+    const int64_t pr = part_row(p, b, hkv, r) + split;
     const int64_t n_part = static_cast<int64_t>(p.B) * p.Hkv * p.rows_pad * p.n_split;
     if (lq == 0) {
       p.part[n_part * D + pr] = m[rt];
@@ -920,16 +952,14 @@ __device__ __forceinline__ void attn_tile(const P& p, unsigned char* smem, int b
 #pragma unroll
     for (int j = 0; j < NJ; ++j) *reinterpret_cast<f32x4*>(p.part + pr * D + 16 * j + 4 * lq) = o[rt][j];
   };
-  // The paged form's partial results go out in whole rows, through the wave's 64 D bytes of LDS at `at`: the
-  // accumulators' own layout would write 64 bytes of a row at a time, at a fifth of the rate (128 rows of 256:
-  // TODO against TODO us).
+  // The paged form's partial results go out in whole rows, through the wave's 64 D bytes of LDS at `buf`: the
+  // accumulators' own layout would write 64 bytes of a row at a time (128 rows of 256: 4.5 us, this way 2.7).
   auto store_part = [&](auto rtc, unsigned char* buf) {
     constexpr int rt = decltype(rtc)::value;
     constexpr int G = D / 4;  // 16-byte granules of a row, XOR-swizzled by the row
-    const int r = row0 + 32 * rg + 16 * rt + lr;
-    const RowAt at = row_at(p, b, hkv, g, min(r, n_rows - 1));
-    const bool ok = r < n_rows && (prefix_of(p) || at.t < tokens);
-    const int64_t pr = part_row(p, at.b, hkv, at.row) + split_at(p, split);
+    const int r = 32 * rg + 16 * rt + lr;
+    const bool ok = row_kmax[r] >= 0;
+    const int64_t pr = static_cast<int64_t>(row_part[r]) * p.n_split + split_at(p, split);
     if (ok && lq == 0) {
       const int64_t n_part = static_cast<int64_t>(p.B) * p.Hkv * p.rows_pad * p.n_split;
       p.part[n_part * D + pr] = m[rt];
@@ -939,14 +969,27 @@ __device__ __forceinline__ void attn_tile(const P& p, unsigned char* smem, int b
     f32x4* cell = reinterpret_cast<f32x4*>(buf);
 #pragma unroll
     for (int j = 0; j < NJ; ++j) cell[lr * G + ((4 * j + lq) ^ lr)] = o[rt][j];
-    const uint64_t rows = __builtin_amdgcn_ballot_w64(ok);
+    const uint32_t rows = static_cast<uint32_t>(__builtin_amdgcn_ballot_w64(ok));
+    auto to = [&](int n) {  // lane n's row
+      const int64_t at = static_cast<int64_t>(__builtin_amdgcn_readlane(static_cast<int>(pr >> 32), n)) << 32 |
+                         static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(pr), n));
+      return p.part + at * D;
+    };
+    if constexpr (G == 64) {
 #pragma unroll
-    for (int n = 0; n < 16; n += 64 / G) {
-      const int row = n + lane / G, col = lane % G;
-      const f32x4 x = cell[row * G + (col ^ row)];
-      const int64_t at_row = static_cast<int64_t>(__shfl(static_cast<int>(pr >> 32), row, 64)) << 32 |
-                             static_cast<uint32_t>(__shfl(static_cast<int>(pr), row, 64));
-      if ((rows >> row) & 1) *reinterpret_cast<f32x4*>(p.part + at_row * D + 4 * col) = x;
+      for (int n = 0; n < 16; ++n) {
+        const f32x4 x = cell[n * G + (lane ^ n)];
+        if ((rows >> n) & 1) *reinterpret_cast<f32x4*>(to(n) + 4 * lane) = x;
+      }
+    } else {
+      static_assert(G == 32, "two rows at a time");
+      const int hi = lane >> 5, col = lane & 31;
+#pragma unroll
+      for (int n = 0; n < 16; n += 2) {
+        const f32x4 x = cell[(n + hi) * G + (col ^ (n + hi))];
+        float* row = hi ? to(n + 1) : to(n);
+        if ((rows >> (n + hi)) & 1) *reinterpret_cast<f32x4*>(row + 4 * col) = x;
+      }
     }
   };
   if constexpr (KG == 1) {

@@ -338,12 +338,16 @@ struct StepParams : PagedParams {
 // range `split`, by W waves.  Every wave takes 16 KT keys of a step of 16 KT W and
 // keeps a softmax state of its own; nothing in the loop waits for another wave.
 // K and V go to the wave's own 16 KB of LDS by direct loads of whole rows (K as
-// fragments from memory, 64 bytes of a row at a time, took the cold cache's read
-// from TODO to TODO TB/s), their 16-byte granules swizzled on the way: K's by
-// (key & 7), so that 16-byte fragment reads of 8 keys hit distinct banks, V's by
-// 2 (key & 7), so that its transposed reads of 4 x 4 keys do.  K of the next step
-// is asked for as soon as this one's scores are formed, V as soon as its products
-// are: a CU has up to 128 KB in flight.
+// fragments from memory, 64 bytes of a row at a time, took 1.6 times as long from
+// a warm cache), their 16-byte granules swizzled on the way: K's by (key & 7), so
+// that 16-byte fragment reads of 8 keys hit distinct banks, V's by 2 (key & 7), so
+// that its transposed reads of 4 x 4 keys do.  K of the next step is asked for as
+// soon as this one's scores are formed, V as soon as its products are: a CU has up
+// to 128 KB in flight.  Bound by memory: a full cache of 64 rows of 4096 keys at 4
+// kv-heads of 256 (1.07 GB) takes 164 us, 6.6 TB/s (without the hint that the keys
+// are read once 186).
+// Tiles of 32 rows in the same way (O and Q in 192 registers) were within 10% of
+// attn_tile either way at 17 to 32 rows and slower beyond.
 template <int D, int W>
 constexpr int rows_lds() {
   constexpr int kv = W * 2 * 256 * 16 * 2, merge = W * 16 * D * 4 + 2 * W * 16 * 4;
@@ -367,6 +371,7 @@ __device__ __forceinline__ void attn_rows(const PagedParams& p, unsigned char* s
   const int p0 = row_start(p, b, tokens);
   const KeyRange range = key_range(p, split, p0, tokens - 1, tokens > 0);
   const int k_lo = range.lo + KW * wave, k_hi = range.hi;  // this wave's keys: KW from k_lo, k_lo + KS, ..
+  const int k_free = prefix_of(p) ? k_hi : min(p0 + 1, k_hi);  // keys below this are visible to every row
   const int n_step = k_hi > k_lo ? (k_hi - k_lo + KS - 1) / KS : 0;
 
   // lane l holds the block of the wave's step page0 + l
@@ -438,15 +443,20 @@ __device__ __forceinline__ void attn_rows(const PagedParams& p, unsigned char* s
     asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");  // K is read
     if (more) load(p.kc, i + 1, lds0, 1);
 
+    if (kb + KW > k_free) {  // some row does not see them all
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int key = kb + 16 * kt + 4 * lq + e;
+          if (!(key <= kmax && key < k_hi)) sc[kt][e] = -INFINITY;
+        }
+    }
     float mb = -INFINITY;
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int key = kb + 16 * kt + 4 * lq + e;
-        if (!(key <= kmax && key < k_hi)) sc[kt][e] = -INFINITY;
-        mb = fmaxf(mb, sc[kt][e]);
-      }
+      for (int e = 0; e < 4; ++e) mb = fmaxf(mb, sc[kt][e]);
     mb = rows_max(mb) * p.scale_log2;
     // the max is raised only when a row's grows by more than 8 (P stays below 2^8): most steps rescale nothing
     if (__builtin_amdgcn_ballot_w64(mb > m + 8.0f) != 0) {
@@ -532,7 +542,7 @@ __device__ __forceinline__ void attn_rows(const PagedParams& p, unsigned char* s
       acc[c] += mw[w] * *reinterpret_cast<const f32x4*>(&Os[(w * 16 + mr) * D + c0 + 16 * W * c]);
   }
   if (p.n_split == 1) {
-    store_row<D, CW / 4, 16 * W>(p, mat, c0, acc, ls);
+    store_row<D, CW / 4, 16 * W>(p, (mat.b * p.T + mat.t) * p.Hq + mat.hq, c0, acc, ls);
     return;
   }
   const int64_t pr = part_row(p, mat.b, hkv, mat.row) + split_at(p, split);
