@@ -423,7 +423,8 @@ int gdn_attn_fwd(const void* q, const void* qg, int64_t qg_ld, const void* k_cac
  *            and free_blocks are written past held and n_free only.
  * All int32.  The first `shared` blocks of a row are never given back.
  * block: a power of two up to 2^20; table rows are table_ld apart; free_blocks
- * has room for n_blocks; B <= 4096; B * T and n_blocks * block below 2^31.
+ * has room for n_blocks; B <= 4096; B * T, n_blocks * block and B * table_ld
+ * below 2^31.
  */
 int gdn_paged_tables(const int32_t* lengths, const int32_t* n_new, int32_t* table, int64_t table_ld,
                      const int32_t* held, int32_t* free_blocks, const int32_t* n_free, int32_t* held_out,
@@ -443,8 +444,8 @@ int gdn_paged_tables(const int32_t* lengths, const int32_t* n_new, int32_t* tabl
  *            [0, n_blocks * block) is padding: its q is zeros, its k and v go
  *            nowhere.  NULL: row b's own block b (n_blocks == B), at pos0[b] + t
  *            clamped as in gdn_attn_qk: the dense cache [B,Hkv,cap,D].
- * Norm and rotation are in fp32 and rounded once.  D in {128, 256}; rot even, and
- * a multiple of D/32 for pairs (i, i + rot/2).  Slots are below 2^31.
+ * Norm and rotation are in fp32 and rounded once.  D in {128, 256}; rot even.
+ * Slots are below 2^31.
  */
 int gdn_attn_rope(const void* qg, int64_t qg_ld, int64_t q_head, const void* k_new, const void* v_new,
                   int64_t kv_ld, const void* q_norm_w, const void* k_norm_w, int w_dtype, float eps,

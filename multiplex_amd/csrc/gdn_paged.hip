@@ -27,9 +27,7 @@ struct TableParams {
   int B, T, table_ld, lg, shared, n_blocks;
 };
 
-constexpr int kTableRows = 4096;  // rows whose running sums a workgroup keeps in LDS
-
-__device__ __forceinline__ int32_t saturate(int64_t x) { return static_cast<int32_t>(min<int64_t>(x, INT32_MAX)); }
+constexpr int kTableRows = 4096, kTableThreads = 1024;
 
 // The last of n ascending entries that is not above x (entry 0 is not).
 __device__ __forceinline__ int last_not_above(const int32_t* at, int n, int x) {
@@ -42,134 +40,156 @@ __device__ __forceinline__ int last_not_above(const int32_t* at, int n, int x) {
   return lo;
 }
 
+// Inclusive sum over the lanes up to this one, by DPP moves: in rows of 16, then row 0's and
+// row 2's last lane to the row above, then lane 31's to the upper half.
+__device__ __forceinline__ int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);  // row_shr 1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, true);  // row_bcast 15, to rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, true);  // row_bcast 31, to rows 2 and 3
+  return x;
+}
+
 // Row b needs max(ceil((len + new) / block), shared) blocks.  Rows with more
 // give the last ones back, onto the free stack's top in row order, then rows
 // with fewer take from the top in row order, as far as the stack reaches: a row
 // that does not get all it asks for gets none, and no row after it any.
-// Every workgroup forms the running sums of all rows by itself and then takes
-// its share of the cells; a cell that one writes, none reads: blocks given back
-// in this call are taken from their giver's table, not from the stack.  State
-// that would be written over what other workgroups read (held_out = held) is
-// written by a launch of one workgroup (kState) behind the others (kCells).
+// Every workgroup forms the running sums of all rows by itself (PER rows a
+// thread) and then takes its share of the cells; a cell that one writes, none
+// reads: blocks given back in this call are taken from their giver's table, not
+// from the stack.  State that would be written over what other workgroups read
+// (held_out = held) is written by a launch of one workgroup (kState) behind the
+// others (kCells).
+// Bound by latency: the launch, the rows' loads, two barriers, and the table's or
+// the stack's loads, of which a thread's first is asked for before the sums
+// (256 rows of one token 6.2 us graph-replayed, 1000 of up to nine 8.1; the first
+// form, which formed a row anew wherever it was needed and summed in 64 bits, 9.5
+// and 10.7).
 constexpr int kCells = 1, kState = 2;
-__global__ __launch_bounds__(256) void tables_kernel(const TableParams p, int what) {
-  __shared__ int32_t back_at[kTableRows + 1], take_at[kTableRows + 1];
-  __shared__ int64_t wave_back[4], wave_take[4];
-  __shared__ int32_t wave_granted[4];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  struct Row {
-    int len, n, have, back, take;
-    bool fits;
-  };
-  auto row_of = [&](int b) {
-    Row r;
-    r.len = max(p.lengths[b], 0);
-    r.n = p.n_new != nullptr ? min(max(p.n_new[b], 0), p.T) : p.T;
-    r.have = min(max(p.held[b], 0), p.table_ld);
-    const int64_t need =
-        max<int64_t>((static_cast<int64_t>(r.len) + r.n + (int64_t(1) << p.lg) - 1) >> p.lg, p.shared);
-    r.fits = need <= p.table_ld;
-    const int want = r.fits ? static_cast<int>(need) : r.have;
-    r.back = max(r.have - want, 0);
-    r.take = max(want - r.have, 0);
-    return r;
-  };
+template <int PER>
+__global__ __launch_bounds__(kTableThreads) void tables_kernel(const TableParams p, int what) {
+  constexpr int NW = kTableThreads / 64;
+  // of each row: what goes before it, its blocks now and then, its length and (where served) new tokens
+  __shared__ int32_t back_at[PER * kTableThreads + 1], take_at[PER * kTableThreads + 1];
+  __shared__ int32_t row_have[PER * kTableThreads], row_want[PER * kTableThreads];
+  __shared__ int32_t row_len[PER * kTableThreads], row_new[PER * kTableThreads];
+  __shared__ int32_t wave_back[NW], wave_take[NW], wave_granted[NW];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t n_slots = static_cast<int64_t>(p.B) * p.T;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * kTableThreads + tid, step = gridDim.x * kTableThreads;
 
-  // running sums: thread tid has rows per * tid ..
-  const int per = (p.B + 255) / 256, b0 = min(per * tid, p.B), b1 = min(b0 + per, p.B);
-  int64_t back = 0, take = 0;
-  for (int b = b0; b < b1; ++b) {
-    const Row r = row_of(b);
-    back += r.back;
-    take += r.take;
-  }
-  int64_t back_sum = back, take_sum = take;
+  int len[PER], fresh[PER], have[PER], want[PER];
+  bool fits[PER];
 #pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const int64_t x = __shfl_up(back_sum, d, 64), y = __shfl_up(take_sum, d, 64);
-    if (lane >= d) {
+  for (int k = 0; k < PER; ++k) {
+    const int b = min(PER * tid + k, p.B - 1);
+    len[k] = p.lengths[b];
+    fresh[k] = p.n_new != nullptr ? p.n_new[b] : p.T;
+    have[k] = p.held[b];
+  }
+  const int n_free = min(max(p.n_free[0], 0), p.n_blocks);
+  // the block that the table lists now at the thread's first token, if it is one of the row's
+  int32_t first_block = 0;
+  if ((what & kCells) && first < n_slots && p.table_ld > 0) {
+    const int b = static_cast<int>(first / p.T), t = static_cast<int>(first - static_cast<int64_t>(b) * p.T);
+    const int64_t c = (static_cast<int64_t>(max(p.lengths[b], 0)) + t) >> p.lg;
+    first_block = p.table[static_cast<int64_t>(b) * p.table_ld + (c < p.table_ld ? c : p.table_ld - 1)];
+  }
+  int back = 0, take = 0;
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const bool row = PER * tid + k < p.B;
+    len[k] = max(len[k], 0);
+    fresh[k] = min(max(fresh[k], 0), p.T);
+    have[k] = row ? min(max(have[k], 0), p.table_ld) : 0;
+    const int64_t need =
+        max<int64_t>((static_cast<int64_t>(len[k]) + fresh[k] + (int64_t(1) << p.lg) - 1) >> p.lg, p.shared);
+    fits[k] = need <= p.table_ld;
+    want[k] = row && fits[k] ? static_cast<int>(need) : have[k];
+    back += max(have[k] - want[k], 0);
+    take += max(want[k] - have[k], 0);
+  }
+  const int back_incl = wave_scan(back), take_incl = wave_scan(take);
+  if (lane == 63) {
+    wave_back[wave] = back_incl;
+    wave_take[wave] = take_incl;
+  }
+  __syncthreads();
+  int back_sum = back_incl - back, take_sum = take_incl - take, all_back = 0;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) {
+    const int x = wave_back[w], y = wave_take[w];
+    if (w < wave) {
       back_sum += x;
       take_sum += y;
     }
+    all_back += x;
   }
-  if (lane == 63) {
-    wave_back[wave] = back_sum;
-    wave_take[wave] = take_sum;
-  }
-  __syncthreads();
-  int64_t all_back = 0;
+  const int top = static_cast<int>(min<int64_t>(static_cast<int64_t>(n_free) + all_back, INT32_MAX));
+  int granted = 0;  // blocks taken by the rows up to this thread's last that takes any
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    if (w < wave) {
-      back_sum += wave_back[w];
-      take_sum += wave_take[w];
+  for (int k = 0; k < PER; ++k) {
+    const int b = PER * tid + k, grow = max(want[k] - have[k], 0);
+    const bool served = fits[k] && (grow == 0 || take_sum + grow <= top);
+    if (!served) want[k] = have[k];
+    if (b < p.B) {
+      back_at[b] = back_sum;
+      take_at[b] = take_sum;
+      row_have[b] = have[k];
+      row_want[b] = want[k];
+      row_len[b] = len[k];
+      row_new[b] = served ? fresh[k] : 0;
     }
-    all_back += wave_back[w];
+    back_sum += max(have[k] - want[k], 0);
+    take_sum += grow;
+    if (served && grow > 0) granted = take_sum;
   }
-  const int n_free = min(max(p.n_free[0], 0), p.n_blocks);
-  const int top = saturate(n_free + all_back);
-  back = back_sum - back;
-  take = take_sum - take;
-  int granted = 0;
-  for (int b = b0; b < b1; ++b) {
-    const Row r = row_of(b);
-    back_at[b] = saturate(back);
-    take_at[b] = saturate(take);
-    back += r.back;
-    take += r.take;
-    if (r.take > 0 && take <= top) granted = static_cast<int>(take);
-  }
-  if (tid == 0) {
-    back_at[p.B] = saturate(all_back);
-    take_at[p.B] = INT32_MAX;
-  }
-#pragma unroll
-  for (int d = 32; d > 0; d /= 2) granted = max(granted, __shfl_xor(granted, d, 64));
-  if (lane == 0) wave_granted[wave] = granted;
+  const uint64_t takers = __builtin_amdgcn_ballot_w64(granted > 0);
+  if (lane == 0) wave_granted[wave] = 0;
+  if (takers != 0 && lane == 63 - __builtin_clzll(takers)) wave_granted[wave] = granted;
+  if (tid == 0) back_at[p.B] = all_back;
   __syncthreads();
-  granted = max(max(wave_granted[0], wave_granted[1]), max(wave_granted[2], wave_granted[3]));
+  granted = 0;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) granted = max(granted, wave_granted[w]);
 
   // the block given back u-th, and the one taken j-th
   auto given = [&](int u) {
     const int b = last_not_above(back_at, p.B, u);
-    const Row r = row_of(b);
-    const int c = r.have - r.back + u - back_at[b];
-    return p.table[static_cast<int64_t>(b) * p.table_ld + min(c, p.table_ld - 1)];
+    return p.table[static_cast<int64_t>(b) * p.table_ld + min(row_want[b] + u - back_at[b], p.table_ld - 1)];
   };
   auto taken = [&](int j) {
     const int s = max(top - 1 - j, 0);
     return s < n_free ? p.free[s] : given(s - n_free);
   };
-  auto served = [&](const Row& r, int b) { return r.fits && (r.take == 0 || take_at[b] + int64_t(r.take) <= top); };
-
-  const int first = blockIdx.x * 256 + tid, step = gridDim.x * 256;
   if (what & kCells) {
-    const int n_back = back_at[p.B];
-    for (int u = first; u < n_back && u < p.n_blocks - n_free; u += step) p.free[n_free + u] = given(u);
-    for (int j = first; j < granted; j += step) {
-      const int b = last_not_above(take_at, p.B, j);
-      p.table[static_cast<int64_t>(b) * p.table_ld + row_of(b).have + j - take_at[b]] = taken(j);
+    for (int64_t u = first; u < all_back && u < p.n_blocks - n_free; u += step) p.free[n_free + u] = given(static_cast<int>(u));
+    for (int64_t j = first; j < granted; j += step) {
+      const int b = last_not_above(take_at, p.B, static_cast<int>(j));
+      p.table[static_cast<int64_t>(b) * p.table_ld + row_have[b] + static_cast<int>(j) - take_at[b]] = taken(static_cast<int>(j));
     }
-    const int64_t n_slots = static_cast<int64_t>(p.B) * p.T;
     for (int64_t i = first; i < n_slots; i += step) {
       const int b = static_cast<int>(i / p.T), t = static_cast<int>(i - static_cast<int64_t>(b) * p.T);
-      const Row r = row_of(b);
       int32_t slot = -1;
-      if (t < r.n && served(r, b)) {
-        const int64_t pos = static_cast<int64_t>(r.len) + t;
-        const int c = static_cast<int>(pos >> p.lg);
-        const int32_t block = c < r.have ? p.table[static_cast<int64_t>(b) * p.table_ld + c] : taken(take_at[b] + c - r.have);
-        slot = static_cast<int32_t>(static_cast<uint32_t>(block) << p.lg) + static_cast<int32_t>(pos & ((1 << p.lg) - 1));
+      if (t < row_new[b]) {
+        const int64_t pos = static_cast<int64_t>(row_len[b]) + t;
+        const int c = static_cast<int>(pos >> p.lg), old = row_have[b];
+        const int32_t block = c >= old ? taken(take_at[b] + c - old)
+                              : i == first ? first_block
+                                           : p.table[static_cast<int64_t>(b) * p.table_ld + c];
+        slot = static_cast<int32_t>((static_cast<uint32_t>(block) << p.lg) + static_cast<uint32_t>(pos & ((1 << p.lg) - 1)));
       }
       p.slots[i] = slot;
     }
   }
   if ((what & kState) && blockIdx.x == 0) {
     __syncthreads();  // one workgroup may write over what it has read
-    for (int b = tid; b < p.B; b += 256) {
-      const Row r = row_of(b);
-      p.held_out[b] = served(r, b) ? r.have - r.back + r.take : r.have;
-    }
+#pragma unroll
+    for (int k = 0; k < PER; ++k)
+      if (PER * tid + k < p.B) p.held_out[PER * tid + k] = want[k];
     if (tid == 0) p.n_free_out[0] = top - granted;
   }
 }
@@ -193,51 +213,65 @@ struct RopeParams {
   int B, T, Hq, Hkv, q_head, block, rot;
   int64_t n_slots;  // n_blocks * block
   float eps, factor;
+  uint32_t per_tok;  // waves of a token: q_items + 2 kv_items
+  int q_items, kv_items;
 };
 
 // y = x / sqrt(mean(x^2) + eps) * w, its pairs turned by pos * turns[i] (a turn
-// is 2 pi) and stretched by factor; everything in fp32, rounded once.
-// One wave takes NH heads of one token (q heads, then k, then v): the angles
-// depend on the token and the lane only and serve all of them.  The angle is
-// exact at any position: pos * turns in 64-bit integers drops whole turns by
-// itself, where pos * frequency in fp32 is off by 0.06 rad at a million; its top
-// 32 bits go to the hardware's sine and cosine, which take turns.
-template <int D, int NH, bool IL>
+// is 2 pi) and stretched by factor; everything in fp32, rounded once.  With r the
+// norm's factor, each dim is y = r (A x + B x'), x' the other of its pair, A = w
+// cos and B = -+ w' sin: A and B serve every head of a token.
+// A wave takes NU groups of 512 / D heads of one token and one kind (q, k or v),
+// 8 dims a lane, x' by a load of its own (from the L1).  The angles are formed by
+// one lane a dim and handed round in LDS; they are exact at any position: pos *
+// turns in 64-bit integers drops whole turns by itself, where pos * frequency in
+// fp32 is off by 0.06 rad at a million, and its top 32 bits go to the hardware's
+// sine and cosine, which take turns.
+// Bound by memory and arithmetic together for many tokens (4096 tokens of 16 + 2 x
+// 4 heads of 256, 100 MB from a cold cache: 24.8 us, their plain copy 19; with 4
+// dims a lane, x' by a lane shuffle, each wave's angles by the lanes that use them
+// and a select per dim 35), by the launch and a few latencies for few (64 tokens
+// 3.6).  One / two / four / eight groups a wave, us: 340 tokens 5.0 / - / 5.5 / -;
+// 680 14.2 / 6.7 / 7.5 / 9.4; 4096 70 / 24.8 / 26.4 / 39.3.
+constexpr int kRopeGroups = 2;      // groups of a wave
+constexpr int64_t kRopeFew = 8192;  // heads of all tokens up to which a wave takes one
+template <int D, int NU, bool IL>
 __global__ __launch_bounds__(256) void attn_rope_kernel(const RopeParams p) {
-  constexpr int EPL = D / 64;  // elements per lane
-  typedef typename RowVec<EPL>::type vec;
+  constexpr int LPH = D / 8, HPU = 64 / LPH;  // lanes per head, heads per group
+  typedef typename RowVec<8>::type vec;
+  __shared__ __align__(16) float trig[4][2][D];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int heads = p.Hq + 2 * p.Hkv;
-  const uint32_t per_tok = (heads + NH - 1) / NH;
-  const uint32_t item = blockIdx.x * 4u + wave;
-  const uint32_t bt = item / per_tok;
+  const uint32_t bt = (blockIdx.x * 4u + wave) / p.per_tok;
   if (bt >= static_cast<uint32_t>(p.B) * p.T) return;  // wave-uniform
-  const int h0 = static_cast<int>(item - bt * per_tok) * NH;
+  int item = static_cast<int>(blockIdx.x * 4u + wave - bt * p.per_tok);
+  // q's, k's, then v's groups
+  const bool is_q = item < p.q_items, is_k = !is_q && item < p.q_items + p.kv_items;
+  if (!is_q) item -= is_k ? p.q_items : p.q_items + p.kv_items;
+  const int H = is_q ? p.Hq : p.Hkv;
   const int b = static_cast<int>(bt / p.T), t = static_cast<int>(bt - static_cast<uint32_t>(b) * p.T);
-  const int d0 = EPL * lane;
+  const int h0 = item * NU * HPU + lane / LPH, d0 = lane % LPH * 8;  // heads h0, h0 + HPU, ..
 
-  vec raw[NH];
+  const uint16_t* src = is_q ? p.qg + bt * p.qg_ld : (is_k ? p.kn : p.vn) + bt * p.kv_ld;
+  const int head_ld = is_q ? p.q_head : D;
+  const int half = p.rot / 2;
+  const bool turned = d0 < p.rot && (is_q || is_k), lower = d0 < half;
+  const bool whole = half % 8 == 0;  // a lane's 8 dims have their partners in one other lane's
+  vec raw[NU], other[NU];
 #pragma unroll
-  for (int n = 0; n < NH; ++n) {
-    const int h = min(h0 + n, heads - 1);
-    const uint16_t* src;
-    if (h < p.Hq) src = p.qg + bt * p.qg_ld + h * p.q_head;
-    else if (h < p.Hq + p.Hkv) src = p.kn + bt * p.kv_ld + (h - p.Hq) * D;
-    else src = p.vn + bt * p.kv_ld + (h - p.Hq - p.Hkv) * D;
-    raw[n] = *reinterpret_cast<const vec*>(src + d0);
-  }
-  const bool norm = p.qw != nullptr;
-  uint32_t qwr[EPL] = {}, kwr[EPL] = {};
-  if (norm) {
-#pragma unroll
-    for (int e = 0; e < EPL; ++e) {
-      if (p.wdt == GDN_DTYPE_F32) {
-        qwr[e] = static_cast<const uint32_t*>(p.qw)[d0 + e];
-        kwr[e] = static_cast<const uint32_t*>(p.kw)[d0 + e];
+  for (int n = 0; n < NU; ++n) {
+    const uint16_t* row = src + min(h0 + n * HPU, H - 1) * head_ld;
+    raw[n] = *reinterpret_cast<const vec*>(row + d0);
+    other[n] = raw[n];
+    if (!IL && turned) {
+      if (whole) {
+        other[n] = *reinterpret_cast<const vec*>(row + (lower ? d0 + half : d0 - half));
       } else {
-        qwr[e] = static_cast<const uint16_t*>(p.qw)[d0 + e];
-        kwr[e] = static_cast<const uint16_t*>(p.kw)[d0 + e];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int d = d0 + e;
+          other[n][e] = row[d < half ? d + half : d < p.rot ? d - half : d];
+        }
       }
     }
   }
@@ -254,74 +288,117 @@ __global__ __launch_bounds__(256) void attn_rope_kernel(const RopeParams p) {
     page = b;
     at = pos = static_cast<uint32_t>(first_pos(p.pos0, b, p.T, p.block)) + t;
   }
-
-  // sine and cosine of the lane's elements; the first of a pair takes -sine
-  const int half = p.rot / 2;
-  const bool lower = d0 < half;
-  const int partner = lower ? lane + half / EPL : lane - half / EPL;
-  float sn[EPL], cs[EPL];
+  uint16_t* dst = is_q ? p.q + static_cast<int64_t>(bt) * p.Hq * D
+                       : (is_k ? p.keys : p.values) + (static_cast<int64_t>(page) * p.Hkv * p.block + at) * D;
+  const int64_t dst_ld = is_q ? D : static_cast<int64_t>(p.block) * D;
+  if (!is_q && pad) return;
+  if (!is_q && !is_k) {  // v goes into its slot as is
 #pragma unroll
-  for (int e = 0; e < EPL; ++e) {
-    sn[e] = 0.0f;
-    cs[e] = 1.0f;
-    if (d0 + e < p.rot) {
-      const int i = IL ? (d0 + e) / 2 : lower ? d0 + e : d0 + e - half;
-      const uint64_t f = p.turns[i];
+    for (int n = 0; n < NU; ++n)
+      if (h0 + n * HPU < H) *reinterpret_cast<vec*>(dst + (h0 + n * HPU) * dst_ld + d0) = raw[n];
+    return;
+  }
+
+  // the weights of the lane's dims and of their partners
+  const void* w = is_q ? p.qw : p.kw;
+  float A[8], B[8];
+  auto load_w = [&](int i, float* out) {
+    if (w == nullptr) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) out[e] = 1.0f;
+    } else if (p.wdt == GDN_DTYPE_F32) {
+      typedef float w8 __attribute__((ext_vector_type(8), aligned(4)));
+      const w8 v = *reinterpret_cast<const w8*>(static_cast<const float*>(w) + i);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) out[e] = v[e];
+    } else {
+      const vec v = *reinterpret_cast<const vec*>(static_cast<const uint16_t*>(w) + i);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) out[e] = p.wdt == GDN_DTYPE_BF16 ? bf16_to_f32(v[e]) : f16_to_f32(v[e]);
+    }
+  };
+  load_w(d0, A);
+  if constexpr (IL) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) B[e] = A[e ^ 1];
+  } else {
+    load_w(!turned || !whole ? d0 : lower ? d0 + half : d0 - half, B);
+    if (turned && !whole) {
+      for (int e = 0; e < 8; ++e) {
+        const int d = d0 + e;
+        float one[8];
+        load_w(min(d < half ? d + half : d < p.rot ? d - half : d, D - 8), one);
+        const int skip = max((d < half ? d + half : d < p.rot ? d - half : d) - (D - 8), 0);
+        float v = one[0];
+#pragma unroll
+        for (int k = 1; k < 8; ++k) v = k == skip ? one[k] : v;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) B[k] = k == e ? v : B[k];
+      }
+    }
+  }
+  // cosine and signed sine of dim d < rot (to the last turned lane's end)
+  float* cs = trig[wave][0];
+  float* sn = trig[wave][1];
+  for (int d = lane; d < ((p.rot + 7) & ~7); d += 64) {
+    float c = 1.0f, s = 0.0f;
+    if (d < p.rot) {
+      const uint64_t f = p.turns[IL ? d / 2 : d < half ? d : d - half];
       const uint32_t phase = static_cast<uint32_t>(f >> 32) * pos + __umulhi(static_cast<uint32_t>(f), pos);
       const float x = static_cast<float>(static_cast<int32_t>(phase)) * 0x1p-32f;
-      const float s = __builtin_amdgcn_sinf(x) * p.factor;
-      sn[e] = (IL ? e % 2 == 0 : lower) ? -s : s;
-      cs[e] = __builtin_amdgcn_cosf(x) * p.factor;
+      c = __builtin_amdgcn_cosf(x) * p.factor;
+      s = __builtin_amdgcn_sinf(x) * p.factor;
+      if (IL ? d % 2 == 0 : d < half) s = -s;
     }
+    cs[d] = c;
+    sn[d] = s;
   }
-  auto weight = [&](uint32_t u) {
-    return p.wdt == GDN_DTYPE_F32 ? __uint_as_float(u)
-                                  : (p.wdt == GDN_DTYPE_BF16 ? bf16_to_f32(static_cast<uint16_t>(u))
-                                                             : f16_to_f32(static_cast<uint16_t>(u)));
-  };
-  float qw[EPL], kw[EPL];
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  {
+    const int d = turned ? d0 : 0;
+    const f32x4 c0 = *reinterpret_cast<const f32x4*>(cs + d), c1 = *reinterpret_cast<const f32x4*>(cs + d + 4);
+    const f32x4 s0 = *reinterpret_cast<const f32x4*>(sn + d), s1 = *reinterpret_cast<const f32x4*>(sn + d + 4);
 #pragma unroll
-  for (int e = 0; e < EPL; ++e) {
-    qw[e] = norm ? weight(qwr[e]) : 1.0f;
-    kw[e] = norm ? weight(kwr[e]) : 1.0f;
+    for (int e = 0; e < 8; ++e) {
+      A[e] *= turned ? (e < 4 ? c0[e & 3] : c1[e & 3]) : 1.0f;
+      B[e] *= turned ? (e < 4 ? s0[e & 3] : s1[e & 3]) : 0.0f;
+    }
   }
 
-  float r[NH];
 #pragma unroll
-  for (int n = 0; n < NH; ++n) {
-    float ss = 0.0f;
+  for (int n = 0; n < NU; ++n) {
+    float x[8], ss = 0.0f;
 #pragma unroll
-    for (int e = 0; e < EPL; ++e) {
-      const float x = bf16_to_f32(raw[n][e]);
-      ss += x * x;
+    for (int e = 0; e < 8; ++e) {
+      x[e] = bf16_to_f32(raw[n][e]);
+      ss = fmaf(x[e], x[e], ss);
     }
-    r[n] = norm ? rsqrtf(wave_sum(ss) / D + p.eps) : 1.0f;
-  }
-  vec out[NH];
-#pragma unroll
-  for (int n = 0; n < NH; ++n) {
-    float x[EPL];
-#pragma unroll
-    for (int e = 0; e < EPL; ++e) x[e] = bf16_to_f32(raw[n][e]) * r[n] * (h0 + n < p.Hq ? qw[e] : kw[e]);
-#pragma unroll
-    for (int e = 0; e < EPL; ++e) {
-      const float other = IL ? x[e ^ 1] : __shfl(x[e], partner, 64);
-      out[n][e] = f32_to_bf16(d0 + e < p.rot ? x[e] * cs[e] + other * sn[e] : x[e]);
+    float r = 1.0f;
+    if (w != nullptr) {
+      ss += dpp_f<GDN_DPP_QUAD_XOR1>(ss);
+      ss += dpp_f<GDN_DPP_QUAD_XOR2>(ss);
+      ss += dpp_f<GDN_DPP_HALF_MIRROR>(ss);
+      ss += dpp_f<GDN_DPP_ROW_MIRROR>(ss);
+      if constexpr (LPH == 32) {
+        const auto s2 = __builtin_amdgcn_permlane16_swap(__float_as_uint(ss), __float_as_uint(ss), false, false);
+        ss = __uint_as_float(s2[0]) + __uint_as_float(s2[1]);
+      }
+      r = rsqrtf(ss / D + p.eps);
     }
-  }
+    typedef uint32_t words __attribute__((ext_vector_type(4), aligned(2)));
+    words out;
 #pragma unroll
-  for (int n = 0; n < NH; ++n) {
-    const int h = h0 + n;
-    if (h >= heads) return;  // wave-uniform
-    if (h < p.Hq) {
-      *reinterpret_cast<vec*>(p.q + (static_cast<int64_t>(bt) * p.Hq + h) * D + d0) = pad ? vec{} : out[n];
-    } else if (!pad) {
-      const bool is_k = h < p.Hq + p.Hkv;  // v goes into its slot as is
-      const int hkv = h - p.Hq - (is_k ? 0 : p.Hkv);
-      *reinterpret_cast<vec*>((is_k ? p.keys : p.values) + ((static_cast<int64_t>(page) * p.Hkv + hkv) * p.block + at) * D + d0) =
-          is_k ? out[n] : raw[n];
+    for (int e = 0; e < 8; e += 2) {
+      const float o0 = IL ? x[e + 1] : bf16_to_f32(other[n][e]), o1 = IL ? x[e] : bf16_to_f32(other[n][e + 1]);
+      out[e / 2] = pk_bf16(r * fmaf(A[e], x[e], B[e] * o0), r * fmaf(A[e + 1], x[e + 1], B[e + 1] * o1));
     }
+    if (h0 + n * HPU < H) *reinterpret_cast<words*>(dst + (h0 + n * HPU) * dst_ld + d0) = pad ? words{0u, 0u, 0u, 0u} : out;
   }
+}
+
+int lg2(int64_t x) {  // of a power of two, else -1
+  return x > 0 && (x & (x - 1)) == 0 ? __builtin_ctzll(static_cast<uint64_t>(x)) : -1;
 }
 
 // ------------------------------------------------------------ attention
@@ -644,10 +721,6 @@ __global__ __launch_bounds__(256) void step_combine_kernel(const PagedParams p) 
   *reinterpret_cast<hvec*>(out) = t < tokens ? y : hvec{};
 }
 
-int lg2(int64_t x) {  // of a power of two, else -1
-  return x > 0 && (x & (x - 1)) == 0 ? __builtin_ctzll(static_cast<uint64_t>(x)) : -1;
-}
-
 }  // namespace
 
 extern "C" int gdn_paged_tables(const int32_t* lengths, const int32_t* n_new, int32_t* table, int64_t table_ld,
@@ -660,8 +733,8 @@ extern "C" int gdn_paged_tables(const int32_t* lengths, const int32_t* n_new, in
       shared > table_ld)
     return fail(GDN_ERR_INVALID, "gdn_paged_tables: bad sizes (blocks are powers of two up to 2^20; shared <= table width)");
   if (B > kTableRows) return fail(GDN_ERR_UNSUPPORTED, "gdn_paged_tables: at most %d rows (got %lld)", kTableRows, (long long)B);
-  if (B * T > INT32_MAX || n_blocks * block > INT32_MAX)
-    return fail(GDN_ERR_UNSUPPORTED, "gdn_paged_tables: tokens and slots must each be below 2^31");
+  if (B * T > INT32_MAX || n_blocks * block > INT32_MAX || B * table_ld > INT32_MAX)
+    return fail(GDN_ERR_UNSUPPORTED, "gdn_paged_tables: tokens, slots and table entries must each be below 2^31");
   if (B == 0) {
     if (n_free_out != n_free) return fail(GDN_ERR_INVALID, "gdn_paged_tables: no rows");
     return GDN_OK;
@@ -673,14 +746,17 @@ extern "C" int gdn_paged_tables(const int32_t* lengths, const int32_t* n_new, in
                          static_cast<int>(B), static_cast<int>(T), static_cast<int>(table_ld), lg,
                          static_cast<int>(shared), static_cast<int>(n_blocks)};
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const int64_t groups = (B * T + 1023) / 1024;
+  // a few tokens a thread: more would wait for each other's loads, fewer repeat the sums
+  const int64_t groups = (B * T + 4 * kTableThreads - 1) / (4 * kTableThreads);
   const unsigned grid = static_cast<unsigned>(groups < 1 ? 1 : groups > 512 ? 512 : groups);
-  const bool in_place = held_out == held || n_free_out == n_free;
-  hipLaunchKernelGGL(tables_kernel, dim3(grid), dim3(256), 0, st, p, grid > 1 && in_place ? kCells : kCells | kState);
-  int rc = gdn_host::check_launch("gdn_paged_tables");
-  if (rc != GDN_OK || !(grid > 1 && in_place)) return rc;
-  hipLaunchKernelGGL(tables_kernel, dim3(1), dim3(256), 0, st, p, kState);
-  return gdn_host::check_launch("gdn_paged_tables/state");
+  const bool behind = grid > 1 && (held_out == held || n_free_out == n_free);
+  auto launch = [&](unsigned n, int what) {
+    if (B <= kTableThreads) hipLaunchKernelGGL(tables_kernel<1>, dim3(n), dim3(kTableThreads), 0, st, p, what);
+    else hipLaunchKernelGGL(tables_kernel<kTableRows / kTableThreads>, dim3(n), dim3(kTableThreads), 0, st, p, what);
+    return gdn_host::check_launch("gdn_paged_tables");
+  };
+  const int rc = launch(grid, behind ? kCells : kCells | kState);
+  return rc != GDN_OK || !behind ? rc : launch(1, kState);
 }
 
 extern "C" int gdn_attn_rope(const void* qg, int64_t qg_ld, int64_t q_head, const void* k_new, const void* v_new,
@@ -693,7 +769,7 @@ extern "C" int gdn_attn_rope(const void* qg, int64_t qg_ld, int64_t q_head, cons
   if (B < 0 || T < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || q_head < D || n_blocks < 0 || block <= 0 ||
       block > INT32_MAX || (!slots && (n_blocks != B || block < T)))
     return fail(GDN_ERR_INVALID, "gdn_attn_rope: bad sizes");
-  if (rot < 0 || rot > D || rot % 2 != 0 || (!interleaved && rot % (2 * (D / 64)) != 0))
+  if (rot < 0 || rot > D || rot % 2 != 0)
     return fail(GDN_ERR_UNSUPPORTED, "gdn_attn_rope: rotary dims %lld not supported for head dim %lld", (long long)rot,
                 (long long)D);
   if ((q_norm_w == nullptr) != (k_norm_w == nullptr) || (q_norm_w && !gdn_host::dtype_ok(w_dtype)) || !(eps >= 0.0f))
@@ -701,7 +777,7 @@ extern "C" int gdn_attn_rope(const void* qg, int64_t qg_ld, int64_t q_head, cons
   if (B * T == 0) return GDN_OK;
   if (!qg || !k_new || !v_new || !pos0 || (rot > 0 && !turns) || !q_out || !keys || !values)
     return fail(GDN_ERR_INVALID, "gdn_attn_rope: null pointer");
-  if (B * T * (Hq + 2 * Hkv) > INT32_MAX || q_head > INT32_MAX)
+  if (B * T * (Hq + 2 * Hkv) > INT32_MAX || Hq * q_head > INT32_MAX)
     return fail(GDN_ERR_UNSUPPORTED, "gdn_attn_rope: problem too large");
   if (slots && n_blocks * block > INT32_MAX)
     return fail(GDN_ERR_UNSUPPORTED, "gdn_attn_rope: slots must be below 2^31");
@@ -735,21 +811,26 @@ extern "C" int gdn_attn_rope(const void* qg, int64_t qg_ld, int64_t q_head, cons
   p.eps = eps;
   p.factor = factor;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  auto launch = [&](auto nh, auto il) {
-    constexpr int NH = decltype(nh)::value;
+  // groups of heads per wave by the heads of all tokens: a wave with more runs longer, and shares its
+  // angles and weights among them
+  auto launch = [&](auto nu, auto il) {
+    constexpr int NU = decltype(nu)::value;
     constexpr bool IL = decltype(il)::value;
-    const dim3 grid(static_cast<unsigned>((B * T * ((Hq + 2 * Hkv + NH - 1) / NH) + 3) / 4));
-    if (D == 256) hipLaunchKernelGGL((attn_rope_kernel<256, NH, IL>), grid, dim3(256), 0, st, p);
-    else hipLaunchKernelGGL((attn_rope_kernel<128, NH, IL>), grid, dim3(256), 0, st, p);
+    const int64_t per = NU * (512 / D);  // heads per wave
+    p.q_items = static_cast<int>((Hq + per - 1) / per);
+    p.kv_items = static_cast<int>((Hkv + per - 1) / per);
+    p.per_tok = static_cast<uint32_t>(p.q_items + 2 * p.kv_items);
+    const dim3 grid(static_cast<unsigned>((B * T * p.per_tok + 3) / 4));
+    if (D == 256) hipLaunchKernelGGL((attn_rope_kernel<256, NU, IL>), grid, dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((attn_rope_kernel<128, NU, IL>), grid, dim3(256), 0, st, p);
   };
-  auto heads_per_wave = [&](auto il) {
+  auto groups_per_wave = [&](auto il) {
     const int64_t rows = B * T * (Hq + 2 * Hkv);
-    if (rows <= 4096) launch(std::integral_constant<int, 1>{}, il);
-    else if (rows <= 16384) launch(std::integral_constant<int, 3>{}, il);
-    else launch(std::integral_constant<int, 6>{}, il);
+    if (rows <= kRopeFew) launch(std::integral_constant<int, 1>{}, il);
+    else launch(std::integral_constant<int, kRopeGroups>{}, il);
   };
-  if (interleaved) heads_per_wave(std::true_type{});
-  else heads_per_wave(std::false_type{});
+  if (interleaved) groups_per_wave(std::true_type{});
+  else groups_per_wave(std::false_type{});
   return gdn_host::check_launch("gdn_attn_rope");
 }
 
@@ -792,7 +873,7 @@ extern "C" int gdn_paged_attn(const void* q, const void* qg, int64_t qg_ld, cons
   if (need > 0 && (workspace == nullptr || workspace_bytes < need || !gdn_host::aligned(workspace, 16)))
     return fail(GDN_ERR_INVALID, "gdn_paged_attn: workspace of %zu bytes is below the %zu needed for %lld key ranges",
                 workspace_bytes, need, (long long)n_split);
-  StepParams p;
+  StepParams p = {};
   p.q = static_cast<const uint16_t*>(q);
   p.qg = static_cast<const uint16_t*>(qg);
   p.qg_ld = qg_ld;

@@ -28,9 +28,13 @@ import torch
 
 from . import _lib
 from .attention import KVCache, _pos_add, _token_stride
-from .gated_delta import _ptr, _require_device, _stream
+from .gated_delta import _require_device, _stream
 
 __all__ = ["paged_tables", "paged_attn", "BlockPool", "PagedKVCache"]
+
+
+def _is_i32(t: torch.Tensor, shape: Tuple[int, ...], index: int) -> bool:
+    return t.dtype is torch.int32 and t.shape == shape and t.get_device() == index and t.is_contiguous()
 
 
 def _i32(t: torch.Tensor, shape: Tuple[int, ...], what: str) -> None:
@@ -58,36 +62,47 @@ def paged_tables(lengths: torch.Tensor, T: int, table: torch.Tensor, held: torch
     tensors unless ``held_out=held``, ``n_free_out=n_free`` ask for them in place
     (without, the same call can be repeated).
     """
-    dev = _require_device((lengths, table, held, free, n_free, n_new, held_out, n_free_out, slots),
-                          ("lengths", "table", "held", "free", "n_free", "n_new", "held_out", "n_free_out", "slots"))
-    B, T = lengths.shape[0] if lengths.dim() == 1 else -1, int(T)
-    if B < 0 or T < 0:
+    dev = lengths.device
+    index = lengths.get_device()
+    T = int(T)
+    # the whole check in a few operations; what is wrong is looked for only where something is
+    if index < 0 or lengths.dim() != 1 or table.dim() != 2 or free.dim() != 1 or T < 0:
+        _refuse_tables(lengths, T, table, held, free, n_free, n_new, held_out, n_free_out, slots)
+    B, width, n_blocks = lengths.shape[0], table.shape[1], free.shape[0]
+    row, one = (B,), (1,)
+    if not (_is_i32(lengths, row, index) and _is_i32(table, (B, width), index) and _is_i32(held, row, index)
+            and _is_i32(free, (n_blocks,), index) and _is_i32(n_free, one, index)
+            and (n_new is None or _is_i32(n_new, row, index))
+            and (held_out is None or held_out is held or _is_i32(held_out, row, index))
+            and (n_free_out is None or n_free_out is n_free or _is_i32(n_free_out, one, index))
+            and (slots is None or _is_i32(slots, (B, T), index))):
+        _refuse_tables(lengths, T, table, held, free, n_free, n_new, held_out, n_free_out, slots)
+    if held_out is None:
+        held_out = torch.empty_like(held)
+    if n_free_out is None:
+        n_free_out = torch.empty_like(n_free) if B else n_free
+    if slots is None:
+        slots = lengths.new_empty((B, T))
+    _lib.call(dev, "gdn_paged_tables", lengths.data_ptr(), None if n_new is None else n_new.data_ptr(),
+              table.data_ptr(), width, held.data_ptr(), free.data_ptr(), n_free.data_ptr(), held_out.data_ptr(),
+              n_free_out.data_ptr(), slots.data_ptr(), B, T, int(block), int(shared), n_blocks, _stream(dev))
+    return slots, held_out, n_free_out
+
+
+def _refuse_tables(lengths, T, table, held, free, n_free, n_new, held_out, n_free_out, slots) -> None:
+    """Raises what is wrong with :func:`paged_tables`' arguments."""
+    _require_device((lengths, table, held, free, n_free, n_new, held_out, n_free_out, slots),
+                    ("lengths", "table", "held", "free", "n_free", "n_new", "held_out", "n_free_out", "slots"))
+    if lengths.dim() != 1 or T < 0:
         raise ValueError("lengths must be a [B] tensor and T >= 0")
     if table.dim() != 2 or free.dim() != 1:
         raise ValueError("table must be [B, width] and free [n_blocks]")
-    _i32(lengths, (B,), "lengths")
-    _i32(table, (B, table.shape[1]), "table")
-    _i32(held, (B,), "held")
-    _i32(free, (free.shape[0],), "free")
-    _i32(n_free, (1,), "n_free")
-    if n_new is not None:
-        _i32(n_new, (B,), "n_new")
-    if held_out is None:
-        held_out = torch.empty_like(held)
-    else:
-        _i32(held_out, (B,), "held_out")
-    if n_free_out is None:
-        n_free_out = torch.empty_like(n_free) if B else n_free
-    else:
-        _i32(n_free_out, (1,), "n_free_out")
-    if slots is None:
-        slots = torch.empty(B, T, dtype=torch.int32, device=dev)
-    else:
-        _i32(slots, (B, T), "slots")
-    _lib.call(dev, "gdn_paged_tables", _ptr(lengths), _ptr(n_new), _ptr(table), table.shape[1], _ptr(held),
-              _ptr(free), _ptr(n_free), _ptr(held_out), _ptr(n_free_out), _ptr(slots), B, T, int(block), int(shared),
-              free.shape[0], _stream(dev))
-    return slots, held_out, n_free_out
+    B = lengths.shape[0]
+    for t, shape, what in ((lengths, (B,), "lengths"), (table, (B, table.shape[1]), "table"), (held, (B,), "held"),
+                           (free, (free.shape[0],), "free"), (n_free, (1,), "n_free"), (n_new, (B,), "n_new"),
+                           (held_out, (B,), "held_out"), (n_free_out, (1,), "n_free_out"), (slots, (B, T), "slots")):
+        if t is not None:
+            _i32(t, shape, what)
 
 
 _cus = {}
@@ -132,8 +147,50 @@ def paged_attn(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, table:
     once for the batch.  ``n_split`` sets the key ranges of the prefix (0: with
     each row's own keys) and of a row's own keys; by default a rule does.
     """
-    dev = _require_device((q, keys, values, table, pos0, n_new, gate, workspace, out),
-                          ("q", "keys", "values", "table", "pos0", "n_new", "gate", "workspace", "out"))
+    dev = q.device
+    index = q.get_device()
+    kv_len_max, shared = int(kv_len_max), int(shared)
+    if index < 0 or q.dim() != 4 or keys.dim() != 4 or table.dim() != 2:
+        _refuse_attn(q, keys, values, table, pos0, kv_len_max, n_new, shared, gate, workspace, out)
+    B, T, Hq, D = q.shape
+    n_blocks, Hkv, block, Dk = keys.shape
+    width = table.shape[1]
+    bf16, row = torch.bfloat16, (B,)
+    if not (q.dtype is bf16 and keys.dtype is bf16 and values.dtype is bf16 and keys.get_device() == index
+            and values.get_device() == index and values.shape == keys.shape and keys.is_contiguous()
+            and values.is_contiguous() and Dk == D and Hkv > 0 and Hq % Hkv == 0
+            and _is_i32(table, (B, width), index) and _is_i32(pos0, row, index)
+            and (n_new is None or _is_i32(n_new, row, index))
+            and 0 <= shared * block <= kv_len_max - (T if n_new is None else 0) and kv_len_max <= width * block
+            and (gate is None or (gate.dtype is bf16 and gate.shape == (B, T, Hq * 2 * D) and gate.get_device() == index))
+            and (workspace is None or workspace.get_device() == index)
+            and (out is None or (out.dtype is bf16 and out.shape == q.shape and out.get_device() == index
+                                 and out.is_contiguous()))):
+        _refuse_attn(q, keys, values, table, pos0, kv_len_max, n_new, shared, gate, workspace, out)
+    qg_ld = 0 if gate is None else _token_stride(gate, Hq * 2 * D, "gate")
+    if not q.is_contiguous():
+        q = q.contiguous()
+    if out is None:
+        out = torch.empty_like(q)
+    prefix = shared * block
+    n_prefix, n_own = _ranges(_cu_count(dev), B, T, Hq, Hkv, prefix, kv_len_max - prefix) if n_split is None else n_split
+    ws, ws_bytes = None, 0
+    if n_prefix + n_own > 1:
+        need = B * T * Hq * (n_prefix + n_own) * (D + 2)  # gdn_paged_attn_workspace_bytes, in floats
+        if workspace is None or workspace.numel() * workspace.element_size() < 4 * need:
+            workspace = torch.empty(need, dtype=torch.float32, device=dev)
+        ws, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    _lib.call(dev, "gdn_paged_attn", q.data_ptr(), None if gate is None else gate.data_ptr(), qg_ld, keys.data_ptr(),
+              values.data_ptr(), table.data_ptr(), width, pos0.data_ptr(), None if n_new is None else n_new.data_ptr(),
+              out.data_ptr(), D ** -0.5 if scale is None else float(scale), B, T, Hq, Hkv, D, n_blocks, block,
+              kv_len_max, shared, n_prefix, n_own, ws, ws_bytes, _stream(dev))
+    return out
+
+
+def _refuse_attn(q, keys, values, table, pos0, kv_len_max, n_new, shared, gate, workspace, out) -> None:
+    """Raises what is wrong with :func:`paged_attn`'s arguments."""
+    _require_device((q, keys, values, table, pos0, n_new, gate, workspace, out),
+                    ("q", "keys", "values", "table", "pos0", "n_new", "gate", "workspace", "out"))
     for t, n in ((q, "q"), (keys, "keys"), (values, "values"), (gate, "gate"), (out, "out")):
         if t is not None and t.dtype is not torch.bfloat16:
             raise ValueError(f"{n} must be bfloat16 (got {t.dtype})")
@@ -142,7 +199,7 @@ def paged_attn(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, table:
     B, T, Hq, D = q.shape
     if keys.dim() != 4 or values.shape != keys.shape or not keys.is_contiguous() or not values.is_contiguous():
         raise ValueError("keys and values must be contiguous [n_blocks, Hkv, block, D] tensors of one shape")
-    n_blocks, Hkv, block, Dk = keys.shape
+    _, Hkv, block, Dk = keys.shape
     if Dk != D or Hkv == 0 or Hq % Hkv != 0:
         raise ValueError(f"pools of {Hkv} heads of {Dk} do not match q's {Hq} heads of {D}")
     if table.dim() != 2:
@@ -152,34 +209,12 @@ def paged_attn(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, table:
     _i32(pos0, (B,), "pos0")
     if n_new is not None:
         _i32(n_new, (B,), "n_new")
-    kv_len_max, shared = int(kv_len_max), int(shared)
     if not 0 <= shared * block <= kv_len_max - (T if n_new is None else 0) or kv_len_max > width * block:
         raise ValueError(f"kv_len_max={kv_len_max} must lie in [shared * block + T, width * block = {width * block}]")
-    qg_ld = 0
-    if gate is not None:
-        if gate.dim() != 3 or tuple(gate.shape) != (B, T, Hq * 2 * D):
-            raise ValueError(f"gate must be [{B}, {T}, {Hq * 2 * D}]")
-        qg_ld = _token_stride(gate, Hq * 2 * D, "gate")
-    if out is None:
-        out = torch.empty(B, T, Hq, D, dtype=torch.bfloat16, device=dev)
-    elif tuple(out.shape) != (B, T, Hq, D) or not out.is_contiguous():
+    if gate is not None and gate.shape != (B, T, Hq * 2 * D):
+        raise ValueError(f"gate must be [{B}, {T}, {Hq * 2 * D}]")
+    if out is not None and (out.shape != q.shape or not out.is_contiguous()):
         raise ValueError(f"out must be a contiguous [{B}, {T}, {Hq}, {D}] tensor")
-    if n_split is None:
-        prefix = shared * block
-        n_split = _ranges(_cu_count(dev), B, T, Hq, Hkv, prefix, kv_len_max - prefix)
-    n_prefix, n_own = n_split
-    ws_bytes = 0
-    if n_prefix + n_own > 1:
-        need = int(_lib.load().gdn_paged_attn_workspace_bytes(B, T, Hq, Hkv, D, n_prefix + n_own))
-        if need > 0 and (workspace is None or workspace.numel() * workspace.element_size() < need):
-            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-        ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
-    q = q.contiguous()
-    scale = D ** -0.5 if scale is None else scale
-    _lib.call(dev, "gdn_paged_attn", _ptr(q), _ptr(gate), qg_ld, _ptr(keys), _ptr(values), _ptr(table), width,
-              _ptr(pos0), _ptr(n_new), _ptr(out), float(scale), B, T, Hq, Hkv, D, n_blocks, block, kv_len_max, shared,
-              n_prefix, n_own, _ptr(workspace), ws_bytes, _stream(dev))
-    return out
 
 
 # ------------------------------------------------------------------ cache

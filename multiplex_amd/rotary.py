@@ -18,7 +18,7 @@ from typing import Optional, Sequence
 import torch
 
 from . import _lib
-from .gated_delta import _dtype_code, _ptr, _require_device, _stream
+from .gated_delta import _dtype_code, _require_device, _stream
 
 __all__ = ["Rotary", "attn_rope"]
 
@@ -124,9 +124,54 @@ def attn_rope(qg: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, q_norm
     The norm is not rounded before the rotation (:func:`attention.attn_qk`
     rounds there, as the reference does).
     """
-    tensors = (qg, k_new, v_new, q_norm_w, k_norm_w, pos0, keys, values, slots, rotary.turns, q_out)
-    dev = _require_device(tensors, ("qg", "k_new", "v_new", "q_norm_w", "k_norm_w", "pos0", "keys", "values", "slots",
-                                    "rotary", "q_out"))
+    dev = qg.device
+    index, turns = qg.get_device(), rotary.turns
+    if index < 0 or qg.dim() != 3 or keys.dim() != 4:
+        _refuse(qg, k_new, v_new, q_norm_w, k_norm_w, pos0, keys, values, turns, slots, gated, q_out)
+    B, T, width = qg.shape
+    n_blocks, Hkv, block, D = keys.shape
+    q_head = 2 * D if gated else D
+    Hq = width // q_head
+    bf16, i32 = torch.bfloat16, torch.int32
+    kv = (B, T, Hkv * D)
+    if not (qg.dtype is bf16 and k_new.dtype is bf16 and v_new.dtype is bf16 and keys.dtype is bf16
+            and values.dtype is bf16 and k_new.get_device() == v_new.get_device() == keys.get_device()
+            == values.get_device() == pos0.get_device() == turns.get_device() == index
+            and values.shape == keys.shape and keys.is_contiguous() and values.is_contiguous()
+            and Hkv > 0 and Hq > 0 and width == Hq * q_head and Hq % Hkv == 0
+            and k_new.shape == kv and v_new.shape == kv
+            and pos0.dtype is i32 and pos0.shape == (B,) and pos0.is_contiguous()
+            and (n_blocks == B and block >= T if slots is None else
+                 slots.dtype is i32 and slots.shape == (B, T) and slots.get_device() == index and slots.is_contiguous())
+            and (q_norm_w is None and k_norm_w is None or q_norm_w is not None and k_norm_w is not None
+                 and q_norm_w.shape == k_norm_w.shape == (D,) and q_norm_w.dtype is k_norm_w.dtype
+                 and q_norm_w.get_device() == k_norm_w.get_device() == index)
+            and (q_out is None or q_out.dtype is bf16 and q_out.shape == (B, T, Hq, D) and q_out.get_device() == index
+                 and q_out.is_contiguous())):
+        _refuse(qg, k_new, v_new, q_norm_w, k_norm_w, pos0, keys, values, turns, slots, gated, q_out)
+    qg_ld = _tokens(qg, B, T, width, "qg")
+    kv_ld = _tokens(k_new, B, T, Hkv * D, "k_new")
+    if _tokens(v_new, B, T, Hkv * D, "v_new") != kv_ld:
+        raise ValueError("k_new and v_new must share one token stride")
+    qn = kn = None
+    wdt = 0
+    if q_norm_w is not None:
+        if not (q_norm_w.is_contiguous() and k_norm_w.is_contiguous()):
+            q_norm_w, k_norm_w = q_norm_w.contiguous(), k_norm_w.contiguous()
+        qn, kn, wdt = q_norm_w.data_ptr(), k_norm_w.data_ptr(), _dtype_code(q_norm_w, "q_norm_w")
+    if q_out is None:
+        q_out = torch.empty((B, T, Hq, D), dtype=bf16, device=dev)
+    _lib.call(dev, "gdn_attn_rope", qg.data_ptr(), qg_ld, q_head, k_new.data_ptr(), v_new.data_ptr(), kv_ld, qn, kn,
+              wdt, float(eps), pos0.data_ptr(), None if slots is None else slots.data_ptr(), turns.data_ptr(),
+              rotary.factor, int(rotary.interleaved), q_out.data_ptr(), keys.data_ptr(), values.data_ptr(), B, T, Hq,
+              Hkv, D, n_blocks, block, rotary.rot, _stream(dev))
+    return q_out
+
+
+def _refuse(qg, k_new, v_new, q_norm_w, k_norm_w, pos0, keys, values, turns, slots, gated, q_out) -> None:
+    """Raises what is wrong with :func:`attn_rope`'s arguments."""
+    _require_device((qg, k_new, v_new, q_norm_w, k_norm_w, pos0, keys, values, slots, turns, q_out),
+                    ("qg", "k_new", "v_new", "q_norm_w", "k_norm_w", "pos0", "keys", "values", "slots", "rotary", "q_out"))
     for t, n in ((qg, "qg"), (k_new, "k_new"), (v_new, "v_new"), (keys, "keys"), (values, "values"), (q_out, "q_out")):
         if t is not None and t.dtype is not torch.bfloat16:
             raise ValueError(f"{n} must be bfloat16 (got {t.dtype})")
@@ -140,10 +185,8 @@ def attn_rope(qg: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, q_norm
     Hq = width // q_head
     if Hq == 0 or width != Hq * q_head or Hkv == 0 or Hq % Hkv != 0:
         raise ValueError(f"qg's {width} columns are not heads of {q_head}, a multiple of {Hkv} of them")
-    qg_ld = _tokens(qg, B, T, width, "qg")
-    kv_ld = _tokens(k_new, B, T, Hkv * D, "k_new")
-    if _tokens(v_new, B, T, Hkv * D, "v_new") != kv_ld:
-        raise ValueError("k_new and v_new must share one token stride")
+    _tokens(k_new, B, T, Hkv * D, "k_new")
+    _tokens(v_new, B, T, Hkv * D, "v_new")
     if pos0.dtype is not torch.int32 or tuple(pos0.shape) != (B,) or not pos0.is_contiguous():
         raise ValueError(f"pos0 must be a contiguous int32 [{B}] tensor")
     if slots is not None:
@@ -153,18 +196,8 @@ def attn_rope(qg: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, q_norm
         raise ValueError(f"without slots keys must be a [B={B}, Hkv, cap >= {T}, D] cache (got {tuple(keys.shape)})")
     if (q_norm_w is None) != (k_norm_w is None):
         raise ValueError("give both norm weights or neither")
-    wdt = 0
-    qn = kn = None
-    if q_norm_w is not None:
-        if tuple(q_norm_w.shape) != (D,) or tuple(k_norm_w.shape) != (D,) or q_norm_w.dtype != k_norm_w.dtype:
-            raise ValueError(f"norm weights must be [{D}] tensors of one dtype")
-        qn, kn = q_norm_w.contiguous(), k_norm_w.contiguous()
-        wdt = _dtype_code(qn, "q_norm_w")
-    if q_out is None:
-        q_out = torch.empty(B, T, Hq, D, dtype=torch.bfloat16, device=dev)
-    elif tuple(q_out.shape) != (B, T, Hq, D) or not q_out.is_contiguous():
+    if q_norm_w is not None and (tuple(q_norm_w.shape) != (D,) or tuple(k_norm_w.shape) != (D,)
+                                 or q_norm_w.dtype != k_norm_w.dtype):
+        raise ValueError(f"norm weights must be [{D}] tensors of one dtype")
+    if q_out is not None and (tuple(q_out.shape) != (B, T, Hq, D) or not q_out.is_contiguous()):
         raise ValueError(f"q_out must be a contiguous [{B}, {T}, {Hq}, {D}] tensor")
-    _lib.call(dev, "gdn_attn_rope", _ptr(qg), qg_ld, q_head, _ptr(k_new), _ptr(v_new), kv_ld, _ptr(qn), _ptr(kn), wdt,
-              float(eps), _ptr(pos0), _ptr(slots), _ptr(rotary.turns), rotary.factor, int(rotary.interleaved),
-              _ptr(q_out), _ptr(keys), _ptr(values), B, T, Hq, Hkv, D, n_blocks, block, rotary.rot, _stream(dev))
-    return q_out

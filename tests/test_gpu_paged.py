@@ -130,6 +130,10 @@ YARN = {"type": "yarn", "factor": 4.0, "original_max_position_embeddings": 32768
     (2, 500, 32, 8, 128, 64, True, None, True, torch.bfloat16, 5000),   # six heads a wave
     (2, 3, 5, 1, 256, 6, True, None, False, torch.float32, 300),        # a lane of two rotated, two plain dims
     (2, 3, 5, 1, 128, 0, False, None, True, torch.float32, 300),        # nothing rotated
+    (3, 7, 6, 2, 256, 72, False, YARN, True, torch.float32, 300),       # pairs that end inside a lane's dims
+    (3, 7, 7, 7, 128, 10, False, None, True, torch.bfloat16, 300),      # heads that end inside a group
+    (2, 900, 7, 1, 128, 128, False, None, True, torch.float32, 300),    # ... several groups a wave
+    (2, 900, 5, 1, 256, 100, True, None, False, torch.float16, 3000),
 ])
 def test_rope_matches_oracle(B, T, Hq, Hkv, D, rot, interleaved, scaling, gated, wdt, far):
     """Against the oracle, with column slices at odd offsets, padded tokens, and slots in any order."""

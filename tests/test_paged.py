@@ -51,6 +51,7 @@ def _tables(lib, **kw):
     (dict(B=4097), _lib.ERR_UNSUPPORTED),
     (dict(T=1 << 31), _lib.ERR_UNSUPPORTED),
     (dict(n_blocks=1 << 25), _lib.ERR_UNSUPPORTED),
+    (dict(ld=1 << 30), _lib.ERR_UNSUPPORTED),
     (dict(B=0, n_free_out=2 * FAKE), _lib.ERR_INVALID),
     (dict(B=0), _lib.OK),
 ])
@@ -73,7 +74,7 @@ def _rope(lib, **kw):
     (dict(Hq=15), _lib.ERR_INVALID),
     (dict(rot=63), _lib.ERR_UNSUPPORTED),
     (dict(rot=258), _lib.ERR_UNSUPPORTED),
-    (dict(rot=4), _lib.ERR_UNSUPPORTED),            # pairs (i, i + 2): half a lane apart
+    (dict(rot=6, B=0), _lib.OK),
     (dict(rot=4, il=1, B=0), _lib.OK),
     (dict(slots=None), _lib.ERR_INVALID),           # dense: one block a row
     (dict(slots=None, n_blocks=2, block=2), _lib.ERR_INVALID),
@@ -131,6 +132,16 @@ def _attn(lib, **kw):
 def test_attention_abi_refusals(lib, kw, status):
     assert _attn(lib, **kw) == status
     assert status == _lib.OK or _lib.last_error()
+
+
+@pytest.mark.parametrize("B,T,Hq,Hkv,D,n", [(2, 3, 16, 4, 256, 3), (7, 1, 12, 4, 128, 2), (64, 1, 16, 4, 256, 33)])
+def test_attention_workspace_as_the_call_takes_it(lib, calls, monkeypatch, B, T, Hq, Hkv, D, n):
+    """The Python call sizes the workspace by itself: exactly the library's."""
+    made = []
+    monkeypatch.setattr(_lib, "call", lambda dev, name, *args: made.append(args))
+    mx.paged_attn(**_attn_args(q=_z(B, T, Hq, D, dtype=BF), keys=_z(5, Hkv, 64, D, dtype=BF),
+                               values=_z(5, Hkv, 64, D, dtype=BF), table=_z(B, 4), pos0=_z(B)), n_split=(1, n - 1))
+    assert made[0][-2] == lib.gdn_paged_attn_workspace_bytes(B, T, Hq, Hkv, D, n) and made[0][-3]
 
 
 def test_attention_workspace(lib):
