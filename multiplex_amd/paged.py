@@ -21,6 +21,7 @@ blocks, and rows that continue one prompt list the prompt's blocks in common:
 
 from __future__ import annotations
 
+import functools
 import weakref
 from typing import List, Optional, Sequence, Tuple
 
@@ -115,18 +116,65 @@ def _cu_count(dev: torch.device) -> int:
     return n
 
 
-def _ranges(cus: int, B: int, T: int, Hq: int, Hkv: int, prefix: int, own: int) -> Tuple[int, int]:
+# us that a workgroup takes, before its first and after its last keys and per step
+# of them: 16 rows (128 keys a step), 128 rows (64 keys); us that the merge of the
+# partial results takes, and per MB of them; the share of kv_len_max that rows
+# hold on average; the share of a workgroup's time that more workgroups than fit
+# at once add.  At head dims up to 128 and 256 (two workgroups a CU, and one).
+# Fitted to graph-replayed times of 3000 sizes (the four head layouts of 4 to 8
+# query heads a group and 128 or 256 dims, 1 to 128 rows, 1 to 512 tokens, prefixes
+# to 16384 and rows' own keys to 32768), 16 choices each; at 13000 others its choice
+# is 3 to 4% slower than the best of them on average, 10 to 14% at one in ten.
+_US = ((6.3, 1.00, 7.3, 1.22, 3.9, 0.36, 0.79, 0.58), (9.7, 1.31, 11.4, 1.54, 4.3, 0.31, 0.76, 0.49))
+_PREFIX_RANGES = (0, 1, 2, 3, 4, 6, 8, 12, 16, 20, 24, 32, 48, 64)
+_OWN_RANGES = (1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128, 256)
+
+
+@functools.lru_cache(maxsize=4096)
+def _ranges(cus: int, B: int, T: int, Hq: int, Hkv: int, D: int, prefix: int, own: int) -> Tuple[int, int]:
     """``(n_prefix, n_own)``: key ranges of the shared prefix (0: read with each
-    row's own keys) and of a row's own keys, for workgroups enough."""
+    row's own keys) and of a row's own keys; both lengths in steps of 64 keys.
+
+    The prefix read once takes work from every row, but leaves partial results
+    to merge; ranges make workgroups enough, each at a price.  So the choice is
+    the least of the times that :data:`_US` gives.  (Decode of 64 rows of 16
+    heads of 256 behind 8192 keys, up to 512 of their own, us: with the rows' own
+    112, in 4 / 12 / 32 ranges 66 / 39 / 53; 4 rows behind 2048: 29, in 16 ranges 16.)
+    """
     rows = T * (Hq // Hkv)
-    if prefix and (B == 1 or rows >= 128):
-        prefix, own = 0, own + prefix
-    tiles = -(-rows // (16 if rows <= 16 else 128))
-    n_own = max(1, min(cus // max(B * Hkv * tiles, 1), own // 128))
-    if not prefix:
-        return 0, n_own
-    tiles = -(-B * rows // (16 if B * rows <= 16 else 128))
-    return max(1, min(cus // (Hkv * tiles), prefix // 128)), n_own
+    few, few_step, many, many_step, merge, merge_mb, filled, crowd = _US[D > 128]
+    slots = cus * (1 if D > 128 else 2)
+
+    def groups(n_rows, blocks, n):
+        """Workgroups of a kv-head, and us that one takes."""
+        of = -(-blocks // n)
+        n = -(-blocks // of)
+        if n_rows <= 16:
+            return n, few + few_step * -(-of // 2)
+        return -(-n_rows // 128) * n, many + many_step * of
+
+    best, choice = None, (0, 1)
+    for p in _PREFIX_RANGES:
+        if p and (B == 1 or rows >= 256 or p > prefix):
+            break
+        own_p = own if p else own + prefix
+        if p:
+            n_p, us_p = groups(B * rows, prefix, p)
+            n_p *= Hkv
+        for o in _OWN_RANGES:
+            if o > 1 and 2 * o > own_p or p and o > 8:
+                break
+            n_o, us = groups(rows, max(own_p, 1), o)
+            n_o *= B * Hkv
+            busy, last, n = n_o * us * filled, us, n_o
+            if p:
+                busy, last, n, us = busy + n_p * us_p, max(us, us_p), n + n_p, min(us, us_p)
+            t = max(last, busy / slots) + (crowd * us if n > slots else 0.0)
+            if p + o > 1:
+                t += merge + merge_mb * 4e-6 * B * T * Hq * D * (p + o)
+            if best is None or t < best:
+                best, choice = t, (p, o)
+    return choice
 
 
 def paged_attn(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, table: torch.Tensor, pos0: torch.Tensor,
@@ -173,7 +221,9 @@ def paged_attn(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, table:
     if out is None:
         out = torch.empty_like(q)
     prefix = shared * block
-    n_prefix, n_own = _ranges(_cu_count(dev), B, T, Hq, Hkv, prefix, kv_len_max - prefix) if n_split is None else n_split
+    if n_split is None:
+        n_split = _ranges(_cu_count(dev), B, T, Hq, Hkv, D, prefix >> 6, (kv_len_max - prefix + 63) >> 6)
+    n_prefix, n_own = n_split
     ws, ws_bytes = None, 0
     if n_prefix + n_own > 1:
         need = B * T * Hq * (n_prefix + n_own) * (D + 2)  # gdn_paged_attn_workspace_bytes, in floats

@@ -528,11 +528,20 @@ def test_cache_refusals(on_cpu):
 
 def test_ranges_are_within_the_keys():
     for cus in (64, 256):
-        for B in (1, 2, 7, 64, 300):
-            for T in (1, 3, 17, 200):
-                for heads in ((16, 4), (16, 2), (8, 8)):
-                    for prefix in (0, 64, 4096):
-                        for own in (T, T + 100, T + 9000):
+        for B in (0, 1, 2, 7, 64, 300):
+            for T in (0, 1, 3, 17, 200):
+                for heads in ((16, 4, 256), (16, 2, 128), (8, 8, 128)):
+                    for prefix in (0, 1, 64):
+                        for own in (0, 1, 5, 150):
                             p, o = paged._ranges(cus, B, T, *heads, prefix, own)
-                            assert o >= 1 and (p == 0 or prefix > 0) and 64 * p <= max(prefix, 64)
-                            assert 64 * (o - 1) <= own + (0 if p else prefix)
+                            assert o >= 1 and p <= prefix
+                            assert o == 1 or 2 * o <= own + (0 if p else prefix)
+
+
+def test_ranges_read_a_long_prefix_once():
+    """Many rows of one token behind a long prefix share its pass; one row, or rows of whole tiles, do not."""
+    assert paged._ranges(256, 64, 1, 16, 4, 256, 128, 8)[0] > 1
+    assert paged._ranges(256, 32, 4, 16, 4, 256, 256, 11)[0] > 1
+    assert paged._ranges(256, 1, 1, 16, 4, 256, 128, 8)[0] == 0
+    assert paged._ranges(256, 4, 512, 16, 4, 256, 64, 10)[0] == 0
+    assert paged._ranges(256, 1, 1, 16, 4, 256, 0, 500)[1] >= 32
