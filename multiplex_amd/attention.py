@@ -525,6 +525,8 @@ class Attention(torch.nn.Module):
             raise ValueError("n_new needs a PagedKVCache")
         qkv = linear(x, self.qkv_proj)
         qg, k, v = qkv.split((2 * Hq * D, Hkv * D, Hkv * D), -1)
+        if pool is not None and B * T == 0:
+            return linear(x.new_empty(B, T, Hq * D), self.o_proj)
         if pool is not None:
             counts = None if n_new is None else cache.counts(n_new)
             slots = cache.reserve(T, n_new, counts)

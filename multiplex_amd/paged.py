@@ -194,6 +194,13 @@ def paged_attn(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, table:
     be the same and full (``pos0[b] >= shared * block``): their keys are read
     once for the batch.  ``n_split`` sets the key ranges of the prefix (0: with
     each row's own keys) and of a row's own keys; by default a rule does.
+    ``workspace``: bytes for the partial results of several ranges (allocated
+    when absent or too small); calls that overlap need one each.
+
+    v of a call's own tokens is taken to be finite: a token's inf or NaN there
+    reaches the earlier tokens of its row in the same call, as a weight of 0 times
+    it does in any product.  What the pools hold past a row's tokens, in padding
+    and in blocks of no row is never used.
     """
     dev = q.device
     index = q.get_device()
@@ -391,7 +398,10 @@ class PagedKVCache:
         return self._tables(self.pos0, self.lengths, T, self.counts(new) if counts is None else counts, new)
 
     def counts(self, n_new: Sequence[int]) -> torch.Tensor:
-        """Per-row counts on the device (through pinned memory: no launch waits)."""
+        """Per-row counts on the device (through pinned memory: no launch waits).
+        A captured graph would copy them from memory that is gone at its replay."""
+        if self.pool.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("per-row counts come from the host and cannot be captured into a graph")
         host = torch.tensor([int(n) for n in n_new], dtype=torch.int32)
         if self.pool.device.type != "cuda":
             return host

@@ -297,3 +297,73 @@ def test_attention_inf_scores():
         got = _np(out)
         assert (np.isnan(got).all(-1) == bad).all()
         assert _errs(got[~bad], ref[~bad]).max() < ATT_TOL
+
+
+def test_offsets_beyond_32_bits():
+    """A pool of 4.6e9 elements: the rows' blocks are its last and first ones, and
+    the result is that of a small pool, bit for bit."""
+    gen = torch.Generator().manual_seed(9)
+    B, T, heads, n = 3, 2, (16, 4, 256), 70000
+    q, gate, keys, values, table, pos0 = _attn_case(gen, B, T, heads, 64, 1, [70, 0, 200], None)
+    where = torch.tensor([0 if i == 0 else n - i for i in range(keys.shape[0])])
+    big = [torch.empty(n, heads[1], 64, heads[2], dtype=torch.bfloat16, device=DEV) for _ in range(2)]
+    for pool, small in zip(big, (keys, values)):
+        pool[where.to(DEV)] = small.to(DEV)
+    inside = (table >= 0) & (table < len(where))
+    far = np.where(inside, where.numpy()[np.where(inside, table, 0)], table)
+    args = dict(shared=1, gate=gate.flatten(2).to(DEV))
+    for split in ((0, 1), (2, 2)):
+        want = mx.paged_attn(q.to(DEV), keys.to(DEV), values.to(DEV), _i32(table), _i32(pos0), 300, n_split=split, **args)
+        got = mx.paged_attn(q.to(DEV), *big, _i32(far), _i32(pos0), 300, n_split=split, **args)
+        assert torch.equal(got, want)
+    # the rotary prep's writes
+    x = torch.randn(2, 1, (2 * 16 + 2 * 4) * 256, generator=gen).to(torch.bfloat16).to(DEV)
+    parts = x.split((2 * 16 * 256, 4 * 256, 4 * 256), -1)
+    slots = torch.tensor([[n * 64 - 1], [5]], dtype=torch.int32, device=DEV)
+    mx.attn_rope(*parts, None, None, 1e-6, _i32([0, 0]), *big, mx.Rotary(64, 1e4, device=DEV), slots=slots)
+    assert torch.equal(big[1][n - 1, :, 63], parts[2][0, 0].view(4, 256))
+    assert torch.equal(big[1][0, :, 5], parts[2][1, 0].view(4, 256))
+    assert torch.equal(big[0][n - 1, :, 63], parts[1][0, 0].view(4, 256))  # position 0, no norm: k as it is
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_attention_of_any_shape(seed):
+    """Random batches, heads, blocks, prefixes and padding, with the rule's key ranges and with others."""
+    rng = np.random.default_rng(100 + seed)
+    gen = torch.Generator().manual_seed(200 + seed)
+    Hkv = int(rng.integers(1, 5))
+    heads = (Hkv * int(rng.integers(1, 9)), Hkv, int(rng.choice([128, 256])))
+    B, T = int(rng.integers(1, 20)), int(rng.choice([1, 1, 2, 5, 17, 40]))
+    block, shared = int(rng.choice([64, 128, 256])), int(rng.integers(0, 6))
+    tails = rng.integers(0, 400, B).tolist()
+    n_new = rng.integers(0, T + 1, B).tolist() if rng.integers(0, 2) else None
+    q, gate, keys, values, table, pos0 = _attn_case(gen, B, T, heads, block, shared, tails, n_new)
+    L = max(p + (T if n_new is None else n) for p, n in zip(pos0, n_new or [T] * B))
+    ref = op.attend(_np(q), _np(keys), _np(values), table, pos0, heads[2] ** -0.5, n_new, _np(gate)[..., heads[2]:])
+    for split in (None, (int(rng.integers(0, 4)) if shared else 0, int(rng.integers(1, 5)))):
+        out = mx.paged_attn(q.to(DEV), keys.to(DEV), values.to(DEV), _i32(table), _i32(pos0), L, shared=shared,
+                            n_new=None if n_new is None else _i32(n_new), gate=gate.flatten(2).to(DEV), n_split=split)
+        torch.cuda.synchronize()
+        for b in range(B):
+            n = T if n_new is None else n_new[b]
+            assert _errs(_np(out[b, :n]), ref[b, :n]).max(initial=0) < ATT_TOL, (b, split)
+            assert not out[b, n:].any()
+
+
+def test_strided_inputs_and_given_outputs():
+    """q as a strided view, the gate as a column slice, out and workspace given (one too small)."""
+    gen = torch.Generator().manual_seed(21)
+    B, T, heads = 3, 2, (16, 4, 256)
+    q, gate, keys, values, table, pos0 = _attn_case(gen, B, T, heads, 64, 1, [70, 0, 200], None)
+    args = (keys.to(DEV), values.to(DEV), _i32(table), _i32(pos0), 300)
+    want = mx.paged_attn(q.to(DEV), *args, shared=1, gate=gate.flatten(2).to(DEV), n_split=(1, 2))
+    wide = torch.zeros(B, T, 16 * 512 + 64, dtype=torch.bfloat16, device=DEV)
+    wide[..., :16 * 512] = gate.flatten(2).to(DEV)
+    strided = torch.zeros(B, T, 16, 512, dtype=torch.bfloat16, device=DEV)
+    strided[..., :256] = q.to(DEV)
+    out = torch.empty(B, T, 16, 256, dtype=torch.bfloat16, device=DEV)
+    for nbytes in (8, 1 << 24):
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=DEV)
+        got = mx.paged_attn(strided[..., :256], *args, shared=1, gate=wide[..., :16 * 512], n_split=(1, 2), out=out,
+                            workspace=ws)
+        assert got is out and torch.equal(out, want)

@@ -214,3 +214,35 @@ def test_two_workspaces_on_two_streams():
             outs.append(_step(s, 1))
     torch.cuda.synchronize()
     assert all(torch.equal(o, w) for o, w in zip(outs, want))
+
+
+@pytest.mark.parametrize("T", [1, 300])
+def test_a_batch_of_no_rows(T):
+    layer = mx.Attention(mx.AttentionArgs(**ARGS), DEV)
+    cache = mx.PagedKVCache(mx.BlockPool(4, 2, 128, 64, DEV), 0)
+    assert layer(torch.empty(0, T, 512, dtype=BF, device=DEV), cache).shape == (0, T, 512)
+    assert cache.offset == 0 and cache.pool.free_blocks == 4
+
+
+def test_counts_are_not_captured():
+    cache = mx.PagedKVCache(mx.BlockPool(4, 2, 128, 64, DEV), 2)
+    cache.reserve(2, [1, 2])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="captured"):
+            cache.reserve(2, [1, 2])
+
+
+def test_rows_past_the_batch_are_left_alone():
+    """Buffers longer than the batch (views of a serving loop's largest): what lies behind stays."""
+    i32 = dict(dtype=torch.int32, device=DEV)
+    lengths, held, slots = torch.full((6,), 3, **i32), torch.full((6,), 9, **i32), torch.full((6, 2), 77, **i32)
+    table = torch.full((6, 4), 55, **i32)
+    held[:2] = 0
+    free, n_free = torch.arange(8, **i32), torch.full((1,), 8, **i32)
+    mx.paged_tables(lengths[:2], 2, table[:2], held[:2], free, n_free, 4, slots=slots[:2], held_out=held[:2],
+                    n_free_out=n_free)
+    assert held.tolist() == [2, 2, 9, 9, 9, 9] and (table[2:] == 55).all() and (slots[2:] == 77).all()
+    assert table[:2].tolist() == [[7, 6, 55, 55], [5, 4, 55, 55]] and n_free.item() == 4
+    assert slots[:2].tolist() == [[31, 24], [23, 16]]

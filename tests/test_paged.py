@@ -545,3 +545,32 @@ def test_ranges_read_a_long_prefix_once():
     assert paged._ranges(256, 1, 1, 16, 4, 256, 128, 8)[0] == 0
     assert paged._ranges(256, 4, 512, 16, 4, 256, 64, 10)[0] == 0
     assert paged._ranges(256, 1, 1, 16, 4, 256, 0, 500)[1] >= 32
+
+
+def test_launches_enter_their_tensors_device(monkeypatch):
+    """Another device than the current one: every launch is made with it current."""
+    import contextlib
+
+    inside, made = [], []
+
+    @contextlib.contextmanager
+    def enter(dev):
+        inside.append(dev)
+        yield
+        inside.pop()
+
+    class Library:
+        def __getattr__(self, name):
+            return lambda *args: made.append((name, len(inside))) or _lib.OK
+
+    monkeypatch.setattr(_lib, "_current_device", lambda: 0)
+    monkeypatch.setattr(torch.cuda, "device", enter)
+    monkeypatch.setattr(_lib, "_lib", Library())
+    for mod in (paged, rotary):
+        monkeypatch.setattr(mod, "_stream", lambda dev: 0)
+        monkeypatch.setattr(mod, "_require_device", lambda tensors, names: torch.device("cpu"))
+    monkeypatch.setattr(paged, "_cu_count", lambda dev: 256)
+    mx.paged_tables(**_tables_args())
+    mx.attn_rope(**_rope_args())
+    mx.paged_attn(**_attn_args())
+    assert made == [("gdn_paged_tables", 1), ("gdn_attn_rope", 1), ("gdn_paged_attn", 1)]
