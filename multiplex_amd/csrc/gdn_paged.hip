@@ -580,11 +580,13 @@ __device__ __forceinline__ void attn_rows(const PagedParams& p, unsigned char* s
 
   // the waves' states merge: thread (row, column piece)
   __syncthreads();
-  float* Os = reinterpret_cast<float*>(smem);  // [W][16][D]
-  float* Ms = Os + W * 16 * D;                 // [W][16]
+  // [W][16][D], a row's 16-byte granules XOR-swizzled by the row: unswizzled, the accumulators' 16 rows lie in the
+  // same banks, and the merge took 4.2 us, not 1.1
+  f32x4* Os = reinterpret_cast<f32x4*>(smem);
+  float* Ms = reinterpret_cast<float*>(smem) + W * 16 * D;  // [W][16]
   float* Ls = Ms + W * 16;
 #pragma unroll
-  for (int j = 0; j < NJ; ++j) *reinterpret_cast<f32x4*>(&Os[(wave * 16 + lr) * D + 16 * j + 4 * lq]) = o[j];
+  for (int j = 0; j < NJ; ++j) Os[(wave * 16 + lr) * (D / 4) + ((4 * j + lq) ^ lr)] = o[j];
   if (lq == 0) {
     Ms[wave * 16 + lr] = m;
     Ls[wave * 16 + lr] = l;
@@ -616,7 +618,7 @@ __device__ __forceinline__ void attn_rows(const PagedParams& p, unsigned char* s
     acc[c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int w = 0; w < W; ++w)
-      acc[c] += mw[w] * *reinterpret_cast<const f32x4*>(&Os[(w * 16 + mr) * D + c0 + 16 * W * c]);
+      acc[c] += mw[w] * Os[(w * 16 + mr) * (D / 4) + ((c0 / 4 + 4 * W * c) ^ mr)];
   }
   if (p.n_split == 1) {
     store_row<D, CW / 4, 16 * W>(p, (mat.b * p.T + mat.t) * p.Hq + mat.hq, c0, acc, ls);
