@@ -121,11 +121,11 @@ def _cu_count(dev: torch.device) -> int:
 # partial results takes, and per MB of them; the share of kv_len_max that rows
 # hold on average; the share of a workgroup's time that more workgroups than fit
 # at once add.  At head dims up to 128 and 256 (two workgroups a CU, and one).
-# Fitted to graph-replayed times of 3000 sizes (the four head layouts of 4 to 8
-# query heads a group and 128 or 256 dims, 1 to 128 rows, 1 to 512 tokens, prefixes
-# to 16384 and rows' own keys to 32768), 16 choices each; at 13000 others its choice
-# is 3 to 4% slower than the best of them on average, 10 to 14% at one in ten.
-_US = ((6.3, 1.00, 7.3, 1.22, 3.9, 0.36, 0.79, 0.58), (9.7, 1.31, 11.4, 1.54, 4.3, 0.31, 0.76, 0.49))
+# Fitted to graph-replayed times of 3000 sizes (four head layouts of 3 to 8 query
+# heads a group and 128 or 256 dims, 1 to 128 rows, 1 to 512 tokens, prefixes to
+# 16384 and rows' own keys to 32768), 16 choices each; at 5500 others its choice is
+# 3 to 4% slower than the best of them on average, 9 to 13% at one in ten.
+_US = ((5.6, 1.03, 7.4, 1.22, 3.8, 0.36, 0.78, 0.55), (7.1, 1.31, 11.4, 1.57, 4.3, 0.31, 0.74, 0.49))
 _PREFIX_RANGES = (0, 1, 2, 3, 4, 6, 8, 12, 16, 20, 24, 32, 48, 64)
 _OWN_RANGES = (1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128, 256)
 
@@ -138,8 +138,9 @@ def _ranges(cus: int, B: int, T: int, Hq: int, Hkv: int, D: int, prefix: int, ow
     The prefix read once takes work from every row, but leaves partial results
     to merge; ranges make workgroups enough, each at a price.  So the choice is
     the least of the times that :data:`_US` gives.  (Decode of 64 rows of 16
-    heads of 256 behind 8192 keys, up to 512 of their own, us: with the rows' own
-    112, in 4 / 12 / 32 ranges 66 / 39 / 53; 4 rows behind 2048: 29, in 16 ranges 16.)
+    heads of 256 behind 8192 keys and up to 512 of their own, us: without a pass
+    of the prefix 110, with it in 4 / 16 / 32 ranges 67 / 37.5 / 51; 4 rows behind
+    2048: 15.3, in 12 ranges 13.8.)
     """
     rows = T * (Hq // Hkv)
     few, few_step, many, many_step, merge, merge_mb, filled, crowd = _US[D > 128]
