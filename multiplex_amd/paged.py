@@ -118,14 +118,15 @@ def _cu_count(dev: torch.device) -> int:
 
 # us that a workgroup takes, before its first and after its last keys and per step
 # of them: 16 rows (128 keys a step), 128 rows (64 keys); us that the merge of the
-# partial results takes, and per MB of them; the share of kv_len_max that rows
-# hold on average; the share of a workgroup's time that more workgroups than fit
-# at once add.  At head dims up to 128 and 256 (two workgroups a CU, and one).
-# Fitted to graph-replayed times of 3000 sizes (four head layouts of 3 to 8 query
-# heads a group and 128 or 256 dims, 1 to 128 rows, 1 to 512 tokens, prefixes to
-# 16384 and rows' own keys to 32768), 16 choices each; at 5500 others its choice is
-# 3 to 4% slower than the best of them on average, 9 to 13% at one in ten.
-_US = ((5.6, 1.03, 7.4, 1.22, 3.8, 0.36, 0.78, 0.55), (7.1, 1.31, 11.4, 1.57, 4.3, 0.31, 0.74, 0.49))
+# partial results takes, and per MB of them; how much of the time between a full
+# row's and the average row's the workgroups take on average.  At head dims up to
+# 128 and 256 (two workgroups a CU, and one).  Fitted to graph-replayed times of
+# 3000 sizes (four head layouts of 3 to 8 query heads a group, 1 to 128 rows, 1 to
+# 512 tokens, prefixes to 16384 and rows' own keys to 32768), 16 choices each; at
+# 5500 others its choice is 3 to 4% slower than the best of them on average, 8 to
+# 13% at one in ten.
+_US = ((5.2, 1.01, 7.2, 1.24, 4.1, 0.37, 0.25), (6.4, 1.27, 11.1, 1.54, 4.9, 0.30, 0.17))
+_MB_US = 5.5  # MB a us from memory
 _PREFIX_RANGES = (0, 1, 2, 3, 4, 6, 8, 12, 16, 20, 24, 32, 48, 64)
 _OWN_RANGES = (1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128, 256)
 
@@ -143,8 +144,9 @@ def _ranges(cus: int, B: int, T: int, Hq: int, Hkv: int, D: int, prefix: int, ow
     2048: 15.3, in 12 ranges 13.8.)
     """
     rows = T * (Hq // Hkv)
-    few, few_step, many, many_step, merge, merge_mb, filled, crowd = _US[D > 128]
+    few, few_step, many, many_step, merge, merge_mb, full = _US[D > 128]
     slots = cus * (1 if D > 128 else 2)
+    read = few + 256e-6 * Hkv * D * (prefix + B * own / 2) / _MB_US  # the keys and values, rows half full
 
     def groups(n_rows, blocks, n):
         """Workgroups of a kv-head, and us that one takes."""
@@ -158,19 +160,26 @@ def _ranges(cus: int, B: int, T: int, Hq: int, Hkv: int, D: int, prefix: int, ow
     for p in _PREFIX_RANGES:
         if p and (B == 1 or rows >= 256 or p > prefix):
             break
-        own_p = own if p else own + prefix
-        if p:
-            n_p, us_p = groups(B * rows, prefix, p)
-            n_p *= Hkv
+        own_p = max(own if p else own + prefix, 1)
+        n_p, us_p = groups(B * rows, prefix, p) if p else (0, 0.0)
+        whole, rest = divmod(n_p * Hkv, slots)  # the prefix's workgroups go first, in rounds of all slots
+        fill = 1.0 - own / (2 * own_p)
         for o in _OWN_RANGES:
             if o > 1 and 2 * o > own_p or p and o > 8:
                 break
-            n_o, us = groups(rows, max(own_p, 1), o)
-            n_o *= B * Hkv
-            busy, last, n = n_o * us * filled, us, n_o
-            if p:
-                busy, last, n, us = busy + n_p * us_p, max(us, us_p), n + n_p, min(us, us_p)
-            t = max(last, busy / slots) + (crowd * us if n > slots else 0.0)
+            n_o, us = groups(rows, own_p, o)
+            n_o *= max(B, 1) * Hkv
+            mean = us * (full + (1.0 - full) * fill)
+            free = slots - rest  # beside the prefix's last round
+            rounds = us_p // mean if rest else 0.0
+            if rest and n_o <= free * rounds:
+                t = max(us_p, (-(-n_o // free) - 1) * mean + us)
+            elif rest:
+                left = -(-max(n_o - free * (rounds + 1), 0) // slots)
+                t = max(us_p + (left * mean + us - mean if left else 0.0), rounds * mean + us)
+            else:
+                t = (-(-n_o // slots) - 1) * mean + us
+            t = max(whole * us_p + t, read)
             if p + o > 1:
                 t += merge + merge_mb * 4e-6 * B * T * Hq * D * (p + o)
             if best is None or t < best:
