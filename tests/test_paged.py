@@ -574,3 +574,58 @@ def test_launches_enter_their_tensors_device(monkeypatch):
     mx.attn_rope(**_rope_args())
     mx.paged_attn(**_attn_args())
     assert made == [("gdn_paged_tables", 1), ("gdn_attn_rope", 1), ("gdn_paged_attn", 1)]
+
+
+# ------------------------------------------------- what pins the oracle
+
+@pytest.mark.parametrize("rot,base,scaling", [
+    (64, 1e7, dict(type="yarn", factor=4.0, original_max_position_embeddings=32768)),
+    (128, 1e6, dict(type="yarn", factor=40.0, original_max_position_embeddings=4096, beta_fast=16.0, beta_slow=2.0)),
+])
+def test_oracle_frequencies_are_transformers(rot, base, scaling):
+    """float32 there: 2^-24 per operation, a few of them."""
+    utils = pytest.importorskip("transformers.modeling_rope_utils")
+    from transformers import PretrainedConfig
+
+    c = PretrainedConfig()
+    c.rope_theta, c.head_dim, c.hidden_size, c.num_attention_heads = base, rot, 4 * rot, 4
+    c.max_position_embeddings = int(scaling["factor"] * scaling["original_max_position_embeddings"])
+    c.rope_parameters = c.rope_scaling = {**scaling, "rope_type": scaling["type"], "rope_theta": base}
+    inv, factor = utils.ROPE_INIT_FUNCTIONS["yarn"](c, torch.device("cpu"))
+    ours, mag = op.frequencies(rot, base, scaling)
+    np.testing.assert_allclose(inv.double().numpy(), ours, rtol=1e-6)
+    assert mag == pytest.approx(factor, rel=1e-12)
+
+
+def test_oracle_rotation_is_the_dense_oracles():
+    from oracle import attention as oa
+
+    rng = np.random.default_rng(1)
+    x, w, pos = rng.standard_normal((5, 3, 128)), rng.standard_normal(128), np.arange(5) + 17
+    inv, factor = op.frequencies(32, 1e4)
+    want = oa.rope(oa.rms_norm(x, w, 1e-6)[None], pos[None], 32, 1e4)[0]
+    np.testing.assert_allclose(op.norm_rotate(x, w, 1e-6, pos, inv, factor, False), want, atol=1e-12)
+    # neighbouring pairs are one complex number each
+    y = op.norm_rotate(x, None, 0.0, pos, inv, 1.5, True)
+    z = (x[..., 0:32:2] + 1j * x[..., 1:32:2]) * np.exp(1j * pos[:, None, None] * inv) * 1.5
+    np.testing.assert_allclose(y[..., 0:32:2] + 1j * y[..., 1:32:2], z, atol=1e-12)
+    np.testing.assert_array_equal(y[..., 32:], x[..., 32:])
+
+
+def test_oracle_attention_is_the_dense_softmax():
+    rng = np.random.default_rng(2)
+    B, T, Hq, Hkv, D, block = 2, 3, 4, 2, 8, 4
+    pos0, n_new = [6, 0], [3, 2]
+    keys, values = rng.standard_normal((2, 9, Hkv, block, D))
+    table = np.array([[4, 7, 2], [8, 0, 1]])
+    q, gate = rng.standard_normal((2, B, T, Hq, D))
+    out = op.attend(q, keys, values, table, pos0, 0.3, n_new, gate)
+    for b in range(B):
+        k = torch.from_numpy(keys[table[b]]).transpose(0, 1).reshape(Hkv, -1, D).repeat_interleave(2, 0)
+        v = torch.from_numpy(values[table[b]]).transpose(0, 1).reshape(Hkv, -1, D).repeat_interleave(2, 0)
+        n = n_new[b]
+        sees = torch.arange(k.shape[1]) <= pos0[b] + torch.arange(n)[:, None]
+        s = (torch.from_numpy(q[b, :n]).transpose(0, 1) @ k.transpose(1, 2) * 0.3).masked_fill(~sees, -math.inf)
+        want = (s.softmax(-1) @ v).transpose(0, 1) * torch.from_numpy(gate[b, :n]).sigmoid()
+        np.testing.assert_allclose(out[b, :n], want.numpy(), atol=1e-12)
+        assert not out[b, n:].any()
