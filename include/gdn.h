@@ -470,9 +470,10 @@ size_t gdn_paged_attn_workspace_bytes(int64_t B, int64_t T, int64_t Hq, int64_t 
  *   n_own    key ranges of a row's own keys
  *   kv_len_max  host bound of pos0[b] + n_new[b], in [shared * block + T (0 where
  *            n_new is given), table_ld * block]
- * block: a power of two from 64 on; B <= 65535.  v of a row's new tokens is taken
- * to be finite (gdn_attn_fwd's too): a weight of 0 times inf or NaN is NaN.  Calls
- * that overlap need a workspace each.  Other arguments as in gdn_attn_fwd.
+ * block: a power of two from 64 on; table_ld * block <= 2^30; B <= 65535.  v of a
+ * row's new tokens is taken to be finite (gdn_attn_fwd's too): a weight of 0 times
+ * inf or NaN is NaN.  Calls that overlap need a workspace each.  Other arguments as
+ * in gdn_attn_fwd.
  */
 int gdn_paged_attn(const void* q, const void* qg, int64_t qg_ld, const void* keys, const void* values,
                    const int32_t* table, int64_t table_ld, const int32_t* pos0, const int32_t* n_new,

@@ -75,7 +75,7 @@ struct PagedParams : AttnParams {
   const int32_t* n_new;  // [B] or null: T
   int table_ld, lg, n_blocks, key0, prefix;
   int split0;  // the launch's first key range of the row's n_split
-  int reread;  // rows' own keys start with the shared ones: other rows read them too
+  int pos_min;  // the shared keys, which every row has; above key0, rows read them too as their own
 };
 
 // A value that no kernel of this library's call writes, by a scalar load where
@@ -92,10 +92,10 @@ __device__ __forceinline__ int row_tokens(const P& p, int b) {
 }
 
 // Position of a row's first new token: the keys it finds in the cache, clamped
-// like first_pos (and not below the keys all rows share).
+// like first_pos (and not below the keys all rows share, however they are read).
 template <class P>
 __device__ __forceinline__ int row_start(const P& p, int b, int tokens) {
-  if constexpr (P::kPaged) return p.prefix ? p.key0 : min(max(const_i32(p.pos0, b), p.key0), p.cap - tokens);
+  if constexpr (P::kPaged) return p.prefix ? p.key0 : min(max(const_i32(p.pos0, b), p.pos_min), p.cap - tokens);
   else return first_pos(p.pos0, b, p.T, p.cap);
 }
 

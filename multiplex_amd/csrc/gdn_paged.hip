@@ -464,8 +464,8 @@ __device__ __forceinline__ void attn_rows(const PagedParams& p, unsigned char* s
   const int row0 = lane / KROW, gran = lane % KROW;
   static_assert(64 % KROW == 0, "whole rows per load");
   constexpr int RL = 64 / KROW;  // rows per load
-  // a row's own keys are read by one workgroup
-  const bool once = !prefix_of(p) && !p.reread;
+  // a row's own keys are read by one workgroup, where none of them are shared
+  const bool once = !prefix_of(p) && p.pos_min == p.key0;
   auto load = [&](const uint16_t* pool, int i, uint32_t lds, int twist) {
     const int kb = k_lo + KS * i;
     const int64_t off = key_off<D>(p, b, hkv, kb, __builtin_amdgcn_readlane(pages, i - page0)) * 2;
@@ -868,7 +868,8 @@ extern "C" int gdn_paged_attn(const void* q, const void* qg, int64_t qg_ld, cons
       !gdn_host::aligned(out, 8) || (qg && (!gdn_host::aligned(qg, 8) || qg_ld % 4 != 0)))
     return fail(GDN_ERR_INVALID, "gdn_paged_attn: misaligned pointer");
   const int64_t g = Hq / Hkv, rows = T * g, n_split = n_prefix + n_own;
-  if (B > 65535 || B * T * Hq > INT32_MAX / 2 || Hkv * n_split > INT32_MAX ||
+  // (ranges of up to 65535 are rounded up to steps, and asked for a step of all lanes ahead: 2^30 keys leave room)
+  if (table_ld * block > (int64_t(1) << 30) || B > 65535 || B * T * Hq > INT32_MAX / 2 || Hkv * n_split > INT32_MAX ||
       B * Hkv * rows * n_split * (D + 2) > (int64_t(1) << 40))
     return fail(GDN_ERR_UNSUPPORTED, "gdn_paged_attn: problem too large");
   const size_t need = gdn_paged_attn_workspace_bytes(B, T, Hq, Hkv, D, n_split);
@@ -899,7 +900,7 @@ extern "C" int gdn_paged_attn(const void* q, const void* qg, int64_t qg_ld, cons
   p.n_blocks = static_cast<int>(n_blocks);
   hipStream_t st = static_cast<hipStream_t>(stream);
   p.key0 = static_cast<int>(n_prefix > 0 ? shared * block : 0);
-  p.reread = n_prefix == 0 && shared > 0;
+  p.pos_min = static_cast<int>(shared * block);
   auto range_len = [](int64_t keys, int64_t n) { return static_cast<int>(((keys + n - 1) / n + KB - 1) / KB * KB); };
   p.n_prefix = static_cast<int>(n_prefix);
   p.n_own = static_cast<int>(n_own);

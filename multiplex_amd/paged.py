@@ -228,7 +228,7 @@ def paged_attn(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, table:
             and (n_new is None or _is_i32(n_new, row, index))
             and 0 <= shared * block <= kv_len_max - (T if n_new is None else 0) and kv_len_max <= width * block
             and (gate is None or (gate.dtype is bf16 and gate.shape == (B, T, Hq * 2 * D) and gate.get_device() == index))
-            and (workspace is None or workspace.get_device() == index)
+            and (workspace is None or workspace.get_device() == index and workspace.is_contiguous())
             and (out is None or (out.dtype is bf16 and out.shape == q.shape and out.get_device() == index
                                  and out.is_contiguous()))):
         _refuse_attn(q, keys, values, table, pos0, kv_len_max, n_new, shared, gate, workspace, out)
@@ -280,6 +280,8 @@ def _refuse_attn(q, keys, values, table, pos0, kv_len_max, n_new, shared, gate, 
         raise ValueError(f"kv_len_max={kv_len_max} must lie in [shared * block + T, width * block = {width * block}]")
     if gate is not None and gate.shape != (B, T, Hq * 2 * D):
         raise ValueError(f"gate must be [{B}, {T}, {Hq * 2 * D}]")
+    if workspace is not None and not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous")
     if out is not None and (out.shape != q.shape or not out.is_contiguous()):
         raise ValueError(f"out must be a contiguous [{B}, {T}, {Hq}, {D}] tensor")
 

@@ -279,6 +279,19 @@ def test_attention_matches_oracle(name):
         assert not out[b, n:].any()
 
 
+@pytest.mark.parametrize("T,n_split", [(1, (0, 1)), (1, (0, 3)), (1, (2, 1)), (40, (0, 1)), (40, (1, 2))])
+def test_positions_below_the_shared_keys(T, n_split):
+    """A position below the shared keys' end is read as that end, whether or not
+    the shared keys are read apart."""
+    heads, block, shared, tails = (16, 4, 256), 64, 2, [0, 5]
+    q, _, keys, values, table, pos0 = _attn_case(torch.Generator().manual_seed(17), 2, T, heads, block, shared, tails, None)
+    given = [pos0[0] - 30, pos0[1]]
+    out = mx.paged_attn(q.to(DEV), keys.to(DEV), values.to(DEV), _i32(table), _i32(given), max(pos0) + T, shared=shared,
+                        n_split=n_split)
+    ref = op.attend(_np(q), _np(keys), _np(values), table, pos0, 256 ** -0.5)
+    assert _errs(_np(out), ref).max() < ATT_TOL
+
+
 def test_attention_inf_scores():
     """A row whose every score is -inf is NaN, one with a +inf score too, as the
     softmax of such scores is; their neighbours are untouched."""

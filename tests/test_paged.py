@@ -242,6 +242,18 @@ def test_attention_refusals(calls, kw):
     assert calls == ["gdn_paged_attn"] * 2
 
 
+def test_attention_workspace_must_be_whole(calls):
+    with pytest.raises(ValueError, match="workspace"):
+        mx.paged_attn(**_attn_args(workspace=_z(1 << 20)[::2]))
+    assert not calls
+
+
+def test_attention_tables_of_too_many_keys(lib):
+    """Ranges are rounded up to steps and looked up a step of all lanes ahead, in 32 bits."""
+    assert _attn(lib, ld=(1 << 24) + 1, L=1 << 30) == _lib.ERR_UNSUPPORTED
+    assert _attn(lib, ld=(1 << 25) - 1, L=2**31 - 64) == _lib.ERR_UNSUPPORTED
+
+
 def test_tensors_must_be_on_a_device():
     with pytest.raises(ValueError, match="ROCm"):
         mx.paged_tables(**_tables_args())
