@@ -629,24 +629,49 @@ __device__ __forceinline__ void attn_tile(const P& p, unsigned char* smem, int b
     }
   };
   auto load_q = [&]() {
+    if constexpr (P::kPaged) {
+      // whole rows straight into the V stages' LDS, as K's blocks are, then as fragments from there (as fragments
+      // from memory, 64 bytes of a row at a time, a workgroup takes 1.8 us more at D = 256; at 128 as long)
+      static_assert(PR * D * 2 <= 2 * VSTAGE, "the rows must fit in the V stages");
+      constexpr int RL = 64 / KROW, QI = PR / (NT / KROW);  // rows per load, loads per wave
+      const int first = __builtin_amdgcn_readfirstlane(row_out[0]);
+      const int last = __builtin_amdgcn_readfirstlane(row_out[min(PR, n_rows - row0) - 1]);
+      const u32x4 rsrc = buf_words(p.q + static_cast<int64_t>(first) * D, (last - first + 1) * (D * 2));
+      const uint32_t qs = __builtin_amdgcn_readfirstlane(
+          static_cast<uint32_t>(reinterpret_cast<uintptr_t>(smem)) + 2 * KSTAGE + wave * (QI * 1024));
+#pragma unroll
+      for (int i = 0; i < QI; ++i) {
+        const int r = (wave * QI + i) * RL + lane / KROW;
+        const uint32_t row = max(row_out[r], first) - first;  // (past the end: the first, not stored)
+        lds_dma16(rsrc, row * (D * 2) + (((lane % KROW) ^ (r & 7)) * 16), qs + i * 1024);
+      }
+      asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" : : : "memory");
+#pragma unroll
+      for (int rt = 0; rt < 2; ++rt) {
+        const int r = 32 * rg + 16 * rt + lr;
+        kmax[rt] = row_kmax[r];
+        const bool ok = kmax[rt] >= 0;
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+          const u32x4 x = *reinterpret_cast<const u32x4*>(smem + 2 * KSTAGE + r * (D * 2) + ((4 * s + lq) ^ (r & 7)) * 16);
+          const bf16x8 f = __builtin_bit_cast(bf16x8, ok ? x : u32x4{0u, 0u, 0u, 0u});
+          if (s < NS - QL) qf[rt][s] = f;
+          else if (kh == 0) *q_lds(rt, s) = f;
+        }
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory");  // the stages are free
+      return;
+    }
     u32x4 v[2][NS];
     bool ok[2];
 #pragma unroll
     for (int rt = 0; rt < 2; ++rt) {
-      const uint16_t* qrow;
-      if constexpr (P::kPaged) {
-        const int r = 32 * rg + 16 * rt + lr;
-        kmax[rt] = row_kmax[r];
-        ok[rt] = kmax[rt] >= 0;
-        qrow = p.q + static_cast<int64_t>(max(row_out[r], 0)) * D;
-      } else {
-        const int r = row0 + 32 * rg + 16 * rt + lr;
-        const RowAt at = row_at(p, b, hkv, g, min(r, n_rows - 1));
-        ok[rt] = r < n_rows;
-        const int hq = ok[rt] ? at.hq : hkv * g;
-        kmax[rt] = p0 + at.t;
-        qrow = p.q + ((static_cast<int64_t>(at.b) * p.T + at.t) * p.Hq + hq) * D;
-      }
+      const int r = row0 + 32 * rg + 16 * rt + lr;
+      const RowAt at = row_at(p, b, hkv, g, min(r, n_rows - 1));
+      ok[rt] = r < n_rows;
+      const int hq = ok[rt] ? at.hq : hkv * g;
+      kmax[rt] = p0 + at.t;
+      const uint16_t* qrow = p.q + ((static_cast<int64_t>(at.b) * p.T + at.t) * p.Hq + hq) * D;
 #pragma unroll
       for (int s = 0; s < NS; ++s) v[rt][s] = *reinterpret_cast<const u32x4*>(qrow + 32 * s + 8 * lq);
     }

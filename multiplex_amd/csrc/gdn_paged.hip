@@ -869,7 +869,7 @@ extern "C" int gdn_paged_attn(const void* q, const void* qg, int64_t qg_ld, cons
     return fail(GDN_ERR_INVALID, "gdn_paged_attn: misaligned pointer");
   const int64_t g = Hq / Hkv, rows = T * g, n_split = n_prefix + n_own;
   // (ranges of up to 65535 are rounded up to steps, and asked for a step of all lanes ahead: 2^30 keys leave room)
-  if (table_ld * block > (int64_t(1) << 30) || B > 65535 || B * T * Hq > INT32_MAX / 2 || Hkv * n_split > INT32_MAX ||
+  if (table_ld * block > (int64_t(1) << 30) || Hkv > 16384 || B > 65535 || B * T * Hq > INT32_MAX / 2 || Hkv * n_split > INT32_MAX ||
       B * Hkv * rows * n_split * (D + 2) > (int64_t(1) << 40))
     return fail(GDN_ERR_UNSUPPORTED, "gdn_paged_attn: problem too large");
   const size_t need = gdn_paged_attn_workspace_bytes(B, T, Hq, Hkv, D, n_split);

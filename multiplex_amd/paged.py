@@ -121,11 +121,11 @@ def _cu_count(dev: torch.device) -> int:
 # partial results takes, and per MB of them; how much of the time between a full
 # row's and the average row's the workgroups take on average.  At head dims up to
 # 128 and 256 (two workgroups a CU, and one).  Fitted to graph-replayed times of
-# 3000 sizes (four head layouts of 3 to 8 query heads a group, 1 to 128 rows, 1 to
+# 7000 sizes (four head layouts of 3 to 8 query heads a group, 1 to 128 rows, 1 to
 # 512 tokens, prefixes to 16384 and rows' own keys to 32768), 16 choices each; at
-# 5500 others its choice is 3 to 4% slower than the best of them on average, 8 to
-# 13% at one in ten.
-_US = ((5.2, 1.01, 7.2, 1.24, 4.1, 0.37, 0.25), (6.4, 1.27, 11.1, 1.54, 4.9, 0.30, 0.17))
+# 19000 its choice is 3% slower than the best of them on average, 9 to 10% at one
+# in ten.
+_US = ((5.2, 1.01, 7.2, 1.24, 4.1, 0.37, 0.25), (6.5, 1.23, 10.5, 1.52, 4.7, 0.28, 0.17))
 _MB_US = 5.5  # MB a us from memory
 _PREFIX_RANGES = (0, 1, 2, 3, 4, 6, 8, 12, 16, 20, 24, 32, 48, 64)
 _OWN_RANGES = (1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128, 256)
