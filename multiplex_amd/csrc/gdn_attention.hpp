@@ -558,13 +558,18 @@ __device__ __forceinline__ float wave_max(float x) {
 constexpr int kPrefillRows = 512;  // rows (tokens x heads of a group) per kv-head from which it is used
 constexpr int PR = 128;            // rows per workgroup
 constexpr int VTP = KB;            // Vt row stride (bf16); 16-byte granules XOR-swizzled by (d & 7)
+// bytes between 8 rows of K and the next 8.  A fragment's read takes 16 rows' granules a cycle: XOR-swizzled by
+// (key & 7) they lie in half of the banks, the pad moves every other 8 rows to the other half (279 -> 480 B/ns a CU)
+constexpr int K_PAD = 128;
+template <int D>
+constexpr int k_stage() { return KB * D * 2 + KB / 8 * K_PAD; }
 
 // k-steps of q kept in LDS: as many as leave the loop without a spill
 template <int KG, class P>
 constexpr int q_lds_steps() { return KG == 2 ? (P::kPaged ? 3 : 2) : 0; }
 template <int D, int KG, class P>
 constexpr int tile_lds() {
-  return 2 * (KB * D * 2 + D * VTP * 2) + (KG == 2 ? 8 * 128 * 4 : 0) + 4 * 2 * q_lds_steps<KG, P>() * 1024 +
+  return 2 * (k_stage<D>() + D * VTP * 2) + (KG == 2 ? 8 * 128 * 4 : 0) + 4 * 2 * q_lds_steps<KG, P>() * 1024 +
          (P::kPaged ? 3 * PR * 4 : 0);
 }
 
@@ -580,7 +585,7 @@ __device__ __forceinline__ void attn_tile(const P& p, unsigned char* smem, int b
   constexpr int KROW = D / 8;                 // 16-byte granules per K row
   constexpr int KDMA = KB * KROW / NT;        // direct loads per thread and K block
   constexpr int VPAIRS = (KB / 4) * KROW / NT;  // (key quad, d octet) pairs per thread and V block
-  constexpr int KSTAGE = KB * D * 2;          // bytes
+  constexpr int KSTAGE = k_stage<D>();        // bytes
   constexpr int VSTAGE = D * VTP * 2;
   static_assert(KDMA * NT == KB * KROW && VPAIRS * NT == (KB / 4) * KROW, "block must split evenly over the threads");
   static_assert(KDMA <= NS && 4 * VPAIRS <= NS, "at most one K and one V load per k-step");
@@ -643,7 +648,7 @@ __device__ __forceinline__ void attn_tile(const P& p, unsigned char* smem, int b
       for (int i = 0; i < QI; ++i) {
         const int r = (wave * QI + i) * RL + lane / KROW;
         const uint32_t row = max(row_out[r], first) - first;  // (past the end: the first, not stored)
-        lds_dma16(rsrc, row * (D * 2) + (((lane % KROW) ^ (r & 7)) * 16), qs + i * 1024);
+        lds_dma16(rsrc, row * (D * 2) + (((lane % KROW) ^ (r & 15)) * 16), qs + i * 1024);
       }
       asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" : : : "memory");
 #pragma unroll
@@ -653,7 +658,7 @@ __device__ __forceinline__ void attn_tile(const P& p, unsigned char* smem, int b
         const bool ok = kmax[rt] >= 0;
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
-          const u32x4 x = *reinterpret_cast<const u32x4*>(smem + 2 * KSTAGE + r * (D * 2) + ((4 * s + lq) ^ (r & 7)) * 16);
+          const u32x4 x = *reinterpret_cast<const u32x4*>(smem + 2 * KSTAGE + r * (D * 2) + ((4 * s + lq) ^ lr) * 16);
           const bf16x8 f = __builtin_bit_cast(bf16x8, ok ? x : u32x4{0u, 0u, 0u, 0u});
           if (s < NS - QL) qf[rt][s] = f;
           else if (kh == 0) *q_lds(rt, s) = f;
@@ -710,19 +715,19 @@ __device__ __forceinline__ void attn_tile(const P& p, unsigned char* smem, int b
     }
   };
   auto block_bytes = [&](int kb) { return min(k_hi - kb, KB) * (D * 2); };
-  // K block -> stage st: thread tid's load i fills physical granule i * NT + tid, which is row
-  // i * KR + tid / KROW, granule (tid % KROW) ^ (row & 7) of the block (the swizzle does not depend on i)
+  // K block -> stage st: thread tid's load i fills row i * KR + tid / KROW, granule tid % KROW, with granule
+  // (tid % KROW) ^ (row & 7) of the block (the swizzle does not depend on i)
   constexpr int KR = NT / KROW;
-  static_assert(KR % 8 == 0, "the swizzle of a granule must not depend on the load");
+  static_assert(KR % 8 == 0 && 8 % (64 / KROW) == 0, "the swizzle of a granule must not depend on the load, nor its pad on the lane");
   const int k_row0 = tid / KROW;
   const uint32_t k_off = k_row0 * (D * 2) + (((tid % KROW) ^ (k_row0 & 7)) * 16);
   // LDS address of the wave's 1 KB slice of load 0 in stage 0
   const uint32_t k_lds = __builtin_amdgcn_readfirstlane(
-      static_cast<uint32_t>(reinterpret_cast<uintptr_t>(smem)) + wave * 1024);
+      static_cast<uint32_t>(reinterpret_cast<uintptr_t>(smem)) + wave * 1024 + wave * (64 / KROW) / 8 * K_PAD);
   auto k_dma = [&](int64_t off, int bytes, int st, int i) {  // the block's bytes from load i's first row on
     constexpr int kLoad = KR * D * 2;
     lds_dma16(buf_words(kc_head + off + i * kLoad, max(bytes - i * kLoad, 0)), k_off,
-              k_lds + st * KSTAGE + i * (NT * 16));
+              k_lds + st * KSTAGE + i * (NT * 16 + KR / 8 * K_PAD));
   };
   // V block -> registers: pair i is key quad tid % 16 (4 rows) x d octet i * NT / 16 + tid / 16
   const int v_kq = tid % (KB / 4), v_dq = tid / (KB / 4);
@@ -755,11 +760,12 @@ __device__ __forceinline__ void attn_tile(const P& p, unsigned char* smem, int b
 #pragma unroll
     for (int j = 0; j < NJ; ++j) o[rt][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-  // K fragment (tile kt, k-step s) of lane (r, q): row 16 kt + r, granule (4s + q) ^ (r & 7)
+  // K fragment (tile kt, k-step s) of lane (r, q): row 16 kt + r (16 rows and two pads a tile), granule (4s + q) ^ (r & 7)
   // = 8 (s >> 1) + 4 ((s & 1) ^ x2) + (q ^ x01) with x = r & 7: one base for even s, one for odd,
   // each plus 64 (s & ~1) bytes
   const int x2 = (lr >> 2) & 1, y01 = lq ^ (lr & 3);
-  const int kf0 = 16 * KTW * kh * (D * 2) + lr * (D * 2);
+  constexpr int KTILE = 16 * D * 2 + 2 * K_PAD;
+  const int kf0 = KTW * kh * KTILE + lr * (D * 2) + (lr >> 3) * K_PAD;
   const int kfe = kf0 + (4 * x2 + y01) * 16, kfo = kf0 + (4 * (x2 ^ 1) + y01) * 16;
   // V^T fragment (j, ks) of lane (r, q): d row 16 j + r, positions 32 ks + 8q .., granule (4 ks + q) ^ (r & 7)
   const int vfo0 = lr * (VTP * 2) + (4 * (x2 ^ (KG == 2 ? kh : 0)) + y01) * 16;
@@ -820,7 +826,7 @@ __device__ __forceinline__ void attn_tile(const P& p, unsigned char* smem, int b
     // S^T = K Q^T: lane (r, q) holds keys 16 kt + 4q + i of row r, for both row tiles
     const unsigned char* Ks = smem + st * KSTAGE;
     auto k_frag = [&](int s, int kt) {
-      return *reinterpret_cast<const bf16x8*>(Ks + ((s & 1) ? kfo : kfe) + kt * 16 * (D * 2) + (s & ~1) * 64);
+      return *reinterpret_cast<const bf16x8*>(Ks + ((s & 1) ? kfo : kfe) + kt * KTILE + (s & ~1) * 64);
     };
     f32x4 sc[2][KTW];
 #pragma unroll

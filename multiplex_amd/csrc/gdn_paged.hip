@@ -416,8 +416,8 @@ struct StepParams : PagedParams {
 // keeps a softmax state of its own; nothing in the loop waits for another wave.
 // K and V go to the wave's own 16 KB of LDS by direct loads of whole rows (K as
 // fragments from memory, 64 bytes of a row at a time, took 1.6 times as long from
-// a warm cache), their 16-byte granules swizzled on the way: K's by (key & 7), so
-// that 16-byte fragment reads of 8 keys hit distinct banks, V's by 2 (key & 7), so
+// a warm cache), their 16-byte granules swizzled on the way: K's by (key & 15), so
+// that 16-byte fragment reads of 16 keys hit distinct banks, V's by 2 (key & 7), so
 // that its transposed reads of 4 x 4 keys do.  K of the next step is asked for as
 // soon as this one's scores are formed, V as soon as its products are: a CU has up
 // to 128 KB in flight.  Bound by memory: a full cache of 64 rows of 4096 keys at 4
@@ -473,7 +473,7 @@ __device__ __forceinline__ void attn_rows(const PagedParams& p, unsigned char* s
 #pragma unroll
     for (int c = 0; c < LD; ++c) {
       const int row = c * RL + row0;
-      const uint32_t off = row * (D * 2) + (gran ^ (twist * (row & 7))) * 16;
+      const uint32_t off = row * (D * 2) + (gran ^ (twist == 1 ? row & 15 : 2 * (row & 7))) * 16;
       if (once) lds_dma16_once(rsrc, off, lds + c * 1024);
       else lds_dma16(rsrc, off, lds + c * 1024);
     }
@@ -514,7 +514,7 @@ __device__ __forceinline__ void attn_rows(const PagedParams& p, unsigned char* s
       f32x4 a = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int s = 0; s < NS; ++s)
-        a = mfma16(*reinterpret_cast<const bf16x8*>(ks + (16 * kt + lr) * (D * 2) + ((4 * s + lq) ^ (lr & 7)) * 16), qf[s], a);
+        a = mfma16(*reinterpret_cast<const bf16x8*>(ks + (16 * kt + lr) * (D * 2) + ((4 * s + lq) ^ lr) * 16), qf[s], a);
       sc[kt] = a;
     }
     asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");  // K is read
