@@ -140,8 +140,9 @@ def _ranges(cus: int, B: int, T: int, Hq: int, Hkv: int, D: int, prefix: int, ow
     to merge; ranges make workgroups enough, each at a price.  So the choice is
     the least of the times that :data:`_US` gives.  (Decode of 64 rows of 16
     heads of 256 behind 8192 keys and up to 512 of their own, us: without a pass
-    of the prefix 110, with it in 4 / 16 / 32 ranges 67 / 37.5 / 51; 4 rows behind
-    2048: 15.3, in 12 ranges 13.8.)
+    of the prefix 113, with it in 4 / 8 / 12 / 16 / 32 ranges 64 / 42 / 35.5 / 37 /
+    47.5; 4 rows behind 2048: in 1 / 4 / 8 ranges of all keys 27 / 15 / 13.2, the
+    prefix apart in 8 / 12 14.2 / 13.6.)
     """
     rows = T * (Hq // Hkv)
     few, few_step, many, many_step, merge, merge_mb, full = _US[D > 128]
