@@ -326,7 +326,8 @@ class PagedKVCache:
     launch, nothing read back) and returns their slots; :meth:`advance` and
     :meth:`trim` move the lengths, and blocks that a rollback left unused go
     back to the pool at the next :meth:`reserve`.  The host keeps the lengths
-    and the number of free blocks, so a full pool raises before any launch.
+    and the number of free blocks, so a full pool raises before any launch, and
+    a step of the cache cannot be captured into a graph (its calls can).
 
     :meth:`fork` starts a batch on a prompt: the rows' tables list the prompt's
     full blocks in common (``shared`` of them, read once for the batch by
@@ -378,9 +379,15 @@ class PagedKVCache:
             raise ValueError(f"n_new must hold {self.batch} counts (got {counts})")
         return counts
 
+    def _not_captured(self) -> None:
+        if self.pool.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("the host keeps a paged cache's lengths and block counts, which a graph's replays would "
+                               "not move: capture paged_tables, attn_rope and paged_attn over tensors of their own")
+
     def _tables(self, lengths: torch.Tensor, host: Sequence[int], T: int, n_new: Optional[torch.Tensor],
                 new: Sequence[int]) -> torch.Tensor:
         """One ``gdn_paged_tables`` in place, with the host's counts kept in step."""
+        self._not_captured()
         need = [max(self._blocks(n + m), self.shared) for n, m in zip(host, new)]
         free = self.pool.free_blocks + sum(self._held) - sum(need)
         if free < 0:
@@ -422,6 +429,7 @@ class PagedKVCache:
 
     def advance(self, T: int, n_new: Optional[Sequence[int]] = None, counts: Optional[torch.Tensor] = None) -> None:
         T = int(T)
+        self._not_captured()
         if n_new is None:
             self.lengths = [n + T for n in self.lengths]
             _pos_add(self.pos0, T, -2**31)
@@ -433,6 +441,7 @@ class PagedKVCache:
     def trim(self, n: int) -> int:
         """Drops the last ``n`` positions of every row (the drafter's rollback),
         at most down to the shared ones; returns how many the longest row lost."""
+        self._not_captured()
         floor = self.floor
         n = max(0, min(int(n), self.offset - floor))
         # rows shorter than the floor (none of a fork's) keep what they hold

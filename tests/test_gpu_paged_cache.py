@@ -234,6 +234,21 @@ def test_counts_are_not_captured():
             cache.reserve(2, [1, 2])
 
 
+@pytest.mark.parametrize("verb", ["reserve", "advance", "trim"])
+def test_a_caches_steps_are_not_captured(verb):
+    """The host's lengths and counts would not move with the replays."""
+    c = mx.PagedKVCache(mx.BlockPool(8, 1, 128, 64, DEV), 2)
+    c.reserve(70)
+    c.advance(70)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="capture"):
+            getattr(c, verb)(3)
+    assert c.lengths == [70, 70] and c._held == [2, 2] and c.pool.free_blocks == 4
+    assert c.reserve(1).tolist() and c.held.tolist() == [2, 2] and c.pool.n_free.tolist() == [4]
+
+
 def test_rows_past_the_batch_are_left_alone():
     """Buffers longer than the batch (views of a serving loop's largest): what lies behind stays."""
     i32 = dict(dtype=torch.int32, device=DEV)
