@@ -98,12 +98,15 @@ class Rotary(torch.nn.Module):
 def _tokens(t: torch.Tensor, B: int, T: int, width: int, what: str) -> int:
     """Elements from one token to the next of a ``[B, T, width]`` view whose
     rows are contiguous (a column slice of a fused GEMM output)."""
-    if tuple(t.shape) != (B, T, width) or (width > 1 and t.stride(2) != 1):
+    if t.shape != (B, T, width):
         raise ValueError(f"{what} must be a [{B}, {T}, {width}] view with contiguous rows (got {tuple(t.shape)})")
-    ld = t.stride(1) if T > 1 else (t.stride(0) if B > 1 else width)
-    if ld < width or (B > 1 and T > 1 and t.stride(0) != T * ld):
+    row, token, dim = t.stride()
+    if dim != 1 and width > 1:
+        raise ValueError(f"{what} must be a [{B}, {T}, {width}] view with contiguous rows")
+    ld = token if T > 1 else (row if B > 1 else width)
+    if ld < width or (B > 1 and T > 1 and row != T * ld):
         raise ValueError(f"{what}: tokens must be one stride apart")
-    return int(ld)
+    return ld
 
 
 def attn_rope(qg: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, q_norm_w: Optional[torch.Tensor],
@@ -125,7 +128,7 @@ def attn_rope(qg: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, q_norm
     rounds there, as the reference does).
     """
     dev = qg.device
-    index, turns = qg.get_device(), rotary.turns
+    index, turns = qg.get_device(), rotary._buffers["turns"]  # (a module's attribute is looked up three times as long)
     if index < 0 or qg.dim() != 3 or keys.dim() != 4:
         _refuse(qg, k_new, v_new, q_norm_w, k_norm_w, pos0, keys, values, turns, slots, gated, q_out)
     B, T, width = qg.shape
@@ -160,7 +163,7 @@ def attn_rope(qg: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, q_norm
             q_norm_w, k_norm_w = q_norm_w.contiguous(), k_norm_w.contiguous()
         qn, kn, wdt = q_norm_w.data_ptr(), k_norm_w.data_ptr(), _dtype_code(q_norm_w, "q_norm_w")
     if q_out is None:
-        q_out = torch.empty((B, T, Hq, D), dtype=bf16, device=dev)
+        q_out = qg.new_empty((B, T, Hq, D))
     _lib.call(dev, "gdn_attn_rope", qg.data_ptr(), qg_ld, q_head, k_new.data_ptr(), v_new.data_ptr(), kv_ld, qn, kn,
               wdt, float(eps), pos0.data_ptr(), None if slots is None else slots.data_ptr(), turns.data_ptr(),
               rotary.factor, int(rotary.interleaved), q_out.data_ptr(), keys.data_ptr(), values.data_ptr(), B, T, Hq,
