@@ -564,9 +564,22 @@ constexpr int K_PAD = 128;
 template <int D>
 constexpr int k_stage() { return KB * D * 2 + KB / 8 * K_PAD; }
 
-// k-steps of q kept in LDS: as many as leave the loop without a spill
+// k-steps of q kept in LDS: as many as leave the loop without a spill.  They are spread over the 8 steps, so that one
+// pair of registers takes each in while the products of the steps between are formed (as the last steps of all, waited
+// for, 4 x 512 tokens behind 4096 keys took 131 us, not 129.6).
 template <int KG, class P>
 constexpr int q_lds_steps() { return KG == 2 ? (P::kPaged ? 3 : 2) : 0; }
+// QL of 8 steps: 1, 4, 7 or 2, 6.  The slot of step s in LDS (-1: it is in registers), and the steps before s that
+// are in registers.
+constexpr int q_slot(int ql, int s) {
+  const int step = ql == 3 ? 3 : 4, first = ql == 3 ? 1 : 2;
+  return ql > 0 && s % step == first ? s / step : -1;
+}
+constexpr int q_reg(int ql, int s) {
+  int n = 0;
+  for (int i = 0; i < s; ++i) n += q_slot(ql, i) < 0;
+  return n;
+}
 template <int D, int KG, class P>
 constexpr int tile_lds() {
   return 2 * (k_stage<D>() + D * VTP * 2) + (KG == 2 ? 8 * 128 * 4 : 0) + 4 * 2 * q_lds_steps<KG, P>() * 1024 +
@@ -611,11 +624,11 @@ __device__ __forceinline__ void attn_tile(const P& p, unsigned char* smem, int b
   const int k_free = prefix_of(p) ? k_hi : min(p0 + row0 / g + 1, k_hi);  // keys below this are visible to every row
   const int nblk = k_hi > k_lo ? (k_hi - k_lo + KB - 1) / KB : 0;
 
-  // the wave's two 16-row tiles; rows past the end compute on q = 0 and are not stored.  The last QL
-  // k-steps of q are kept in LDS (both waves of a row group read one copy)
-  auto q_lds = [&](int rt, int s) {
-    return reinterpret_cast<bf16x8*>(smem + 2 * (KSTAGE + VSTAGE) + kMl) +
-           ((rg * 2 + rt) * QL + s - (NS - QL)) * 64 + lane;
+  // the wave's two 16-row tiles; rows past the end compute on q = 0 and are not stored.  QL k-steps of q are
+  // kept in LDS (both waves of a row group read one copy)
+  static_assert(QL == 0 || (NS == 8 && q_reg(QL, NS) == NS - QL), "steps of q in LDS");
+  auto q_lds = [&](int rt, int slot) {
+    return reinterpret_cast<bf16x8*>(smem + 2 * (KSTAGE + VSTAGE) + kMl) + ((rg * 2 + rt) * QL + slot) * 64 + lane;
   };
   int kmax[2];
   bf16x8 qf[2][NS - QL];
@@ -660,8 +673,8 @@ __device__ __forceinline__ void attn_tile(const P& p, unsigned char* smem, int b
         for (int s = 0; s < NS; ++s) {
           const u32x4 x = *reinterpret_cast<const u32x4*>(smem + 2 * KSTAGE + r * (D * 2) + ((4 * s + lq) ^ lr) * 16);
           const bf16x8 f = __builtin_bit_cast(bf16x8, ok ? x : u32x4{0u, 0u, 0u, 0u});
-          if (s < NS - QL) qf[rt][s] = f;
-          else if (kh == 0) *q_lds(rt, s) = f;
+          if (q_slot(QL, s) < 0) qf[rt][q_reg(QL, s)] = f;
+          else if (kh == 0) *q_lds(rt, q_slot(QL, s)) = f;
         }
       }
       asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory");  // the stages are free
@@ -685,8 +698,8 @@ __device__ __forceinline__ void attn_tile(const P& p, unsigned char* smem, int b
 #pragma unroll
       for (int s = 0; s < NS; ++s) {
         const bf16x8 f = __builtin_bit_cast(bf16x8, ok[rt] ? v[rt][s] : u32x4{0u, 0u, 0u, 0u});
-        if (s < NS - QL) qf[rt][s] = f;
-        else if (kh == 0) *q_lds(rt, s) = f;
+        if (q_slot(QL, s) < 0) qf[rt][q_reg(QL, s)] = f;
+        else if (kh == 0) *q_lds(rt, q_slot(QL, s)) = f;
       }
   };
   if constexpr (!P::kPaged) load_q();
@@ -833,26 +846,35 @@ __device__ __forceinline__ void attn_tile(const P& p, unsigned char* smem, int b
     for (int kt = 0; kt < KTW; ++kt) sc[0][kt] = sc[1][kt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     // fragments f = (k-step f / KTW, tile f % KTW), KPF of them in flight
     constexpr int KPF = KG == 2 ? 3 : 4;
-    bf16x8 kf[KPF];
+    bf16x8 kf[KPF], ql[2];
 #pragma unroll
     for (int f = 0; f < KPF; ++f) kf[f] = k_frag(f / KTW, f % KTW);
+    if constexpr (QL > 0) {
+      ql[0] = *q_lds(0, 0);
+      ql[1] = *q_lds(1, 0);
+    }
 #pragma unroll
     for (int f = 0; f < NS * KTW; ++f) {
       const int s = f / KTW, kt = f % KTW;
       const bf16x8 a = kf[f % KPF];
       if (f + KPF < NS * KTW) kf[f % KPF] = k_frag((f + KPF) / KTW, (f + KPF) % KTW);
       if (kt == 0 && s < KDMA) k_dma(off1, nb1, st ^ 1, s);
-      const bool in_regs = s < NS - QL;
-      sc[0][kt] = mfma16(a, in_regs ? qf[0][in_regs ? s : 0] : *q_lds(0, s), sc[0][kt]);
-      sc[1][kt] = mfma16(a, in_regs ? qf[1][in_regs ? s : 0] : *q_lds(1, s), sc[1][kt]);
+      const int slot = q_slot(QL, s), reg = slot < 0 ? q_reg(QL, s) : 0;
+      sc[0][kt] = mfma16(a, slot < 0 ? qf[0][reg] : ql[0], sc[0][kt]);
+      sc[1][kt] = mfma16(a, slot < 0 ? qf[1][reg] : ql[1], sc[1][kt]);
+      if (slot >= 0 && slot + 1 < QL && kt == KTW - 1) {  // the next of them
+        ql[0] = *q_lds(0, slot + 1);
+        ql[1] = *q_lds(1, slot + 1);
+      }
     }
     // issue order: fragment f + KPF read ahead of fragment f's two products
-    __builtin_amdgcn_sched_group_barrier(0x100, KPF, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, KPF + (QL > 0 ? 2 : 0), 0);
 #pragma unroll
     for (int f = 0; f < NS * KTW; ++f) {
       if (f + KPF < NS * KTW) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-      if (f % KTW == 0 && f / KTW >= NS - QL) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);  // q
       __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+      const int slot = q_slot(QL, f / KTW);
+      if (slot >= 0 && slot + 1 < QL && f % KTW == KTW - 1) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);  // q
     }
 
     if (kb + KB > k_free) {
