@@ -468,6 +468,8 @@ size_t gdn_paged_attn_workspace_bytes(int64_t B, int64_t T, int64_t Hq, int64_t 
  *   n_prefix > 0: the shared keys are read once for all rows of the batch, in
  *            n_prefix ranges, apart from each row's own; 0: with the row's own
  *   n_own    key ranges of a row's own keys
+ *   prefix_rows, own_rows  query rows (token times head of a group) of a workgroup, 16
+ *            or 128, over the shared and the own keys
  *   kv_len_max  host bound of pos0[b] + n_new[b], in [shared * block + T (0 where
  *            n_new is given), table_ld * block]
  * block: a power of two from 64 on; table_ld * block <= 2^30; B <= 65535.  v of a
@@ -479,8 +481,8 @@ int gdn_paged_attn(const void* q, const void* qg, int64_t qg_ld, const void* key
                    const int32_t* table, int64_t table_ld, const int32_t* pos0, const int32_t* n_new,
                    void* out, float scale, int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
                    int64_t n_blocks, int64_t block, int64_t kv_len_max, int64_t shared,
-                   int64_t n_prefix, int64_t n_own, void* workspace, size_t workspace_bytes,
-                   void* stream);
+                   int64_t n_prefix, int64_t n_own, int64_t prefix_rows, int64_t own_rows,
+                   void* workspace, size_t workspace_bytes, void* stream);
 
 /* RMSNorm of bf16 rows (mlx nn.RMSNorm): y = h / sqrt(mean(h^2) + eps) * w
  * with h = x, or h = bf16(x + res) when res is not NULL (a residual add

@@ -209,7 +209,7 @@ _SIGNATURES = {
     "gdn_paged_attn": (
         c_int,
         [_P, _P, _I64, _P, _P, _P, _I64, _P, _P, _P, c_float, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
-         _I64, _I64, _P, c_size_t, _P],
+         _I64, _I64, _I64, _I64, _P, c_size_t, _P],
     ),
     "gdn_rms_norm": (c_int, [_P, _P, _P, _P, c_int, _P, _I64, _I64, _I64, c_float, _P]),
     "gdn_pos_add": (c_int, [_P, _I64, c_int32, c_int32, _P]),

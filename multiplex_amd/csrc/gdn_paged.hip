@@ -408,10 +408,11 @@ int lg2(int64_t x) {  // of a power of two, else -1
 struct StepParams : PagedParams {
   int n_prefix, n_own;        // key ranges
   int len_prefix, len_own;    // keys of a range
-  int prefix_tiles, own_tiles;  // row tiles; 0: the rows fit the 16 of attn_rows
+  int prefix_tiles, own_tiles;  // row tiles
+  int prefix_few, own_few;      // of the 16 rows of attn_rows, not the PR of attn_tile
 };
 
-// Up to 16 rows of kv-head hkv (of batch entry b, or of the whole batch) over key
+// Rows 16 rb .. of kv-head hkv (of batch entry b, or of the whole batch) over key
 // range `split`, by W waves.  Every wave takes 16 KT keys of a step of 16 KT W and
 // keeps a softmax state of its own; nothing in the loop waits for another wave.
 // K and V go to the wave's own 16 KB of LDS by direct loads of whole rows (K as
@@ -431,7 +432,7 @@ constexpr int rows_lds() {
   return kv > merge ? kv : merge;
 }
 template <int D, int W>
-__device__ __forceinline__ void attn_rows(const PagedParams& p, unsigned char* smem, int b, int hkv, int split) {
+__device__ __forceinline__ void attn_rows(const PagedParams& p, unsigned char* smem, int b, int hkv, int rb, int split) {
   constexpr int KT = 256 / D;         // 16-key tiles per wave and step
   constexpr int KW = 16 * KT;         // keys per wave and step
   constexpr int KS = KW * W;          // keys per step
@@ -440,15 +441,15 @@ __device__ __forceinline__ void attn_rows(const PagedParams& p, unsigned char* s
   constexpr int LD = KW * KROW / 64;  // direct loads of 1 KB per wave, step and operand
   constexpr int STAGE = KW * D * 2;   // bytes
   const int g = p.Hq / p.Hkv;
-  const int n_rows = tile_rows(p, g);
+  const int row0 = 16 * rb, n_rows = min(tile_rows(p, g) - row0, 16);  // this workgroup's
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lr = lane & 15, lq = lane >> 4;
   const int tokens = row_tokens(p, b);
   const int p0 = row_start(p, b, tokens);
-  const KeyRange range = key_range(p, split, p0, tokens - 1, tokens > 0);
+  const KeyRange range = key_range(p, split, p0, min((row0 + 15) / g, tokens - 1), row0 / g < tokens);
   const int k_lo = range.lo + KW * wave, k_hi = range.hi;  // this wave's keys: KW from k_lo, k_lo + KS, ..
-  const int k_free = prefix_of(p) ? k_hi : min(p0 + 1, k_hi);  // keys below this are visible to every row
+  const int k_free = prefix_of(p) ? k_hi : min(p0 + row0 / g + 1, k_hi);  // keys below this are visible to every row
   const int n_step = k_hi > k_lo ? (k_hi - k_lo + KS - 1) / KS : 0;
 
   // lane l holds the block of the wave's step page0 + l
@@ -461,18 +462,18 @@ __device__ __forceinline__ void attn_rows(const PagedParams& p, unsigned char* s
   unsigned char* ks = smem + wave * (2 * STAGE);
   const unsigned char* vs = ks + STAGE;
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(ks)));
-  const int row0 = lane / KROW, gran = lane % KROW;
+  const int key0 = lane / KROW, gran = lane % KROW;
   static_assert(64 % KROW == 0, "whole rows per load");
   constexpr int RL = 64 / KROW;  // rows per load
-  // a row's own keys are read by one workgroup, where none of them are shared
-  const bool once = !prefix_of(p) && p.pos_min == p.key0;
+  // one row tile's own keys are read by one workgroup, where none of them are shared
+  const bool once = !prefix_of(p) && p.pos_min == p.key0 && tile_rows(p, g) <= 16;
   auto load = [&](const uint16_t* pool, int i, uint32_t lds, int twist) {
     const int kb = k_lo + KS * i;
     const int64_t off = key_off<D>(p, b, hkv, kb, __builtin_amdgcn_readlane(pages, i - page0)) * 2;
     const u32x4 rsrc = buf_words(reinterpret_cast<const unsigned char*>(pool) + off, min(k_hi - kb, KW) * (D * 2));
 #pragma unroll
     for (int c = 0; c < LD; ++c) {
-      const int row = c * RL + row0;
+      const int row = c * RL + key0;
       const uint32_t off = row * (D * 2) + (gran ^ (twist == 1 ? row & 15 : 2 * (row & 7))) * 16;
       if (once) lds_dma16_once(rsrc, off, lds + c * 1024);
       else lds_dma16(rsrc, off, lds + c * 1024);
@@ -484,7 +485,7 @@ __device__ __forceinline__ void attn_rows(const PagedParams& p, unsigned char* s
     load(p.kc, 0, lds0, 1);
   }
   // lane lr's row: Q as the B operand of S^T = K Q^T
-  const RowAt at = row_at(p, b, hkv, g, lr < n_rows ? lr : 0);
+  const RowAt at = row_at(p, b, hkv, g, row0 + (lr < n_rows ? lr : 0));
   const bool row_ok = lr < n_rows && (prefix_of(p) || at.t < tokens);
   const int kmax = prefix_of(p) ? INT_MAX : p0 + at.t;  // last key the row may see
   u32x4 qr[NS];
@@ -596,7 +597,7 @@ __device__ __forceinline__ void attn_rows(const PagedParams& p, unsigned char* s
   static_assert(CW % 4 == 0, "whole pieces");
   const int mr = threadIdx.x / (4 * W), c0 = (threadIdx.x % (4 * W)) * 4;
   if (mr >= n_rows) return;
-  const RowAt mat = row_at(p, b, hkv, g, mr);
+  const RowAt mat = row_at(p, b, hkv, g, row0 + mr);
   if (!prefix_of(p) && mat.t >= tokens) {  // a padded token
     if (p.n_split == 1) {
 #pragma unroll
@@ -646,7 +647,7 @@ __global__ __launch_bounds__(step_threads<D>()) void attn_step_kernel(const Step
   // the pairs are a multiple of the eight, and its L2 reads them once
   PagedParams r = p;
   int i = blockIdx.x;
-  const int n_prefix = p.Hkv * p.n_prefix * max(p.prefix_tiles, 1);
+  const int n_prefix = p.Hkv * p.n_prefix * p.prefix_tiles;
   r.prefix = i < n_prefix;
   if (!r.prefix) i -= n_prefix;
   r.split0 = r.prefix ? 0 : p.n_prefix;
@@ -657,7 +658,7 @@ __global__ __launch_bounds__(step_threads<D>()) void attn_step_kernel(const Step
   const int split = hs / p.Hkv, hkv = hs - split * p.Hkv;
   const int batch = r.prefix ? 1 : p.B;
   const int tile = tb / batch, b = tb - tile * batch;
-  if (tiles == 0) attn_rows<D, W>(r, smem, b, hkv, split);
+  if (r.prefix ? p.prefix_few : p.own_few) attn_rows<D, W>(r, smem, b, hkv, tiles - 1 - tile, split);
   else attn_tile<D, KG>(r, smem, b, hkv, tiles - 1 - tile, split);  // longest key ranges first
 }
 
@@ -846,7 +847,8 @@ extern "C" int gdn_paged_attn(const void* q, const void* qg, int64_t qg_ld, cons
                               const int32_t* table, int64_t table_ld, const int32_t* pos0, const int32_t* n_new,
                               void* out, float scale, int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
                               int64_t n_blocks, int64_t block, int64_t kv_len_max, int64_t shared, int64_t n_prefix,
-                              int64_t n_own, void* workspace, size_t workspace_bytes, void* stream) {
+                              int64_t n_own, int64_t prefix_rows, int64_t own_rows, void* workspace,
+                              size_t workspace_bytes, void* stream) {
   using gdn_host::fail;
   if (D != 128 && D != 256) return fail(GDN_ERR_UNSUPPORTED, "gdn_paged_attn: head dim must be 128 or 256 (got %lld)", (long long)D);
   const int lg = lg2(block);
@@ -856,7 +858,8 @@ extern "C" int gdn_paged_attn(const void* q, const void* qg, int64_t qg_ld, cons
       table_ld <= 0 || table_ld > INT32_MAX || table_ld * block > INT32_MAX || T > table_ld * block ||
       kv_len_max > table_ld * block || shared < 0 || shared > table_ld ||
       kv_len_max < shared * block + (n_new ? 0 : T) || n_prefix < 0 || n_prefix > 65535 || n_own < 1 ||
-      n_own > 65535 || (n_prefix > 0 && shared == 0))
+      n_own > 65535 || (n_prefix > 0 && shared == 0) || (prefix_rows != 16 && prefix_rows != PR) ||
+      (own_rows != 16 && own_rows != PR))
     return fail(GDN_ERR_INVALID,
                 "gdn_paged_attn: bad sizes (kv_len_max must lie in [shared * block + T, table width * block])");
   if (!(scale > 0.0f)) return fail(GDN_ERR_INVALID, "gdn_paged_attn: scale must be positive");
@@ -906,11 +909,12 @@ extern "C" int gdn_paged_attn(const void* q, const void* qg, int64_t qg_ld, cons
   p.n_own = static_cast<int>(n_own);
   p.len_prefix = n_prefix > 0 ? range_len(p.key0, n_prefix) : 0;
   p.len_own = range_len(kv_len_max - p.key0, n_own);
-  auto tiles_of = [](int64_t n) { return static_cast<int>(n <= 16 ? 0 : (n + PR - 1) / PR); };
-  p.prefix_tiles = n_prefix > 0 ? tiles_of(B * rows) : 0;
-  p.own_tiles = tiles_of(rows);
-  const int64_t groups = Hkv * (n_prefix * (p.prefix_tiles > 1 ? p.prefix_tiles : 1) +
-                                B * n_own * (p.own_tiles > 1 ? p.own_tiles : 1));
+  auto tiles_of = [](int64_t n, int64_t tile) { return static_cast<int>((n + tile - 1) / tile); };
+  p.prefix_few = prefix_rows == 16;
+  p.own_few = own_rows == 16;
+  p.prefix_tiles = n_prefix > 0 ? tiles_of(B * rows, prefix_rows) : 0;
+  p.own_tiles = tiles_of(rows, own_rows);
+  const int64_t groups = Hkv * (n_prefix * p.prefix_tiles + B * n_own * p.own_tiles);
   if (groups > INT32_MAX) return fail(GDN_ERR_UNSUPPORTED, "gdn_paged_attn: problem too large");
   if (D == 256) hipLaunchKernelGGL(attn_step_kernel<256>, dim3(static_cast<unsigned>(groups)), dim3(512), 0, st, p);
   else hipLaunchKernelGGL(attn_step_kernel<128>, dim3(static_cast<unsigned>(groups)), dim3(256), 0, st, p);

@@ -123,18 +123,19 @@ def _cu_count(dev: torch.device) -> int:
 # 128 and 256 (two workgroups a CU, and one).  Fitted to graph-replayed times of
 # 7000 sizes (four head layouts of 3 to 8 query heads a group, 1 to 128 rows, 1 to
 # 512 tokens, prefixes to 16384 and rows' own keys to 32768), 16 choices each; at
-# 19000 its choice is 3% slower than the best of them on average, 9 to 10% at one
-# in ten.
+# 26000 its choice is 2.5 to 3.5% slower than the best of them on average, 8 to 11%
+# at one in ten.
 _US = ((5.2, 1.01, 7.2, 1.24, 4.1, 0.37, 0.25), (6.5, 1.23, 10.5, 1.52, 4.7, 0.28, 0.17))
-_MB_US = 5.5  # MB a us from memory
+_MB_US, _L2_MB_US = 5.5, 25.0  # MB a us from memory, and from the L2s
 _PREFIX_RANGES = (0, 1, 2, 3, 4, 6, 8, 12, 16, 20, 24, 32, 48, 64)
 _OWN_RANGES = (1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128, 256)
 
 
 @functools.lru_cache(maxsize=4096)
-def _ranges(cus: int, B: int, T: int, Hq: int, Hkv: int, D: int, prefix: int, own: int) -> Tuple[int, int]:
-    """``(n_prefix, n_own)``: key ranges of the shared prefix (0: read with each
-    row's own keys) and of a row's own keys; both lengths in steps of 64 keys.
+def _ranges(cus: int, B: int, T: int, Hq: int, Hkv: int, D: int, prefix: int, own: int) -> Tuple[int, int, int, int]:
+    """``(n_prefix, n_own, prefix_rows, own_rows)``: key ranges of the shared prefix
+    (0: read with each row's own keys) and of a row's own keys, and the query rows
+    of a workgroup over each; both lengths in steps of 64 keys.
 
     The prefix read once takes work from every row, but leaves partial results
     to merge; ranges make workgroups enough, each at a price.  So the choice is
@@ -143,32 +144,39 @@ def _ranges(cus: int, B: int, T: int, Hq: int, Hkv: int, D: int, prefix: int, ow
     of the prefix 113, with it in 4 / 8 / 12 / 16 / 32 ranges 64 / 42 / 35.5 / 37 /
     47.5; 4 rows behind 2048: in 1 / 4 / 8 ranges of all keys 27 / 15 / 13.2, the
     prefix apart in 8 / 12 14.2 / 13.6.)
+
+    Workgroups of 16 rows start and end sooner, but the keys are read once for
+    every 16.  Where there are 17 to 512 rows, the better kind takes on average 0.89
+    of the time of 128-row workgroups alone (6 x 4 drafts of 8 heads a group behind
+    5952 keys 26.7 and, in 16s, 21.5 us; a row of 16 tokens over 2000 keys 17.3 and
+    13.9; 32 rows of one token behind 8192 keys 28 and 32).
     """
     rows = T * (Hq // Hkv)
     few, few_step, many, many_step, merge, merge_mb, full = _US[D > 128]
     slots = cus * (1 if D > 128 else 2)
     read = few + 256e-6 * Hkv * D * (prefix + B * own / 2) / _MB_US  # the keys and values, rows half full
 
-    def groups(n_rows, blocks, n):
-        """Workgroups of a kv-head, and us that one takes."""
+    def groups(n_rows, blocks, n, tile):
+        """Workgroups of a kv-head, us that one takes, and MB that they read."""
         of = -(-blocks // n)
-        n = -(-blocks // of)
-        if n_rows <= 16:
-            return n, few + few_step * -(-of // 2)
-        return -(-n_rows // 128) * n, many + many_step * of
+        n = -(-blocks // of) * -(-n_rows // tile)
+        return n, few + few_step * -(-of // 2) if tile == 16 else many + many_step * of, 256e-6 * D * n * of
 
-    best, choice = None, (0, 1)
-    for p in _PREFIX_RANGES:
+    def tiles(n_rows):
+        return (16,) if n_rows <= 16 else (16, 128) if n_rows <= 512 else (128,)
+
+    best, choice = None, (0, 1, 128, 128)
+    for p, tp in [(0, 128)] + [(p, tp) for p in _PREFIX_RANGES[1:] for tp in tiles(B * rows)]:
         if p and (B == 1 or rows >= 256 or p > prefix):
             break
         own_p = max(own if p else own + prefix, 1)
-        n_p, us_p = groups(B * rows, prefix, p) if p else (0, 0.0)
+        n_p, us_p, mb_p = groups(B * rows, prefix, p, tp) if p else (0, 0.0, 0.0)
         whole, rest = divmod(n_p * Hkv, slots)  # the prefix's workgroups go first, in rounds of all slots
         fill = 1.0 - own / (2 * own_p)
-        for o in _OWN_RANGES:
+        for o, to in [(o, to) for o in _OWN_RANGES for to in tiles(rows)]:
             if o > 1 and 2 * o > own_p or p and o > 8:
                 break
-            n_o, us = groups(rows, own_p, o)
+            n_o, us, mb = groups(rows, own_p, o, to)
             n_o *= max(B, 1) * Hkv
             mean = us * (full + (1.0 - full) * fill)
             free = slots - rest  # beside the prefix's last round
@@ -180,18 +188,18 @@ def _ranges(cus: int, B: int, T: int, Hq: int, Hkv: int, D: int, prefix: int, ow
                 t = max(us_p + (left * mean + us - mean if left else 0.0), rounds * mean + us)
             else:
                 t = (-(-n_o // slots) - 1) * mean + us
-            t = max(whole * us_p + t, read)
+            t = max(whole * us_p + t, read, few + Hkv * (mb_p + B * mb * fill) / _L2_MB_US)
             if p + o > 1:
                 t += merge + merge_mb * 4e-6 * B * T * Hq * D * (p + o)
             if best is None or t < best:
-                best, choice = t, (p, o)
+                best, choice = t, (p, o, tp, to)
     return choice
 
 
 def paged_attn(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, table: torch.Tensor, pos0: torch.Tensor,
                kv_len_max: int, *, n_new: Optional[torch.Tensor] = None, shared: int = 0,
                gate: Optional[torch.Tensor] = None, scale: Optional[float] = None,
-               n_split: Optional[Tuple[int, int]] = None, workspace: Optional[torch.Tensor] = None,
+               n_split: Optional[Tuple[int, ...]] = None, workspace: Optional[torch.Tensor] = None,
                out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Causal GQA attention of q ``[B, T, Hq, D]`` over the blocks that ``table``
     ``[B, width]`` lists (``gdn_paged_attn``), times sigmoid of the gate half of
@@ -204,7 +212,9 @@ def paged_attn(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, table:
     it are not read).  The first ``shared`` entries of every row's table have to
     be the same and full (``pos0[b] >= shared * block``): their keys are read
     once for the batch.  ``n_split`` sets the key ranges of the prefix (0: with
-    each row's own keys) and of a row's own keys; by default a rule does.
+    each row's own keys) and of a row's own keys, and, where it has four entries,
+    the query rows of a workgroup over each (16 or 128; otherwise 16 where no more
+    are there); by default a rule does.
     ``workspace``: bytes for the partial results of several ranges (allocated
     when absent or too small); calls that overlap need one each.
 
@@ -241,7 +251,10 @@ def paged_attn(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, table:
     prefix = shared * block
     if n_split is None:
         n_split = _ranges(_cu_count(dev), B, T, Hq, Hkv, D, prefix >> 6, (kv_len_max - prefix + 63) >> 6)
-    n_prefix, n_own = n_split
+    if len(n_split) == 2:
+        rows = T * (Hq // Hkv)
+        n_split = (*n_split, 16 if B * rows <= 16 else 128, 16 if rows <= 16 else 128)
+    n_prefix, n_own, prefix_rows, own_rows = n_split
     ws, ws_bytes = None, 0
     if n_prefix + n_own > 1:
         need = B * T * Hq * (n_prefix + n_own) * (D + 2)  # gdn_paged_attn_workspace_bytes, in floats
@@ -251,7 +264,7 @@ def paged_attn(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, table:
     _lib.call(dev, "gdn_paged_attn", q.data_ptr(), None if gate is None else gate.data_ptr(), qg_ld, keys.data_ptr(),
               values.data_ptr(), table.data_ptr(), width, pos0.data_ptr(), None if n_new is None else n_new.data_ptr(),
               out.data_ptr(), D ** -0.5 if scale is None else float(scale), B, T, Hq, Hkv, D, n_blocks, block,
-              kv_len_max, shared, n_prefix, n_own, ws, ws_bytes, _stream(dev))
+              kv_len_max, shared, n_prefix, n_own, prefix_rows, own_rows, ws, ws_bytes, _stream(dev))
     return out
 
 

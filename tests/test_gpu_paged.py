@@ -258,6 +258,13 @@ CASES = {
     "long_chunk_ranges": (2, 130, (16, 4, 256), 64, 2, [0, 700], [130, 77], (0, 5), True),
     "prefix_200_rows": (50, 1, (16, 4, 256), 64, 9, [b for b in range(50)], None, (4, 1), True),
     "prefix_600_rows_d128": (75, 2, (16, 4, 128), 64, 4, [b for b in range(75)], [b % 3 for b in range(75)], (3, 2), True),
+    "prefix_in_16s": (12, 1, (16, 4, 256), 64, 5, [13 * b for b in range(12)], None, (3, 1, 16, 16), True),
+    "prefix_in_16s_of_3_heads": (9, 3, (12, 4, 128), 64, 7, [30 * b for b in range(9)], [b % 4 for b in range(9)], (4, 2, 16, 16), True),
+    "own_in_16s": (3, 13, (16, 4, 256), 64, 1, [0, 60, 300], None, (0, 1, 128, 16), True),
+    "own_in_16s_ranges": (3, 9, (16, 2, 128), 128, 1, [0, 60, 700], [9, 0, 5], (0, 4, 128, 16), True),
+    "own_in_16s_of_3_heads": (2, 23, (6, 2, 256), 64, 0, [0, 133], [23, 7], (0, 2, 128, 16), False),
+    "both_in_16s": (5, 8, (16, 4, 256), 64, 4, [0, 64, 200, 3, 127], [8, 1, 0, 7, 3], (2, 2, 16, 16), True),
+    "own_in_128s_of_few": (4, 1, (16, 4, 256), 64, 2, [0, 5, 64, 200], None, (2, 1, 128, 128), True),
     "prefix_ends_in_range": (33, 1, (16, 4, 256), 64, 5, [b for b in range(33)], None, (3, 1), True),
 }
 
@@ -353,7 +360,8 @@ def test_attention_of_any_shape(seed):
     q, gate, keys, values, table, pos0 = _attn_case(gen, B, T, heads, block, shared, tails, n_new)
     L = max(p + (T if n_new is None else n) for p, n in zip(pos0, n_new or [T] * B))
     ref = op.attend(_np(q), _np(keys), _np(values), table, pos0, heads[2] ** -0.5, n_new, _np(gate)[..., heads[2]:])
-    for split in (None, (int(rng.integers(0, 4)) if shared else 0, int(rng.integers(1, 5)))):
+    ranges = (int(rng.integers(0, 4)) if shared else 0, int(rng.integers(1, 5)))
+    for split in (None, ranges, (*ranges, 16, 16), (*ranges, 128, 128)):
         out = mx.paged_attn(q.to(DEV), keys.to(DEV), values.to(DEV), _i32(table), _i32(pos0), L, shared=shared,
                             n_new=None if n_new is None else _i32(n_new), gate=gate.flatten(2).to(DEV), n_split=split)
         torch.cuda.synchronize()

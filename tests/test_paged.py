@@ -96,7 +96,7 @@ def test_rope_abi_refusals(lib, kw, status):
 def _attn(lib, **kw):
     a = dict(q=FAKE, qg=FAKE, qg_ld=0, keys=FAKE, values=FAKE, table=FAKE, ld=10, pos0=FAKE, n_new=None, out=FAKE,
              scale=0.1, B=2, T=3, Hq=16, Hkv=4, D=256, n_blocks=5, block=64, L=600, shared=2, n_prefix=1, n_own=2,
-             ws=FAKE, ws_bytes=1 << 40)
+             prefix_rows=16, own_rows=128, ws=FAKE, ws_bytes=1 << 40)
     a.update(kw)
     return lib.gdn_paged_attn(*a.values(), None)
 
@@ -117,6 +117,8 @@ def _attn(lib, **kw):
     (dict(n_own=0), _lib.ERR_INVALID),
     (dict(n_prefix=-1), _lib.ERR_INVALID),
     (dict(n_own=65536), _lib.ERR_INVALID),
+    (dict(prefix_rows=64), _lib.ERR_INVALID),
+    (dict(own_rows=0), _lib.ERR_INVALID),
     (dict(scale=0.0), _lib.ERR_INVALID),
     (dict(q=FAKE + 8), _lib.ERR_INVALID),
     (dict(keys=FAKE + 8), _lib.ERR_INVALID),
@@ -545,8 +547,8 @@ def test_ranges_are_within_the_keys():
                 for heads in ((16, 4, 256), (16, 2, 128), (8, 8, 128)):
                     for prefix in (0, 1, 64):
                         for own in (0, 1, 5, 150):
-                            p, o = paged._ranges(cus, B, T, *heads, prefix, own)
-                            assert o >= 1 and p <= prefix
+                            p, o, *rows = paged._ranges(cus, B, T, *heads, prefix, own)
+                            assert o >= 1 and p <= prefix and set(rows) <= {16, 128}
                             assert o == 1 or 2 * o <= own + (0 if p else prefix)
 
 
