@@ -424,8 +424,10 @@ struct StepParams : PagedParams {
 // to 128 KB in flight.  Bound by memory: a full cache of 64 rows of 4096 keys at 4
 // kv-heads of 256 (1.07 GB) takes 164 us, 6.6 TB/s (without the hint that the keys
 // are read once 186).
-// Tiles of 32 rows in the same way (O and Q in 192 registers) were within 10% of
-// attn_tile either way at 17 to 32 rows and slower beyond.
+// More than 16 rows may take several workgroups, each of which reads the keys: from
+// the L2, as those of one range run on one XCD.  Tiles of 32 rows in the same way
+// (O and Q in 192 registers) were within 10% of attn_tile either way at 17 to 32
+// rows and slower beyond.
 template <int D, int W>
 constexpr int rows_lds() {
   constexpr int kv = W * 2 * 256 * 16 * 2, merge = W * 16 * D * 4 + 2 * W * 16 * 4;
