@@ -154,7 +154,7 @@ def _ranges(cus: int, B: int, T: int, Hq: int, Hkv: int, D: int, prefix: int, ow
     rows = T * (Hq // Hkv)
     few, few_step, many, many_step, merge, merge_mb, full = _US[D > 128]
     slots = cus * (1 if D > 128 else 2)
-    read = few + 256e-6 * Hkv * D * (prefix + B * own / 2) / _MB_US  # the keys and values, rows half full
+    read = 256e-6 * Hkv * D * (prefix + B * own / 2) / _MB_US  # the keys and values, rows half full
 
     def groups(n_rows, blocks, n, tile):
         """Workgroups of a kv-head, us that one takes, and MB that they read."""
@@ -188,7 +188,8 @@ def _ranges(cus: int, B: int, T: int, Hq: int, Hkv: int, D: int, prefix: int, ow
                 t = max(us_p + (left * mean + us - mean if left else 0.0), rounds * mean + us)
             else:
                 t = (-(-n_o // slots) - 1) * mean + us
-            t = max(whole * us_p + t, read, few + Hkv * (mb_p + B * mb * fill) / _L2_MB_US)
+            ends = many if 128 in (to, tp if p else 16) else few  # before the first and after the last keys
+            t = max(whole * us_p + t, ends + read, ends + Hkv * (mb_p + B * mb * fill) / _L2_MB_US)
             if p + o > 1:
                 t += merge + merge_mb * 4e-6 * B * T * Hq * D * (p + o)
             if best is None or t < best:
