@@ -447,6 +447,9 @@ class Attention(torch.nn.Module):
         self.q_norm = RMSNorm(D, args.rms_norm_eps, device)
         self.k_norm = RMSNorm(D, args.rms_norm_eps, device)
         self.scale = D ** -0.5
+        said = (args.rope_scaling or {}).get("partial_rotary_factor")
+        if said is not None and int(D * said) != args.rot:
+            raise ValueError(f"rope scaling says partial_rotary_factor={said}, the layer {args.partial_rotary_factor}")
         self.rotary = Rotary(args.rot, args.rope_theta, interleaved=args.rope_traditional, scaling=args.rope_scaling,
                              device=device)
         self.n_split = n_split

@@ -23,25 +23,51 @@ from .gated_delta import _dtype_code, _require_device, _stream
 __all__ = ["Rotary", "attn_rope"]
 
 
+# what a rope_scaling dict may hold, by its kind; _SAID goes with every kind and changes nothing here (a base other
+# than the layer's is refused; a token of text has one position in all sections of a head)
+_SAID = ("type", "rope_type", "rope_theta", "partial_rotary_factor", "max_position_embeddings",
+         "original_max_position_embeddings", "finetuned", "mrope_section", "mrope_interleaved")
+_READ = {
+    "linear": ("factor",),
+    "yarn": ("factor", "beta_fast", "beta_slow", "attention_factor", "mscale", "mscale_all_dim", "truncate"),
+}
+
+
+def _kind(scaling: Optional[dict]) -> str:
+    return (scaling.get("type") or scaling.get("rope_type") or "default") if scaling else "default"
+
+
+def _number(scaling: dict, key: str, default: Optional[float] = None) -> float:
+    x = scaling.get(key)
+    x = default if x is None else x
+    if x is None or not math.isfinite(x):
+        raise ValueError(f"{_kind(scaling)} scaling needs a finite {key} (got {scaling.get(key)})")
+    return float(x)
+
+
 def _scaled(inv: Sequence[float], rot: int, base: float, scaling: Optional[dict]):
     """``(frequencies, factor)`` of a ``rope_scaling`` dict as model
-    configurations hold it."""
-    if not scaling:
-        return list(inv), 1.0
-    kind = scaling.get("type") or scaling.get("rope_type") or "default"
+    configurations hold it.  A key that would change them and is not read raises."""
+    kind = _kind(scaling)
+    if scaling and scaling.get("rope_theta") is not None and float(scaling["rope_theta"]) != base:
+        raise ValueError(f"rope scaling says rope_theta={scaling['rope_theta']}, the layer base {base}")
     if kind == "default":
         return list(inv), 1.0
-    if kind not in ("linear", "yarn"):
+    if kind not in _READ:
         raise ValueError(f"rope scaling {kind!r} is not one of default, linear, yarn (give inv_freq instead)")
-    s = float(scaling["factor"])
-    if not (math.isfinite(s) and s > 0):
+    unread = sorted(k for k, v in scaling.items() if v is not None and k not in _SAID and k not in _READ[kind])
+    if unread:
+        raise ValueError(f"{kind} scaling does not read {', '.join(unread)} (give inv_freq instead)")
+    s = _number(scaling, "factor")
+    if not s > 0:
         raise ValueError(f"rope scaling factor must be positive (got {s})")
     if kind == "linear":
         return [f / s for f in inv], 1.0
     # pairs that turn more than beta_fast times over the original context keep
     # their frequency, those below beta_slow turns are stretched by s, a ramp
-    # over the pair index in between; the rotated dims grow by 1 + ln(s) / 10
-    context = float(scaling["original_max_position_embeddings"])
+    # over the pair index in between (its ends whole pairs, unless truncate is
+    # false)
+    context = _number(scaling, "original_max_position_embeddings")
     fast, slow = float(scaling.get("beta_fast") or 32.0), float(scaling.get("beta_slow") or 1.0)
     if not (context > 0 and base > 1 and fast > 0 and slow > 0):
         raise ValueError("yarn scaling needs base > 1 and a positive context and betas")
@@ -49,13 +75,31 @@ def _scaled(inv: Sequence[float], rot: int, base: float, scaling: Optional[dict]
     def pair(turns):
         return rot * math.log(context / (turns * 2 * math.pi)) / (2 * math.log(base))
 
-    lo, hi = max(math.floor(pair(fast)), 0), min(math.ceil(pair(slow)), rot - 1)
+    lo, hi = pair(fast), pair(slow)
+    truncate = scaling.get("truncate")
+    if truncate is None or truncate:
+        lo, hi = math.floor(lo), math.ceil(hi)
+    lo, hi = max(lo, 0), min(hi, rot - 1)
     span = hi - lo if hi != lo else 0.001
     ramp = [min(max((i - lo) / span, 0.0), 1.0) for i in range(rot // 2)]
-    factor = scaling.get("attention_factor")
-    if factor is None:
-        factor = 0.1 * math.log(s) + 1.0 if s > 1 else 1.0
-    return [f / s * r + f * (1.0 - r) for f, r in zip(inv, ramp)], float(factor)
+    return [f / s * r + f * (1.0 - r) for f, r in zip(inv, ramp)], _yarn_factor(s, scaling)
+
+
+def _yarn_factor(s: float, scaling: dict) -> float:
+    """What the rotated dims grow by: ``attention_factor``, or 1 + ln(s) / 10, or
+    with both mscales given the ratio of their 1 + mscale ln(s) / 10."""
+    if scaling.get("attention_factor") is not None:
+        return _number(scaling, "attention_factor")
+    m, m_all = _number(scaling, "mscale", 1.0), _number(scaling, "mscale_all_dim", 0.0)
+
+    def grown(m):
+        return 0.1 * m * math.log(s) + 1.0 if s > 1 else 1.0
+
+    if scaling.get("mscale") is not None and m != 0 and m_all != 0:
+        return grown(m) / grown(m_all)
+    if m != 1 or m_all != 0:  # read by some implementations, passed over by others
+        raise ValueError("yarn scaling takes mscale and mscale_all_dim together (or give attention_factor)")
+    return grown(1.0)
 
 
 class Rotary(torch.nn.Module):
@@ -64,8 +108,10 @@ class Rotary(torch.nn.Module):
     ``inv_freq[i] = base ** (-2 i / rot)`` radians per position, scaled by
     ``scaling`` (``{"type": "linear", "factor": s}``, or ``"yarn"`` with
     ``factor``, ``original_max_position_embeddings`` and optionally
-    ``beta_fast``, ``beta_slow`` and ``attention_factor``), or given as
-    ``inv_freq``.  ``interleaved`` pairs neighbouring dims.
+    ``beta_fast``, ``beta_slow``, ``truncate``, and ``attention_factor`` or
+    ``mscale`` with ``mscale_all_dim``; a key that would change them and is not
+    read raises), or given as ``inv_freq``.  ``interleaved`` pairs neighbouring
+    dims.
     """
 
     def __init__(self, rot: int, base: float, *, interleaved: bool = False, scaling: Optional[dict] = None,
@@ -76,9 +122,8 @@ class Rotary(torch.nn.Module):
         if not base > 0:
             raise ValueError(f"base must be positive (got {base})")
         self.rot, self.base, self.interleaved = int(rot), float(base), bool(interleaved)
-        kind = (scaling.get("type") or scaling.get("rope_type") or "default") if scaling else "default"
         # what gdn_attn_qk computes: half pairs of unscaled frequencies
-        self.plain = not interleaved and kind == "default" and inv_freq is None
+        self.plain = not interleaved and _kind(scaling) == "default" and inv_freq is None
         if inv_freq is None:
             inv = [base ** (-2.0 * i / rot) for i in range(rot // 2)]
             self.inv_freq, self.factor = _scaled(inv, rot, float(base), scaling)

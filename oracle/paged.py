@@ -56,10 +56,14 @@ def frequencies(rot, base, scaling=None):
     context = scaling["original_max_position_embeddings"]
     turns = {n: rot * math.log(context / (n * 2 * math.pi)) / (2 * math.log(base))
              for n in (scaling.get("beta_fast", 32.0), scaling.get("beta_slow", 1.0))}
-    lo = max(math.floor(turns[scaling.get("beta_fast", 32.0)]), 0)
-    hi = min(math.ceil(turns[scaling.get("beta_slow", 1.0)]), rot - 1)
+    lo, hi = turns[scaling.get("beta_fast", 32.0)], turns[scaling.get("beta_slow", 1.0)]
+    if scaling.get("truncate", True):
+        lo, hi = math.floor(lo), math.ceil(hi)
+    lo, hi = max(lo, 0), min(hi, rot - 1)
     keep = 1.0 - np.clip((np.arange(rot // 2) - lo) / (hi - lo if hi != lo else 0.001), 0.0, 1.0)
-    factor = scaling.get("attention_factor", 0.1 * math.log(s) + 1.0 if s > 1 else 1.0)
+    log_s = max(math.log(s), 0.0)
+    factor = (1.0 + 0.1 * scaling.get("mscale", 1.0) * log_s) / (1.0 + 0.1 * scaling.get("mscale_all_dim", 0.0) * log_s)
+    factor = scaling.get("attention_factor", factor)
     return inv * keep + inv / s * (1.0 - keep), factor
 
 

@@ -307,6 +307,61 @@ def test_rotary_refusals(kw):
         mx.Rotary(**{**dict(rot=8, base=1e4), **kw})
 
 
+YARN40 = dict(type="yarn", factor=40.0, original_max_position_embeddings=4096)
+
+
+@pytest.mark.parametrize("extra", [
+    dict(mscale=1.0, mscale_all_dim=1.0), dict(mscale=0.707, mscale_all_dim=1.0), dict(mscale=1.0, mscale_all_dim=0.7),
+    dict(mscale=1.0), dict(mscale=1.0, mscale_all_dim=0.0), dict(truncate=False), dict(truncate=True),
+    dict(truncate=False, beta_fast=16.0, beta_slow=2.0, mscale=0.7, mscale_all_dim=0.9),
+    dict(attention_factor=1.25, mscale=0.7, mscale_all_dim=0.9),
+])
+def test_yarn_keys_are_read(extra):
+    """Every key that changes a yarn embedding, against the oracle and against transformers, whose frequencies are
+    float32: 2^-24 per operation, a few of them."""
+    utils = pytest.importorskip("transformers.modeling_rope_utils")
+    from transformers import PretrainedConfig
+
+    scaling, rot, base = {**YARN40, **extra}, 64, 1e4
+    r = mx.Rotary(rot, base, scaling=scaling)
+    inv, factor = op.frequencies(rot, base, scaling)
+    np.testing.assert_allclose(r.inv_freq, inv, rtol=1e-13)
+    assert r.factor == pytest.approx(factor, rel=1e-14)
+    c = PretrainedConfig()
+    c.rope_theta, c.head_dim, c.hidden_size, c.num_attention_heads = base, rot, 4 * rot, 4
+    c.max_position_embeddings = 40 * 4096
+    c.rope_parameters = c.rope_scaling = {**scaling, "rope_type": "yarn", "rope_theta": base}
+    want, mag = utils.ROPE_INIT_FUNCTIONS["yarn"](c, torch.device("cpu"))
+    np.testing.assert_allclose(r.inv_freq, want.double().numpy(), rtol=1e-6)
+    assert r.factor == pytest.approx(mag, rel=1e-12)
+
+
+@pytest.mark.parametrize("scaling", [
+    dict(YARN40, short_factor=[1.0]), dict(YARN40, mscale=0.707), dict(YARN40, mscale_all_dim=1.0),
+    dict(YARN40, mscale=0.0, mscale_all_dim=1.0), dict(YARN40, mscale=0.707, mscale_all_dim=0.0),
+    dict(YARN40, mscale=math.nan, mscale_all_dim=1.0), dict(YARN40, attention_factor=math.inf),
+    dict(YARN40, rope_theta=1e6), dict(type="default", rope_theta=1e6), dict(type="yarn", factor=4.0),
+    dict(type="yarn", original_max_position_embeddings=4096), dict(type="linear"),
+    dict(type="linear", factor=2.0, attention_factor=1.25), dict(type="linear", factor=2.0, high_freq_factor=4.0),
+])
+def test_scaling_keys_that_are_not_read_raise(scaling):
+    with pytest.raises(ValueError):
+        mx.Rotary(64, 1e4, scaling=scaling)
+
+
+def test_scaling_of_a_whole_configuration():
+    """Keys that say what the layer knows, or what text does not use, go with any kind."""
+    said = dict(rope_theta=1e4, partial_rotary_factor=0.25, mrope_section=[11, 11, 10], mrope_interleaved=True,
+                max_position_embeddings=163840, finetuned=True, beta_fast=None)
+    assert mx.Rotary(64, 1e4, scaling={**YARN40, **said}).inv_freq == mx.Rotary(64, 1e4, scaling=YARN40).inv_freq
+    assert mx.Rotary(64, 1e4, scaling={"rope_type": "default", **said}).plain
+    args = dict(hidden_size=256, num_attention_heads=2, num_key_value_heads=1, head_dim=128, intermediate_size=512,
+                rope_theta=1e4)
+    mx.Attention(mx.AttentionArgs(**args, rope_scaling={**YARN40, **said}))
+    with pytest.raises(ValueError, match="partial_rotary_factor"):
+        mx.Attention(mx.AttentionArgs(**args, rope_scaling={**YARN40, "partial_rotary_factor": 1.0}))
+
+
 def test_layers_take_scaled_frequencies():
     args = mx.AttentionArgs(256, 2, 1, 128, 512, rope_scaling={"type": "linear", "factor": 2.0}, rope_traditional=True)
     layer = mx.Attention(args)
