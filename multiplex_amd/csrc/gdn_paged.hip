@@ -220,7 +220,8 @@ struct RopeParams {
 // y = x / sqrt(mean(x^2) + eps) * w, its pairs turned by pos * turns[i] (a turn
 // is 2 pi) and stretched by factor; everything in fp32, rounded once.  With r the
 // norm's factor, each dim is y = r (A x + B x'), x' the other of its pair, A = w
-// cos and B = -+ w' sin: A and B serve every head of a token.
+// cos and B = -+ w' sin: A and B serve every head of a token.  A dim that does not
+// turn takes x' = 0, not B = 0 alone: 0 times an inf or NaN beside it is NaN.
 // A wave takes NU groups of 512 / D heads of one token and one kind (q, k or v),
 // 8 dims a lane, x' by a load of its own (from the L1).  The angles are formed by
 // one lane a dim and handed round in LDS; they are exact at any position: pos *
@@ -262,7 +263,7 @@ __global__ __launch_bounds__(256) void attn_rope_kernel(const RopeParams p) {
   for (int n = 0; n < NU; ++n) {
     const uint16_t* row = src + min(h0 + n * HPU, H - 1) * head_ld;
     raw[n] = *reinterpret_cast<const vec*>(row + d0);
-    other[n] = raw[n];
+    other[n] = vec{};
     if (!IL && turned) {
       if (whole) {
         other[n] = *reinterpret_cast<const vec*>(row + (lower ? d0 + half : d0 - half));
@@ -270,7 +271,8 @@ __global__ __launch_bounds__(256) void attn_rope_kernel(const RopeParams p) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const int d = d0 + e;
-          other[n][e] = row[d < half ? d + half : d < p.rot ? d - half : d];
+          const uint16_t x = row[d < half ? d + half : d < p.rot ? d - half : d];
+          other[n][e] = d < p.rot ? x : 0;
         }
       }
     }
@@ -361,8 +363,9 @@ __global__ __launch_bounds__(256) void attn_rope_kernel(const RopeParams p) {
     const f32x4 s0 = *reinterpret_cast<const f32x4*>(sn + d), s1 = *reinterpret_cast<const f32x4*>(sn + d + 4);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      A[e] *= turned ? (e < 4 ? c0[e & 3] : c1[e & 3]) : 1.0f;
-      B[e] *= turned ? (e < 4 ? s0[e & 3] : s1[e & 3]) : 0.0f;
+      const bool turns = turned && d0 + e < p.rot;
+      A[e] *= turns ? (e < 4 ? c0[e & 3] : c1[e & 3]) : 1.0f;
+      B[e] = turns ? B[e] * (e < 4 ? s0[e & 3] : s1[e & 3]) : 0.0f;
     }
   }
 
@@ -390,7 +393,9 @@ __global__ __launch_bounds__(256) void attn_rope_kernel(const RopeParams p) {
     words out;
 #pragma unroll
     for (int e = 0; e < 8; e += 2) {
-      const float o0 = IL ? x[e + 1] : bf16_to_f32(other[n][e]), o1 = IL ? x[e] : bf16_to_f32(other[n][e + 1]);
+      const bool turns = d0 + e < p.rot;  // (both of a pair, as rot is even)
+      const float o0 = IL ? (turns ? x[e + 1] : 0.0f) : bf16_to_f32(other[n][e]);
+      const float o1 = IL ? (turns ? x[e] : 0.0f) : bf16_to_f32(other[n][e + 1]);
       out[e / 2] = pk_bf16(r * fmaf(A[e], x[e], B[e] * o0), r * fmaf(A[e + 1], x[e + 1], B[e + 1] * o1));
     }
     if (h0 + n * HPU < H) *reinterpret_cast<words*>(dst + (h0 + n * HPU) * dst_ld + d0) = pad ? words{0u, 0u, 0u, 0u} : out;

@@ -174,6 +174,43 @@ def test_rope_matches_oracle(B, T, Hq, Hkv, D, rot, interleaved, scaling, gated,
 
 
 @pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("D,rot,norm", [
+    (256, 64, False), (256, 64, True), (128, 0, False), (256, 6, False), (256, 72, False), (256, 72, True),
+    (128, 128, False), (128, 10, True),
+])
+def test_rope_keeps_infinities_where_they_are(D, rot, norm, interleaved):
+    """inf and NaN in a live token: a dim that does not turn is its own alone (without a norm bit for bit), a pair
+    that turns takes what the definition gives it, and with a norm an inf makes the other dims 0, a NaN all NaN.
+    Finite values to a rounding, 2^-8 of the value; the angle's fp32 (below 1e-6) times |x| |w| < 20 beside it."""
+    gen = torch.Generator().manual_seed(D + rot)
+    B, T, Hq, Hkv = 2, 6, 4, 2
+    q, k = (torch.randn(B, T, H, D, generator=gen).to(torch.bfloat16) for H in (Hq, Hkv))
+    for x in (q, k):
+        for t, (d, v) in enumerate([(D - 3, np.inf), (D - 4, np.nan), (rot, -np.inf), (rot + 1, np.nan), (2, np.inf)]):
+            x[0, t, 0, d % D] = v
+            x[1, t, -1, (d + 1) % D] = v
+    v = torch.randn(B, T, Hkv * D, generator=gen).to(torch.bfloat16)
+    w = torch.randn(D, generator=gen) * 0.2 + 1 if norm else None
+    keys = torch.zeros(1, Hkv, 64, D, dtype=torch.bfloat16, device=DEV)
+    values = torch.zeros_like(keys)
+    rotary = mx.Rotary(rot, 1e4, interleaved=interleaved, device=DEV)
+    dw = None if w is None else w.to(DEV)
+    pos0, slots = [3, 50], np.arange(B * T).reshape(B, T)
+    got = mx.attn_rope(q.view(B, T, -1).to(DEV), k.view(B, T, -1).to(DEV), v.to(DEV), dw, dw, 1e-6, _i32(pos0), keys,
+                       values, rotary, slots=_i32(slots), gated=False)
+    stored = keys[0].transpose(0, 1)[:B * T].reshape(B, T, Hkv, D)
+    inv, factor = op.frequencies(rot, 1e4) if rot else (np.zeros(0), 1.0)
+    for x, y in ((q, got), (k, stored)):
+        for b in range(B):
+            with np.errstate(invalid="ignore"):
+                ref = op.norm_rotate(_np(x[b]), None if w is None else _np(w), 1e-6, pos0[b] + np.arange(T), inv, factor,
+                                     interleaved)
+            np.testing.assert_allclose(_np(y[b]), ref, rtol=2.0**-8, atol=2e-5)
+            if not norm:
+                np.testing.assert_array_equal(_np(y[b])[..., rot:], _np(x[b])[..., rot:])
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
 def test_rope_into_a_dense_cache(interleaved):
     gen = torch.Generator().manual_seed(3)
     B, T, Hq, Hkv, D, rot, cap = 3, 5, 8, 2, 256, 64, 70
