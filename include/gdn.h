@@ -461,7 +461,8 @@ size_t gdn_paged_attn_workspace_bytes(int64_t B, int64_t T, int64_t Hq, int64_t 
 
 /*
  * gdn_attn_fwd over block tables: token t < n_new[b] (all T where n_new is NULL)
- * of row b sees keys 0 .. pos0[b] + t; other tokens' outputs are zeros.
+ * of row b sees keys 0 .. pos0[b] + t; other tokens' outputs are zeros (T is then only
+ * the width that q is padded to, and may exceed what a table lists).
  *   table    [B, table_ld] int32; entries are read as if clamped to the pool
  *   shared   blocks at the start of every row's table that are the same (and
  *            full) in all rows; pos0[b] is read as at least shared * block

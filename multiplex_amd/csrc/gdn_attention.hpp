@@ -76,6 +76,7 @@ struct PagedParams : AttnParams {
   int table_ld, lg, n_blocks, key0, prefix;
   int split0;  // the launch's first key range of the row's n_split
   int pos_min;  // the shared keys, which every row has; above key0, rows read them too as their own
+  int new_max;  // T, or the keys that a table lists behind the shared ones, where they are fewer (n_new is read as no more)
 };
 
 // A value that no kernel of this library's call writes, by a scalar load where
@@ -87,7 +88,7 @@ __device__ __forceinline__ int32_t const_i32(const int32_t* p, int64_t i) {
 // The new tokens of a row.
 template <class P>
 __device__ __forceinline__ int row_tokens(const P& p, int b) {
-  if constexpr (P::kPaged) return p.n_new != nullptr ? min(max(const_i32(p.n_new, b), 0), p.T) : p.T;
+  if constexpr (P::kPaged) return p.n_new != nullptr ? min(max(const_i32(p.n_new, b), 0), p.new_max) : p.T;
   else return p.T;
 }
 

@@ -8,6 +8,8 @@
 //   attention            the kernels of gdn_attention.hpp over the tables: the
 //                        keys that all rows share once for the whole batch, each
 //                        row's own, and the partial results merged.
+#include <algorithm>
+
 #include "gdn_attention.hpp"
 
 namespace {
@@ -862,7 +864,7 @@ extern "C" int gdn_paged_attn(const void* q, const void* qg, int64_t qg_ld, cons
   if (lg < 6 || lg > 20)
     return fail(GDN_ERR_UNSUPPORTED, "gdn_paged_attn: blocks must be powers of two from 64 to 2^20 keys (got %lld)", (long long)block);
   if (B < 0 || T < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || n_blocks <= 0 || n_blocks > INT32_MAX ||
-      table_ld <= 0 || table_ld > INT32_MAX || table_ld * block > INT32_MAX || T > table_ld * block ||
+      table_ld <= 0 || table_ld > INT32_MAX || table_ld * block > INT32_MAX ||
       kv_len_max > table_ld * block || shared < 0 || shared > table_ld ||
       kv_len_max < shared * block + (n_new ? 0 : T) || n_prefix < 0 || n_prefix > 65535 || n_own < 1 ||
       n_own > 65535 || (n_prefix > 0 && shared == 0) || (prefix_rows != 16 && prefix_rows != PR) ||
@@ -911,6 +913,7 @@ extern "C" int gdn_paged_attn(const void* q, const void* qg, int64_t qg_ld, cons
   hipStream_t st = static_cast<hipStream_t>(stream);
   p.key0 = static_cast<int>(n_prefix > 0 ? shared * block : 0);
   p.pos_min = static_cast<int>(shared * block);
+  p.new_max = static_cast<int>(std::min(T, table_ld * block - shared * block));
   auto range_len = [](int64_t keys, int64_t n) { return static_cast<int>(((keys + n - 1) / n + KB - 1) / KB * KB); };
   p.n_prefix = static_cast<int>(n_prefix);
   p.n_own = static_cast<int>(n_own);

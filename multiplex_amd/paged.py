@@ -209,7 +209,7 @@ def paged_attn(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, table:
     keys, values ``[n_blocks, Hkv, block, D]`` bf16 pools, block a power of two
     from 64 on; pos0 ``[B]`` int32: token t of row b sees keys 0 .. pos0[b] + t.
     ``n_new`` ``[B]`` int32: a row's tokens past it are padding, whose outputs are
-    zeros.  ``kv_len_max`` bounds ``pos0[b] + n_new[b]`` (host value; keys beyond
+    zeros; T may then exceed what the tables list.  ``kv_len_max`` bounds ``pos0[b] + n_new[b]`` (host value; keys beyond
     it are not read).  The first ``shared`` entries of every row's table have to
     be the same and full (``pos0[b] >= shared * block``): their keys are read
     once for the batch.  ``n_split`` sets the key ranges of the prefix (0: with

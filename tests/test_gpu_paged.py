@@ -336,6 +336,26 @@ def test_positions_below_the_shared_keys(T, n_split):
     assert _errs(_np(out), ref).max() < ATT_TOL
 
 
+@pytest.mark.parametrize("heads", [(16, 4, 256), (12, 4, 128)])
+@pytest.mark.parametrize("shared,tails,n_new", [(0, [0, 3, 0, 58], [10, 5, 0, 70]), (2, [0, 60, 0, 64], [64, 4, 0, 0])])
+def test_padding_past_the_tables(heads, shared, tails, n_new):
+    """300 tokens a row of which few are real, over tables that list just what those need."""
+    B, T, block = 4, 300, 64
+    q, gate, keys, values, table, pos0 = _attn_case(torch.Generator().manual_seed(31), B, T, heads, block, shared, tails,
+                                                    n_new)
+    L = max(p + n for p, n in zip(pos0, n_new))
+    table = np.ascontiguousarray(table[:, :-(-L // block)])
+    assert T > table.shape[1] * block
+    ref = op.attend(_np(q), _np(keys), _np(values), table, pos0, heads[2] ** -0.5, n_new, _np(gate)[..., heads[2]:])
+    for split in (None, (0, 1), (0, 2, 16, 16), (0, 3, 128, 128), *([(2, 1, 16, 128), (1, 2, 128, 16)] if shared else [])):
+        out = mx.paged_attn(q.to(DEV), keys.to(DEV), values.to(DEV), _i32(table), _i32(pos0), L, shared=shared,
+                            n_new=_i32(n_new), gate=gate.flatten(2).to(DEV), n_split=split)
+        torch.cuda.synchronize()
+        for b, n in enumerate(n_new):
+            assert _errs(_np(out[b, :n]), ref[b, :n]).max(initial=0) < ATT_TOL, (b, split)
+            assert not out[b, n:].any()
+
+
 def test_attention_inf_scores():
     """A row whose every score is -inf is NaN, one with a +inf score too, as the
     softmax of such scores is; their neighbours are untouched."""

@@ -95,6 +95,22 @@ def test_ragged_rows_equal_rows_alone():
         layer(x, mx.KVCache(4, 2, 128, 256, DEV), n_new=[1] * 4)
 
 
+def test_a_step_padded_past_a_fresh_caches_tables():
+    """The tables list what the rows' real tokens need, however wide the call is padded."""
+    torch.manual_seed(11)
+    gen = torch.Generator().manual_seed(11)
+    layer = mx.Attention(mx.AttentionArgs(**ARGS, **ROPE), DEV)
+    pool = mx.BlockPool(20, 2, 128, 64, DEV)
+    cache, alone = mx.PagedKVCache(pool, 2), [mx.PagedKVCache(pool, 1) for _ in range(2)]
+    for T, n_new in ((300, [10, 5]), (512, [1, 0]), (700, [0, 200])):
+        x = _x(gen, 2, T)
+        y = layer(x, cache, n_new=n_new)
+        for b, n in enumerate(n_new):
+            if n:
+                assert _rel(y[b, :n], layer(x[b : b + 1, :n], alone[b])[0]) < LAYER_TOL
+    assert cache.lengths == cache.pos0.tolist() == [11, 205] and cache.capacity == 256
+
+
 @pytest.mark.parametrize("rows", [1, 5, 40])
 def test_forks_equal_whole_rows(rows):
     """A batch on a shared prompt against each row's prompt kept densely, through

@@ -136,6 +136,14 @@ def test_attention_abi_refusals(lib, kw, status):
     assert status == _lib.OK or _lib.last_error()
 
 
+@pytest.mark.parametrize("T", [641, 700, 1 << 20])
+def test_attention_pads_past_the_tables(lib, T):
+    """With n_new, T is the width of the padding and bounds no keys; without, every token is one."""
+    assert _attn(lib, T=T, n_new=FAKE, B=0) == _lib.OK
+    assert _attn(lib, T=T, n_new=FAKE, q=None) == _lib.ERR_INVALID and "null pointer" in _lib.last_error()
+    assert _attn(lib, T=T, B=0) == _lib.ERR_INVALID
+
+
 @pytest.mark.parametrize("B,T,Hq,Hkv,D,n", [(2, 3, 16, 4, 256, 3), (7, 1, 12, 4, 128, 2), (64, 1, 16, 4, 256, 33)])
 def test_attention_workspace_as_the_call_takes_it(lib, calls, monkeypatch, B, T, Hq, Hkv, D, n):
     """The Python call sizes the workspace by itself: exactly the library's."""
