@@ -584,7 +584,8 @@ class PagedKVCache:
     def state(self, kv) -> None:
         """Replaces the contents by ``[keys, values]`` ``[B, Hkv, L, D]``: every row
         then holds L positions of its own and shares none (a prefix-cache
-        restore, as with :class:`KVCache`)."""
+        restore, as with :class:`KVCache`).  Where the pool has room for both, the
+        old rows go last, and a step that fails leaves them."""
         keys, values = kv
         _, Hkv, bs, D = self.pool.keys.shape
         if keys.dim() != 4 or values.shape != keys.shape or (keys.shape[1], keys.shape[3]) != (Hkv, D):
@@ -593,11 +594,23 @@ class PagedKVCache:
         own = sum(h - self.shared for h in self._held)
         if B * self._blocks(L) > self.pool.free_blocks + own:
             raise RuntimeError("block pool exhausted: no room for the state")
-        self.release()
+        if any(c.batch for c in self._forks):
+            raise RuntimeError("rows whose blocks a fork shares cannot be replaced before it")
         fresh = PagedKVCache(self.pool, B, max(L, self.capacity))
-        slots = fresh.reserve(L).long()
-        for pool, x in ((self.pool.keys, keys), (self.pool.values, values)):
-            pool[slots // bs, :, slots % bs] = x.transpose(1, 2).to(pool.dtype)
-        fresh.advance(L)
+        keys, values = keys.to(self.pool.keys), values.to(self.pool.values)
+        beside = B * self._blocks(L) <= self.pool.free_blocks
+        if not beside:
+            self.release()
+        try:
+            slots = fresh.reserve(L).long()
+            for pool, x in ((self.pool.keys, keys), (self.pool.values, values)):
+                pool[slots // bs, :, slots % bs] = x.transpose(1, 2)
+            fresh.advance(L)
+        except BaseException:
+            if any(fresh._held):
+                fresh.release()
+            raise
+        if beside:
+            self.release()
         self.table, self.held, self.pos0 = fresh.table, fresh.held, fresh.pos0
         self.lengths, self._held = fresh.lengths, fresh._held

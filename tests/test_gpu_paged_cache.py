@@ -265,6 +265,20 @@ def test_a_caches_steps_are_not_captured(verb):
     assert c.reserve(1).tolist() and c.held.tolist() == [2, 2] and c.pool.n_free.tolist() == [4]
 
 
+def test_state_from_the_host():
+    """Stored keys and values come back from host memory, as into a dense cache."""
+    gen = torch.Generator().manual_seed(12)
+    k, v = torch.randn(2, 3, 2, 90, 128, generator=gen)
+    cache, dense = mx.PagedKVCache(mx.BlockPool(8, 2, 128, 64, DEV), 2), mx.KVCache(3, 2, 128, 256, DEV)
+    cache.reserve(70)
+    cache.advance(70)
+    for c in (cache, dense):
+        c.state = k, v
+    assert cache.lengths == cache.pos0.tolist() == [90] * 3 and cache.pool.free_blocks == 2
+    for a, b in zip(cache.state, dense.state):
+        assert torch.equal(a, b)
+
+
 def test_rows_past_the_batch_are_left_alone():
     """Buffers longer than the batch (views of a serving loop's largest): what lies behind stays."""
     i32 = dict(dtype=torch.int32, device=DEV)

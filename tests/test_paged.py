@@ -580,6 +580,38 @@ def test_cache_state_is_replaced(on_cpu):
     _check(c, [0] * 3)
 
 
+@pytest.mark.parametrize("rows,device,step", [(4097, "cpu", None), (2, "meta", None), (2, "cpu", "reserve"),
+                                              (2, "cpu", "advance")])
+def test_cache_state_that_cannot_be_replaced_stays(on_cpu, monkeypatch, rows, device, step):
+    """More rows than a cache takes, tensors without values, or a step that fails half way: the contents are what
+    they were (the pool has room for both), and no block is lost."""
+    pool = _pool(5000)
+    c = mx.PagedKVCache(pool, 2)
+    _write(c, 70)
+
+    def fails(*args, **kw):
+        raise MemoryError
+
+    k = torch.zeros(1, 2, 30, 128, dtype=BF, device=device).expand(rows, 2, 30, 128)
+    with monkeypatch.context() as m:
+        if step:
+            m.setattr(mx.PagedKVCache, step, fails)
+        with pytest.raises((ValueError, NotImplementedError, MemoryError)):
+            c.state = k, k
+    assert c.batch == 2 and pool.free_blocks == 5000 - 4
+    _check(c, [0, 0])
+
+
+def test_cache_state_is_replaced_where_only_its_own_blocks_are_left(on_cpu):
+    pool = _pool(5)
+    c = mx.PagedKVCache(pool, 2)
+    _write(c, 100)
+    k = torch.arange(60).to(BF).view(1, 1, 60, 1).expand(4, 2, 60, 128)
+    c.state = k, -k
+    assert c.batch == 4 and pool.free_blocks == 1
+    _check(c, [0] * 4)
+
+
 def test_cache_refusals(on_cpu):
     pool = _pool()
     with pytest.raises(ValueError):
