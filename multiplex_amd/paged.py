@@ -504,17 +504,26 @@ class PagedKVCache:
 
     def _fill(self, n: int, table: torch.Tensor) -> None:
         """Every row's positions from the shared blocks on up to n, copied from the
-        blocks of ``table`` ``[1, width]``."""
-        self.pos0.fill_(n)
-        self.lengths = [n] * self.batch
-        self._tables(self.pos0, self.lengths, 0, None, [0] * self.batch)
-        lo, hi = self.shared, self._blocks(n)
-        if hi > lo:
-            src = table[0, lo:hi].long()
-            for pool in (self.pool.keys, self.pool.values):
-                blocks = pool.index_select(0, src)
-                for b in range(self.batch):
-                    pool.index_copy_(0, self.table[b, lo:hi].long(), blocks)
+        blocks of ``table`` ``[1, width]``.  Where that fails the cache has no rows
+        and holds no blocks."""
+        rows = self.batch
+        try:
+            self.pos0.fill_(n)
+            self.lengths = [n] * rows
+            self._tables(self.pos0, self.lengths, 0, None, [0] * rows)
+            lo, hi = self.shared, self._blocks(n)
+            if hi > lo:
+                src = table[0, lo:hi].long()
+                for pool in (self.pool.keys, self.pool.values):
+                    blocks = pool.index_select(0, src)
+                    for b in range(rows):
+                        pool.index_copy_(0, self.table[b, lo:hi].long(), blocks)
+        except BaseException:
+            if sum(self._held) > self.shared * rows:
+                self._tables(self.counts([0] * rows), [0] * rows, 0, None, [0] * rows)
+            self.table, self.held, self.pos0 = self.table[:0], self.held[:0], self.pos0[:0]
+            self.lengths, self._held, self.shared, self._prefix = [], [], 0, None
+            raise
 
     def fork(self, n: int) -> "PagedKVCache":
         """n rows that continue this one-row cache's prompt, sharing its full blocks."""

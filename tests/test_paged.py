@@ -551,6 +551,32 @@ def test_forks_of_forks(on_cpu):
     assert pool.free_blocks == 40 and sorted(pool.free.tolist()) == list(range(40))
 
 
+@pytest.mark.parametrize("step", ["index_copy_", "index_select", "fill_"])
+@pytest.mark.parametrize("make", ["fork", "extract"])
+def test_a_copy_that_fails_keeps_no_blocks(on_cpu, monkeypatch, make, step):
+    """A fork or an extracted row that cannot be filled (out of memory, say): its blocks are free again, and the
+    prompt is nobody's prefix."""
+    pool = _pool()
+    prompt = mx.PagedKVCache(pool, 1)
+    _write(prompt, 150)
+    rows = prompt.fork(2)
+    _write(rows, 50)
+    free = pool.free_blocks
+
+    def fails(*args, **kw):
+        raise MemoryError
+
+    with monkeypatch.context() as m:
+        m.setattr(torch.Tensor, step, fails)
+        with pytest.raises(MemoryError) as kept:  # noqa: F841 (the failed cache lives on in its traceback)
+            prompt.fork(3) if make == "fork" else rows.extract(1)
+    assert pool.free_blocks == free == int(pool.n_free)
+    _check(rows, [0, 0])
+    rows.release()
+    prompt.release()
+    assert pool.free_blocks == 40 and sorted(pool.free.tolist()) == list(range(40))
+
+
 def test_fork_of_a_short_prompt_shares_nothing(on_cpu):
     pool = _pool(3)
     prompt = mx.PagedKVCache(pool, 1)
