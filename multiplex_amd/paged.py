@@ -553,17 +553,18 @@ class PagedKVCache:
     @classmethod
     def merge(cls, caches: Sequence["PagedKVCache"]) -> "PagedKVCache":
         """Rows of several caches of one pool as one batch (a batch join).  The
-        rows move: the caches given have none afterwards."""
-        first = caches[0]
+        rows move: the caches given have none afterwards.  One without rows joins
+        any others of its pool."""
+        first = next((c for c in caches if c.batch), caches[0])
         if len({id(c) for c in caches}) != len(caches):
             raise ValueError("a cache cannot be merged with itself")
-        if any(c.pool is not first.pool or c.shared != first.shared or c._prefix is not first._prefix
+        if any(c.pool is not first.pool or c.batch and (c.shared != first.shared or c._prefix is not first._prefix)
                for c in caches):
             raise ValueError("caches of different pools or prefixes cannot be merged")
         if any(f.batch for c in caches for f in c._forks):
             raise RuntimeError("rows whose blocks a fork shares cannot move")
         out = cls(first.pool, sum(c.batch for c in caches), max(c.capacity for c in caches))
-        if first.shared:
+        if first.batch and first.shared:
             out._share(first._prefix, first.table[:1], first.shared)
         r = 0
         for c in caches:

@@ -498,6 +498,30 @@ def test_cache_filter_extract_merge(on_cpu):
     assert pool.free_blocks == 40 and sorted(pool.free.tolist()) == list(range(40))
 
 
+@pytest.mark.parametrize("at", [0, 1])
+@pytest.mark.parametrize("empty", ["left", "fork", "new"])
+def test_rows_join_an_empty_batch(on_cpu, empty, at):
+    """A batch whose rows have all left (or that never had any) takes rows of any prefix."""
+    pool = _pool()
+    prompt = mx.PagedKVCache(pool, 1)
+    _write(prompt, 150)
+    batch = mx.PagedKVCache(pool, 0) if empty == "new" else prompt.fork(2 if empty == "left" else 0)
+    if empty == "left":
+        batch.filter([])
+    joins = prompt.fork(3)
+    m = mx.PagedKVCache.merge([batch, joins] if at == 0 else [joins, batch])
+    assert m.batch == 3 and m.shared == 2 and joins.batch == batch.batch == 0
+    _write(m, 9)
+    _check(m, [0] * 3)
+    with pytest.raises(RuntimeError, match="fork"):
+        prompt.release()
+    m.release()
+    empties = mx.PagedKVCache.merge([m, joins])
+    assert empties.batch == empties.shared == 0
+    prompt.release()
+    assert pool.free_blocks == 40 and sorted(pool.free.tolist()) == list(range(40))
+
+
 @pytest.mark.parametrize("keep", [[0, 0], [3], [-1]])
 def test_cache_filter_refusals(on_cpu, keep):
     c = mx.PagedKVCache(_pool(), 3)
