@@ -137,7 +137,16 @@ class Rotary(torch.nn.Module):
         for f in self.inv_freq:
             u = round(math.fmod(f / (2 * math.pi), 1.0) * 2.0**64) % 2**64
             fixed.append(u - 2**64 if u >= 2**63 else u)  # the same 64 bits as a signed number
+        self._fixed = fixed
         self.register_buffer("turns", torch.tensor(fixed, dtype=torch.int64, device=device), persistent=False)
+
+    def _apply(self, fn, recurse=True):
+        """Moves the module; the frequencies are formed anew where they arrive, as
+        a checkpoint for a layer made without memory does not hold them."""
+        super()._apply(fn, recurse)
+        dev = self.turns.device
+        self.turns = torch.tensor(self._fixed, dtype=torch.int64, device=dev)
+        return self
 
 
 def _tokens(t: torch.Tensor, B: int, T: int, width: int, what: str) -> int:

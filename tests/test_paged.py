@@ -303,6 +303,16 @@ def test_frequencies_given():
     assert not r.plain and r.factor == 1.0 and not list(r.state_dict())
 
 
+@pytest.mark.parametrize("made,move", [("meta", lambda m: m.to_empty(device="cpu")), ("cpu", lambda m: m.to(torch.bfloat16)),
+                                       ("cpu", lambda m: m.to("meta").to_empty(device="cpu"))])
+def test_frequencies_survive_a_move(made, move):
+    """A layer made without memory and filled from a checkpoint has its frequencies, which no checkpoint holds."""
+    args = mx.AttentionArgs(256, 2, 1, 128, 512, rope_scaling={"type": "linear", "factor": 2.0})
+    want = mx.Attention(args).rotary.turns
+    got = move(mx.Attention(args, made)).rotary.turns
+    assert got.dtype is torch.int64 and got.device.type == "cpu" and torch.equal(got, want)
+
+
 @pytest.mark.parametrize("kw", [
     dict(rot=7), dict(rot=-2), dict(base=0.0), dict(scaling={"type": "other", "factor": 2.0}),
     dict(scaling={"type": "linear", "factor": 0.0}), dict(scaling={"type": "linear", "factor": math.inf}),
