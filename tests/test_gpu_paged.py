@@ -101,6 +101,30 @@ def test_tables_match_oracle(B, T, block, shared, longest, ragged, spare, in_pla
         assert h is d["held"] and f is d["n_free"]
 
 
+@pytest.mark.parametrize("B,T,block,shared,longest,ragged,spare", [
+    (1024, 2, 64, 1, 700, True, 900),    # the last batch of one row a thread
+    (1025, 3, 64, 2, 900, True, 2000),   # four rows a thread, the last thread's mostly past the batch
+    (1027, 100, 64, 0, 300, False, 40),  # ... the list runs out, several workgroups
+    (3001, 130, 128, 1, 500, True, 60),  # ... many workgroups, the list all but empty
+    (4095, 5, 64, 3, 200, True, 4000),
+    (4096, 1, 256, 2, 2000, True, 700),
+])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_tables_of_many_ragged_rows(B, T, block, shared, longest, ragged, spare, in_place):
+    """Over 1024 rows a thread of tables_kernel takes four: batches that end inside a thread's, ragged and shared."""
+    rng = np.random.default_rng(B * 1000 + T)
+    lengths, n_new, table, held, free, n_free = _tables_case(rng, B, T, block, shared, longest, ragged, spare)
+    ref = op.tables(lengths, T, table, held, free, n_free, block, n_new, shared)
+    d = dict(lengths=_i32(lengths), table=_i32(table), held=_i32(held), free=_i32(free), n_free=_i32([n_free]))
+    out = dict(held_out=d["held"], n_free_out=d["n_free"]) if in_place else {}
+    for _ in range(1 if in_place else 2):
+        slots, h, f = mx.paged_tables(d["lengths"], T, d["table"], d["held"], d["free"], d["n_free"], block,
+                                      n_new=None if n_new is None else _i32(n_new), shared=shared, **out)
+        torch.cuda.synchronize()
+        for got, want in zip((slots, h, f[0], d["table"], d["free"]), ref):
+            np.testing.assert_array_equal(got.cpu().numpy(), want)
+
+
 def test_tables_row_too_long_for_its_table():
     """A row that needs more blocks than its table is wide keeps what it holds
     and gets no slots; the others go on."""
