@@ -123,8 +123,8 @@ def _cu_count(dev: torch.device) -> int:
 # 128 and 256 (two workgroups a CU, and one).  Fitted to graph-replayed times of
 # 7000 sizes (four head layouts of 3 to 8 query heads a group, 1 to 128 rows, 1 to
 # 512 tokens, prefixes to 16384 and rows' own keys to 32768), 16 choices each; at
-# 26000 its choice is 2.5 to 3.5% slower than the best of them on average, 8 to 11%
-# at one in ten.
+# 11500, with up to 40 choices measured, the rule's is 2.5 to 3.9% slower than the
+# best of them on average, 8 to 11% at one in ten.
 _US = ((5.2, 1.01, 7.2, 1.24, 4.1, 0.37, 0.25), (6.5, 1.23, 10.5, 1.52, 4.7, 0.28, 0.17))
 _MB_US, _L2_MB_US = 5.5, 25.0  # MB a us from memory, and from the L2s
 _PREFIX_RANGES = (0, 1, 2, 3, 4, 6, 8, 12, 16, 20, 24, 32, 48, 64)
@@ -139,7 +139,8 @@ def _ranges(cus: int, B: int, T: int, Hq: int, Hkv: int, D: int, prefix: int, ow
 
     The prefix read once takes work from every row, but leaves partial results
     to merge; ranges make workgroups enough, each at a price.  So the choice is
-    the least of the times that :data:`_US` gives.  (Decode of 64 rows of 16
+    the least of the times that :data:`_US` gives, searched for once for a step's
+    sizes: 15 to 550 us of the host's time, then 0.1.  (Decode of 64 rows of 16
     heads of 256 behind 8192 keys and up to 512 of their own, us: without a pass
     of the prefix 113, with it in 4 / 8 / 12 / 16 / 32 ranges 64 / 42 / 35.5 / 37 /
     47.5; 4 rows behind 2048: in 1 / 4 / 8 ranges of all keys 27 / 15 / 13.2, the
@@ -346,8 +347,9 @@ class PagedKVCache:
     :meth:`fork` starts a batch on a prompt: the rows' tables list the prompt's
     full blocks in common (``shared`` of them, read once for the batch by
     :func:`paged_attn`), the rest of it is copied.  The prompt's cache keeps its
-    blocks while such a batch lives.  :meth:`release` gives a batch's blocks back.
-    All caches of one pool are used on one stream.
+    blocks while such a batch lives.  :meth:`release` gives a batch's blocks back
+    (a cache that is dropped without it keeps them).  All caches of one pool are
+    used on one stream.
     """
 
     def __init__(self, pool: BlockPool, batch: int, capacity: int = 256):
