@@ -494,6 +494,70 @@ int gdn_paged_attn(const void* q, const void* qg, int64_t qg_ld, const void* key
 int gdn_rms_norm(const void* x, const void* res, void* h_out, const void* w, int w_dtype, void* y,
                  int64_t y_ld, int64_t rows, int64_t D, float eps, void* stream);
 
+/* ---------------------------------------------------------------------
+ * Sparse MLPs: a router's choice of experts, the experts' products, and dense
+ * products with an epilogue (the shared expert's).  bf16 activations and
+ * weights, fp32 sums.
+ * --------------------------------------------------------------------- */
+
+/*
+ * For each of the B*T tokens, k of E experts and their weights:
+ *   logits  E values a token (dtype), tokens ld elements apart
+ *   s       softmax of the logits, or (sigmoid != 0) 1 / (1 + exp(-logit))
+ *   c       s + bias[e] (NULL: s); the choice goes by c, the weights are s
+ *   groups  equal ranges of experts: only the top_groups with the largest sums
+ *           of their group_best (1 or 2) largest c can be chosen from
+ *   indices [B*T, k]  the experts in the order of falling c, of equals the lowest
+ *           index first; a NaN counts below every number
+ *   weights [B*T, k]  s, divided by their sum (renormalize != 0), times scale;
+ *           0 where all of a token's are
+ *   n_new   [B] (NULL: T): tokens t >= n_new[b] of row b are padding: -1 and 0
+ * Computed in 64 bits.  E up to 1024, k up to 64, groups up to 64.
+ */
+int gdn_route_experts(const void* logits, int dtype, int64_t ld, const float* bias, const int32_t* n_new,
+                      int32_t* indices, float* weights, int64_t B, int64_t T, int64_t E, int64_t k, int sigmoid,
+                      int64_t groups, int64_t top_groups, int64_t group_best, int renormalize, float scale,
+                      void* stream);
+
+/* Workspace bytes of gdn_expert_mlp (0 for sizes it does not take). */
+size_t gdn_expert_mlp_workspace_bytes(int64_t N, int64_t H, int64_t I, int64_t E, int64_t k);
+
+/*
+ * out[t] = base[t] + sum_j weights[t][j] * mlp_e(x[t]) with e = indices[t][j] and
+ * mlp_e(x) = (silu(x G_e^T) * (x U_e^T)) D_e^T:
+ *   x [N, H], base (NULL: 0) and out [N, H]: rows ldx, ldb, ldo elements apart
+ *   gate_up [E, 2I, H] (G_e's rows, then U_e's), down [E, H, I], contiguous
+ *   indices, weights [N, k]; a choice outside [0, E) adds nothing, one that
+ *   stands twice is added twice
+ * silu(..) * .. and an expert's result are rounded to bf16, the sum of the k once.
+ * out may alias base.  Calls that overlap need a workspace each.
+ * H and I multiples of 8, strides too; pointers 16-byte aligned; x spans less
+ * than 2 GiB, an expert's gate_up too.
+ */
+int gdn_expert_mlp(const void* x, int64_t ldx, const void* gate_up, const void* down, const int32_t* indices,
+                   const float* weights, const void* base, int64_t ldb, void* out, int64_t ldo, int64_t N, int64_t H,
+                   int64_t I, int64_t E, int64_t k, void* workspace, size_t workspace_bytes, void* stream);
+
+/* activations of gdn_linear_act */
+#define GDN_ACT_NONE 0
+#define GDN_ACT_RELU 1
+#define GDN_ACT_SILU 2
+#define GDN_ACT_GELU 3      /* x (1 + erf(x / sqrt 2)) / 2 */
+#define GDN_ACT_GELU_TANH 4 /* its tanh form */
+#define GDN_ACT_SWIGLU 5    /* silu(gate) * up */
+
+/*
+ * out[M, N] = act(x[M, K] W^T + bias) * sigmoid(row_gate[m]) + residual[m], rounded once:
+ *   W [N, K] row-major, or [2N, K] for SWIGLU (the gates' rows, then the ups')
+ *   bias (NULL: none)      one value a row of W
+ *   row_gate (NULL: none)  one value a row of x, ldg elements apart
+ *   residual (NULL: none)  bf16 rows ldr elements apart; out may alias it
+ * K and ldx multiples of 8, x and W 16-byte aligned.
+ */
+int gdn_linear_act(const void* x, int64_t ldx, const void* W, const void* bias, int bias_dtype, int act,
+                   const void* row_gate, int row_gate_dtype, int64_t ldg, const void* residual, int64_t ldr, void* out,
+                   int64_t ldo, int64_t M, int64_t N, int64_t K, void* stream);
+
 /* A KV cache's offsets: pos[b] = max(pos[b] + delta, lo) for B rows. */
 int gdn_pos_add(int32_t* pos, int64_t B, int32_t delta, int32_t lo, void* stream);
 

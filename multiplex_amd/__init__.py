@@ -26,7 +26,8 @@ from .cache import ArraysCache, clone_ssm, merge_layer, restore_ssm, restore_ssm
 from .state_pool import PooledBatch, StatePool
 from . import prefix_state
 from .epilogue import gated_rms_norm, prepare_gated_rms_norm
-from .linear import DecodeWorkspace, gated_norm_linear_decode, linear_decode
+from .experts import SparseMLP, expert_mlp, expert_mlp_workspace_bytes, route_experts
+from .linear import DecodeWorkspace, gated_norm_linear_decode, linear_act, linear_decode
 from .mixer import GatedDeltaNet, commit_verified
 from .mixed_step import MixedStep
 from .attention import Attention, AttentionArgs, DecoderLayer, KVCache, MTPHead
@@ -43,6 +44,11 @@ __all__ = [
     "PagedKVCache",
     "paged_attn",
     "paged_tables",
+    "SparseMLP",
+    "expert_mlp",
+    "expert_mlp_workspace_bytes",
+    "linear_act",
+    "route_experts",
     "Rotary",
     "attn_rope",
     "ArraysCache",

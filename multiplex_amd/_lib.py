@@ -58,6 +58,10 @@ EXPORTS = (
     "gdn_paged_attn_workspace_bytes",
     "gdn_paged_attn",
     "gdn_rms_norm",
+    "gdn_route_experts",
+    "gdn_expert_mlp_workspace_bytes",
+    "gdn_expert_mlp",
+    "gdn_linear_act",
     "gdn_pos_add",
     "gdn_silu_mul",
     "gdn_linear_decode_workspace_bytes",
@@ -212,6 +216,19 @@ _SIGNATURES = {
          _I64, _I64, _I64, _I64, _P, c_size_t, _P],
     ),
     "gdn_rms_norm": (c_int, [_P, _P, _P, _P, c_int, _P, _I64, _I64, _I64, c_float, _P]),
+    "gdn_route_experts": (
+        c_int,
+        [_P, c_int, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _I64, c_int, _I64, _I64, _I64, c_int, c_float, _P],
+    ),
+    "gdn_expert_mlp_workspace_bytes": (c_size_t, [_I64, _I64, _I64, _I64, _I64]),
+    "gdn_expert_mlp": (
+        c_int,
+        [_P, _I64, _P, _P, _P, _P, _P, _I64, _P, _I64, _I64, _I64, _I64, _I64, _I64, _P, c_size_t, _P],
+    ),
+    "gdn_linear_act": (
+        c_int,
+        [_P, _I64, _P, _P, c_int, c_int, _P, c_int, _I64, _P, _I64, _P, _I64, _I64, _I64, _I64, _P],
+    ),
     "gdn_pos_add": (c_int, [_P, _I64, c_int32, c_int32, _P]),
     "gdn_silu_mul": (c_int, [_P, _P, _I64, _I64, _P]),
     "gdn_linear_decode_workspace_bytes": (c_size_t, [_I64, _I64, _I64]),

@@ -70,6 +70,16 @@ class AttentionArgs:
     # a long context's scaling and neighbouring pairs (mlx's ``traditional``): see :class:`Rotary`
     rope_scaling: Optional[dict] = None
     rope_traditional: bool = False
+    # a sparse MLP in place of the dense one (:class:`multiplex_amd.SparseMLP`) where num_experts > 0
+    num_experts: int = 0
+    num_experts_per_tok: int = 0
+    moe_intermediate_size: int = 0
+    shared_expert_intermediate_size: int = 0  # 0: no shared expert
+    norm_topk_prob: bool = True
+    scoring_func: str = "softmax"
+    n_group: int = 1
+    topk_group: int = 1
+    routed_scaling_factor: float = 1.0
 
     @property
     def rot(self) -> int:
@@ -572,17 +582,22 @@ class MLP(torch.nn.Module):
 
 
 class DecoderLayer(torch.nn.Module):
-    """mlx-lm ``qwen3_5.DecoderLayer`` at a full-attention index (dense MLP)."""
+    """mlx-lm ``qwen3_5.DecoderLayer`` at a full-attention index, with a dense MLP or,
+    where ``args.num_experts`` > 0, a sparse one."""
 
     def __init__(self, args: AttentionArgs, device=None, dtype=torch.bfloat16):
         super().__init__()
         self.self_attn = Attention(args, device, dtype)
-        self.mlp = MLP(args.hidden_size, args.intermediate_size, device, dtype)
+        self.mlp = (SparseMLP(args, device, dtype) if args.num_experts > 0 else
+                    MLP(args.hidden_size, args.intermediate_size, device, dtype))
         self.input_layernorm = RMSNorm(args.hidden_size, args.rms_norm_eps, device)
         self.post_attention_layernorm = RMSNorm(args.hidden_size, args.rms_norm_eps, device)
 
     def forward(self, x: torch.Tensor, cache: "KVCache | PagedKVCache",
                 n_new: Optional[Sequence[int]] = None) -> torch.Tensor:
+        if isinstance(self.mlp, SparseMLP):  # the last sum is formed in the MLP's own launch
+            h, y, counts = self._attend(x, None, cache, n_new)
+            return self.mlp(y, residual=h, n_new=counts)
         h, m = self.forward_parts(x, None, cache, n_new)
         return h + m
 
@@ -592,13 +607,22 @@ class DecoderLayer(torch.nn.Module):
         sum is its output: the caller adds them inside the next norm
         (``gdn_rms_norm`` with a residual, the same bf16 rounding point), so no
         residual add runs as a launch of its own."""
+        h, y, counts = self._attend(x, residual, cache, n_new)
+        return h, self.mlp(y, n_new=counts) if isinstance(self.mlp, SparseMLP) else self.mlp(y)
+
+    def _attend(self, x, residual, cache, n_new):
+        """The layer up to its MLP: the residual stream, the MLP's input, and (for a
+        sparse MLP) the rows' counts of new tokens on the device."""
+        counts = None
+        if n_new is not None and isinstance(self.mlp, SparseMLP) and hasattr(cache, "counts"):
+            counts = cache.counts(n_new)
         if residual is None:
             xin, y0 = x, self.input_layernorm(x)
         else:
             xin, y0 = self.input_layernorm(x, residual=residual)
         # the residual add in front of the second norm is fused into it
         h, y = self.post_attention_layernorm(xin, residual=self.self_attn(y0, cache, n_new))
-        return h, self.mlp(y)
+        return h, y, counts
 
 
 class MTPHead(torch.nn.Module):
@@ -652,6 +676,8 @@ class MTPHead(torch.nn.Module):
             if c.size() > target:
                 c.trim(c.size() - target)
 
+
+from .experts import SparseMLP  # noqa: E402
 
 # the paged cache builds on this module's
 from .paged import BlockPool, PagedKVCache, paged_attn  # noqa: E402

@@ -24,6 +24,8 @@ SOURCES = [
     "gdn_attention.hip",
     "gdn_paged.hip",
     "gdn_linear.hip",
+    "gdn_route.hip",
+    "gdn_experts.hip",
 ]
 ARCH = "gfx950"
 

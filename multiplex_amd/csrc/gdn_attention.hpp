@@ -507,23 +507,8 @@ __global__ __launch_bounds__(256) void attn_fwd_kernel(const AttnParams p) {
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t buf_rsrc(const void* base, uint32_t bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, static_cast<int>(bytes), 0x00020000);
 }
-// The same descriptor as four words, for inline assembly.
-__device__ __forceinline__ u32x4 buf_words(const void* base, uint32_t bytes) {
-  const uint64_t a = reinterpret_cast<uint64_t>(base);
-  return u32x4{static_cast<uint32_t>(a), static_cast<uint32_t>(a >> 32) & 0xffffu, bytes, 0x00020000u};
-}
 
-// 16 bytes per lane from a buffer (byte offset voff) straight into LDS at lds_base + 16 * lane (rsrc and
-// lds_base wave-uniform).  Issued from inline assembly: the compiler's wait insertion, seeing an LDS DMA in
-// a loop, would otherwise drain every LDS read with lgkmcnt(0).  It increments vmcnt like any load; the
-// caller waits for it (vmcnt(0)) before the barrier that publishes the block.
-__device__ __forceinline__ void lds_dma16(u32x4 rsrc, uint32_t voff, uint32_t lds_base) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
-               :
-               : "v"(voff), "s"(rsrc), "s"(lds_base)
-               : "memory", "m0");
-}
-// The same for bytes that are read once: not kept in the caches.
+// lds_dma16 for bytes that are read once: not kept in the caches.
 __device__ __forceinline__ void lds_dma16_once(u32x4 rsrc, uint32_t voff, uint32_t lds_base) {
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen nt lds"
                :

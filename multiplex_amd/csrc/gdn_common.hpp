@@ -362,6 +362,25 @@ __device__ __forceinline__ float wave_sum(float x) {
   return x;
 }
 
+// ------------------------------------------- loads straight into LDS
+
+// A raw buffer descriptor of `bytes` bytes at `base` (wave-uniform) as four words, for inline assembly: reads past
+// its end return zeros.
+__device__ __forceinline__ u32x4 buf_words(const void* base, uint32_t bytes) {
+  const uint64_t a = reinterpret_cast<uint64_t>(base);
+  return u32x4{static_cast<uint32_t>(a), static_cast<uint32_t>(a >> 32) & 0xffffu, bytes, 0x00020000u};
+}
+
+// 16 bytes per lane from a buffer (byte offset voff) straight into LDS at lds_base + 16 * lane (rsrc and
+// lds_base wave-uniform).  Issued from inline assembly: the compiler's wait insertion, seeing an LDS DMA in
+// a loop, would otherwise drain every LDS read with lgkmcnt(0).  It increments vmcnt like any load; the
+// caller waits for it (vmcnt(0)) before the barrier that publishes the block.
+__device__ __forceinline__ void lds_dma16(u32x4 rsrc, uint32_t voff, uint32_t lds_base) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
+               :
+               : "v"(voff), "s"(rsrc), "s"(lds_base)
+               : "memory", "m0");
+}
 // ------------------------------------------- 8-element row slices
 
 constexpr int CPL = 8;  // channels per lane

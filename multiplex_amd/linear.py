@@ -18,7 +18,8 @@ columns it runs ``gdn_linear_rows16``'s kernel, which leaves the workspace it
 is given alone.
 
 :func:`linear` is the layers' plain projection: a few rows by
-``gdn_linear_rows16``, the library beyond.
+``gdn_linear_rows16``, the library beyond.  :func:`linear_act` is a projection
+with its epilogue (bias, activation, row gate, residual) in the product's launch.
 
 The sliced kernel sums its K slices through a workspace of fp32 partials and one
 ticket per output tile; the tickets must start at zero and every call
@@ -37,7 +38,7 @@ import torch.autograd.forward_ad as forward_ad
 from . import _lib
 from .gated_delta import _dtype_code, _ptr, _require_device, _stream
 
-__all__ = ["linear", "DECODE_MAX_ROWS", "FUSED_NORM_MAX_ROWS", "DecodeWorkspace", "linear_decode",
+__all__ = ["linear", "linear_act", "DECODE_MAX_ROWS", "FUSED_NORM_MAX_ROWS", "DecodeWorkspace", "linear_decode",
            "gated_norm_linear_decode", "linear_decode_workspace_bytes", "decode_shape_ok"]
 
 DECODE_MAX_ROWS = 64
@@ -202,3 +203,130 @@ def gated_norm_linear_decode(y: torch.Tensor, z: torch.Tensor, norm_weight: Opti
             raise ValueError(f"norm_weight must be [{head_dim}]")
         norm_weight = norm_weight.contiguous()
     return _launch(y, z, norm_weight, eps, head_dim, weight, out, workspace)
+
+
+# -------------------------------------------------- products with an epilogue
+
+_ACTS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4, "swiglu": 5}
+
+
+def _even_rows(t: torch.Tensor) -> Optional[int]:
+    """Elements from a row of ``[..., D]`` to the next where the rows are contiguous
+    and evenly spaced (a column slice of a wider buffer), else None."""
+    if t.is_contiguous():
+        return t.shape[-1]
+    D = t.shape[-1]
+    if t.stride(-1) != 1 and D != 1:
+        return None
+    ld, rows = 0, 1
+    for n, step in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+        if n == 1:
+            continue
+        if rows == 1:
+            ld = step
+        elif step != rows * ld:
+            return None
+        rows *= n
+    return (D if rows == 1 else ld) if rows == 1 or ld >= D else None
+
+
+def _forward_only(tensors, names) -> None:
+    """These calls have no backward: a gradient asked for is an error, not lost."""
+    if torch.is_grad_enabled():
+        for t, n in zip(tensors, names):
+            if t is not None and t.requires_grad:
+                raise ValueError(f"{n} requires a gradient, which this call does not form (use torch.no_grad())")
+
+
+def _apart(out: torch.Tensor, others, names) -> None:
+    """``out`` must not overlap what other workgroups still read."""
+    lo, hi = _extent(out)
+    for t, n in zip(others, names):
+        if t is not None and t.numel():
+            a, b = _extent(t)
+            if a < hi and lo < b:
+                raise ValueError(f"out overlaps {n}")
+
+
+def _extent(t: torch.Tensor):
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()) if n > 1)
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _out_rows(out: torch.Tensor, shape, added: Optional[torch.Tensor], reads, names) -> None:
+    """``out`` is of ``shape``, apart from ``reads`` (and of ``added``, which may be
+    the same rows, since each is read by the thread that writes it)."""
+    if out.dtype is not torch.bfloat16 or out.shape != shape or _even_rows(out) is None:
+        raise ValueError(f"out must be bf16 rows of shape {list(shape)}, evenly spaced (got {out.dtype} {list(out.shape)})")
+    _apart(out, reads, names)
+    if added is not None and not (added.data_ptr() == out.data_ptr() and added.stride() == out.stride()):
+        _apart(out, (added,), ("what is added to it",))
+
+
+def linear_act(x: torch.Tensor, weight: torch.Tensor, *, bias: Optional[torch.Tensor] = None,
+               activation: Optional[str] = None, row_gate: Optional[torch.Tensor] = None,
+               residual: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``act(x @ weight.T + bias) * sigmoid(row_gate) + residual`` in one launch
+    (``gdn_linear_act``), rounded once.
+
+    x ``[..., K]`` and weight ``[N, K]`` bf16, K a multiple of 8; ``activation`` is
+    None, "relu", "silu", "gelu" (erf), "gelu_tanh" or "swiglu" (``silu(gate) * up``:
+    weight's and bias's first half are the gate's rows, N is half of theirs).
+    bias ``[rows of weight]``, row_gate ``[...]`` (one logit per row of x, such as
+    a column of another product) in bf16, fp16 or fp32; residual ``[..., N]`` bf16.
+    x and residual may be column slices of wider buffers.  ``out`` may be the
+    residual itself.  There is no backward.
+    """
+    dev = _require_device((x, weight, bias, row_gate, residual, out),
+                          ("x", "weight", "bias", "row_gate", "residual", "out"))
+    if activation not in _ACTS:
+        raise ValueError(f"activation must be one of {[a for a in _ACTS]} (got {activation!r})")
+    if x.dtype is not torch.bfloat16 or weight.dtype is not torch.bfloat16:
+        raise ValueError(f"x and weight must be bfloat16 (got {x.dtype}, {weight.dtype})")
+    if x.dim() < 1 or weight.dim() != 2 or weight.shape[1] != x.shape[-1]:
+        raise ValueError(f"weight must be [N, {x.shape[-1] if x.dim() else 'K'}] (got {list(weight.shape)})")
+    rows, K = weight.shape
+    act = _ACTS[activation]
+    if act == 5 and rows % 2:
+        raise ValueError("swiglu needs the gate's rows and as many of up's")
+    _forward_only((x, weight, bias, row_gate, residual), ("x", "weight", "bias", "row_gate", "residual"))
+    N = rows // 2 if act == 5 else rows
+    lead = x.shape[:-1]
+    shape = (*lead, N)
+    M = lead.numel()
+    if K % 8 or K == 0 or N == 0:
+        raise ValueError(f"K must be a positive multiple of 8 and N positive (got K={K}, N={N})")
+    ldx = _even_rows(x)
+    if ldx is None or ldx % 8 or x.data_ptr() % 16:
+        x, ldx = x.clone(memory_format=torch.contiguous_format), K
+    if not weight.is_contiguous() or weight.data_ptr() % 16:
+        weight = weight.clone(memory_format=torch.contiguous_format)
+    bias_dt = gate_dt = ldg = ldr = 0
+    if bias is not None:
+        if bias.shape != (rows,):
+            raise ValueError(f"bias must be [{rows}] (got {list(bias.shape)})")
+        bias, bias_dt = bias.contiguous(), _dtype_code(bias, "bias")
+    if row_gate is not None:
+        if row_gate.shape != lead:
+            raise ValueError(f"row_gate must be {list(lead)}, one value per row of x (got {list(row_gate.shape)})")
+        gate_dt = _dtype_code(row_gate, "row_gate")
+        ldg = _even_rows(row_gate.unsqueeze(-1))
+        if ldg is None:
+            row_gate, ldg = row_gate.contiguous(), 1
+    if residual is not None:
+        if residual.dtype is not torch.bfloat16 or residual.shape != shape:
+            raise ValueError(f"residual must be bf16 {list(shape)} (got {residual.dtype} {list(residual.shape)})")
+        ldr = _even_rows(residual)
+        if ldr is None:
+            if out is not None:
+                _apart(out, (residual,), ("residual",))
+            residual, ldr = residual.contiguous(), N
+    if out is None:
+        out = torch.empty(shape, dtype=torch.bfloat16, device=dev)
+        ldo = N
+    else:
+        _out_rows(out, shape, residual, (x, weight, bias, row_gate), ("x", "weight", "bias", "row_gate"))
+        ldo = _even_rows(out)
+    _lib.call(dev, "gdn_linear_act", x.data_ptr(), ldx, weight.data_ptr(), _ptr(bias), bias_dt, act, _ptr(row_gate),
+              gate_dt, ldg, _ptr(residual), ldr, out.data_ptr(), ldo, M, N, K, _stream(dev))
+    return out
