@@ -26,6 +26,7 @@ SOURCES = [
     "gdn_linear.hip",
     "gdn_route.hip",
     "gdn_experts.hip",
+    "gdn_linear_act.hip",
 ]
 ARCH = "gfx950"
 

@@ -15,6 +15,7 @@ every token runs.
 
 from __future__ import annotations
 
+import functools
 from typing import Optional, Tuple
 
 import torch
@@ -26,6 +27,7 @@ from .linear import _even_rows, _forward_only, _out_rows, linear_act
 __all__ = ["route_experts", "expert_mlp", "expert_mlp_workspace_bytes", "SparseMLP"]
 
 _SCORING = {"softmax": 0, "sigmoid": 1}
+_FLOATS = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
 
 
 def route_experts(logits: torch.Tensor, k: int, *, scoring: str = "softmax", bias: Optional[torch.Tensor] = None,
@@ -48,6 +50,27 @@ def route_experts(logits: torch.Tensor, k: int, *, scoring: str = "softmax", bia
     with indices -1 and weights 0, which :func:`expert_mlp` passes over.
     Computed in 64 bits, so that scores that differ at all are told apart.
     """
+    # a plain call's checks in a few operations; what is wrong, or laid out otherwise, is looked into below
+    index = logits.get_device()
+    code = _FLOATS.get(logits.dtype)
+    if not (index >= 0 and code is not None and logits.dim() > 1 and k.__class__ is int and k > 0 and scoring in _SCORING
+            and not (torch.is_grad_enabled() and (logits.requires_grad or bias is not None and bias.requires_grad))
+            and logits.is_contiguous() and n_new is None
+            and (bias is None or bias.dtype is torch.float32 and bias.get_device() == index and bias.is_contiguous()
+                 and bias.shape == logits.shape[-1:])):
+        return _route_general(logits, k, scoring, bias, groups, top_groups, group_best, renormalize, scale, n_new)
+    dev, E = logits.device, logits.shape[-1]
+    shape = (*logits.shape[:-1], k)
+    indices = torch.empty(shape, dtype=torch.int32, device=dev)
+    weights = torch.empty(shape, dtype=torch.float32, device=dev)
+    _lib.call(dev, "gdn_route_experts", logits.data_ptr(), code, E, None if bias is None else bias.data_ptr(), None,
+              indices.data_ptr(), weights.data_ptr(), indices.numel() // k, 1, E, k, _SCORING[scoring], int(groups),
+              int(top_groups), int(group_best), 1 if renormalize else 0, float(scale), _stream(dev))
+    return indices, weights
+
+
+def _route_general(logits, k, scoring, bias, groups, top_groups, group_best, renormalize, scale, n_new):
+    """:func:`route_experts` of any layout; raises what is wrong with its arguments."""
     dev = _require_device((logits, bias, n_new), ("logits", "bias", "n_new"))
     if logits.dim() < 1:
         raise ValueError("logits must be [..., E]")
@@ -80,6 +103,7 @@ def route_experts(logits: torch.Tensor, k: int, *, scoring: str = "softmax", bia
     return indices, weights
 
 
+@functools.lru_cache(maxsize=1024)
 def expert_mlp_workspace_bytes(tokens: int, hidden: int, inner: int, experts: int, k: int) -> int:
     """Bytes that :func:`expert_mlp` needs as its workspace."""
     return int(_lib.load().gdn_expert_mlp_workspace_bytes(tokens, hidden, inner, experts, k))
@@ -102,6 +126,39 @@ def expert_mlp(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor, indic
     or too small); calls that overlap need one each.  ``out`` may be the base
     itself.  There is no backward.
     """
+    index, bf16 = x.get_device(), torch.bfloat16
+    E, H, I = down.shape if down.dim() == 3 else (0, 0, 0)
+    lead, k = x.shape[:-1], indices.shape[-1] if indices.dim() else 0
+    # a plain call's checks in a few operations; what is wrong, or laid out otherwise, is looked into below
+    if not (index >= 0 and out is None and x.dtype is bf16 and gate_up.dtype is bf16 and down.dtype is bf16
+            and indices.dtype is torch.int32 and weights.dtype is torch.float32 and gate_up.get_device() == index
+            and down.get_device() == index and indices.get_device() == index and weights.get_device() == index
+            and gate_up.shape == (E, 2 * I, H) and x.dim() > 0 and x.shape[-1] == H and indices.shape[:-1] == lead
+            and weights.shape == indices.shape and x.is_contiguous() and gate_up.is_contiguous()
+            and down.is_contiguous() and indices.is_contiguous() and weights.is_contiguous() and x.data_ptr() % 16 == 0
+            and (base is None or base.dtype is bf16 and base.get_device() == index and base.shape == x.shape
+                 and base.is_contiguous() and base.data_ptr() % 16 == 0)
+            and (workspace is None or workspace.get_device() == index and workspace.is_contiguous())
+            and not (torch.is_grad_enabled() and (x.requires_grad or gate_up.requires_grad or down.requires_grad or
+                                                  weights.requires_grad or base is not None and base.requires_grad))):
+        return _expert_mlp_general(x, gate_up, down, indices, weights, base, out, workspace)
+    dev = x.device
+    return _expert_mlp_call(dev, x, H, gate_up, down, indices, weights, base, H, torch.empty_like(x), H, workspace,
+                            x.numel() // H if H else 0, H, I, E, k)
+
+
+def _expert_mlp_call(dev, x, ldx, gate_up, down, indices, weights, base, ldb, out, ldo, workspace, N, H, I, E, k):
+    need = expert_mlp_workspace_bytes(N, H, I, E, k)
+    if workspace is None or workspace.numel() * workspace.element_size() < need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    _lib.call(dev, "gdn_expert_mlp", x.data_ptr(), ldx, gate_up.data_ptr(), down.data_ptr(), indices.data_ptr(),
+              weights.data_ptr(), None if base is None else base.data_ptr(), ldb, out.data_ptr(), ldo, N, H, I, E, k,
+              workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream(dev))
+    return out
+
+
+def _expert_mlp_general(x, gate_up, down, indices, weights, base, out, workspace):
+    """:func:`expert_mlp` of any layout; raises what is wrong with its arguments."""
     dev = _require_device((x, gate_up, down, indices, weights, base, out, workspace),
                           ("x", "gate_up", "down", "indices", "weights", "base", "out", "workspace"))
     bf16 = torch.bfloat16
@@ -141,15 +198,9 @@ def expert_mlp(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor, indic
         _out_rows(out, x.shape, base, (x, gate_up, down, indices, weights, workspace),
                   ("x", "gate_up", "down", "indices", "weights", "workspace"))
         ldo = _even_rows(out)
-    need = expert_mlp_workspace_bytes(N, H, I, E, k)
     if workspace is not None and not workspace.is_contiguous():
         raise ValueError("workspace must be contiguous")
-    if workspace is None or workspace.numel() * workspace.element_size() < need:
-        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-    _lib.call(dev, "gdn_expert_mlp", x.data_ptr(), ldx, gate_up.data_ptr(), down.data_ptr(), indices.data_ptr(),
-              weights.data_ptr(), _ptr(base), ldb, out.data_ptr(), ldo, N, H, I, E, k, workspace.data_ptr(),
-              workspace.numel() * workspace.element_size(), _stream(dev))
-    return out
+    return _expert_mlp_call(dev, x, ldx, gate_up, down, indices, weights, base, ldb, out, ldo, workspace, N, H, I, E, k)
 
 
 def _weight(*shape, device, dtype) -> torch.nn.Parameter:

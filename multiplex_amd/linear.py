@@ -277,6 +277,30 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, *, bias: Optional[torch.Te
     x and residual may be column slices of wider buffers.  ``out`` may be the
     residual itself.  There is no backward.
     """
+    # a plain call's checks in a few operations; what is wrong, or laid out otherwise, is looked into below
+    index, bf16, act = x.get_device(), torch.bfloat16, _ACTS.get(activation)
+    if (index >= 0 and act is not None and x.dtype is bf16 and weight.dtype is bf16 and weight.dim() == 2 and x.dim() > 0
+            and bias is None and row_gate is None and out is None and weight.get_device() == index
+            and x.is_contiguous() and weight.is_contiguous()
+            and not (torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
+                                                  or residual is not None and residual.requires_grad))):
+        rows, K = weight.shape
+        N = rows // 2 if act == 5 else rows
+        shape, xp, wp = x.shape[:-1] + (N,), x.data_ptr(), weight.data_ptr()
+        if (x.shape[-1] == K and K > 0 and K % 8 == 0 and N > 0 and (act != 5 or rows % 2 == 0) and (xp | wp) % 16 == 0
+                and (residual is None or residual.dtype is bf16 and residual.get_device() == index
+                     and residual.shape == shape and residual.is_contiguous())):
+            dev = x.device
+            out = torch.empty(shape, dtype=bf16, device=dev)
+            _lib.call(dev, "gdn_linear_act", xp, K, wp, None, 0, act, None, 0, 0,
+                      None if residual is None else residual.data_ptr(), N, out.data_ptr(), N, x.numel() // K, N, K,
+                      _stream(dev))
+            return out
+    return _linear_act_general(x, weight, bias, activation, row_gate, residual, out)
+
+
+def _linear_act_general(x, weight, bias, activation, row_gate, residual, out):
+    """:func:`linear_act` of any layout; raises what is wrong with its arguments."""
     dev = _require_device((x, weight, bias, row_gate, residual, out),
                           ("x", "weight", "bias", "row_gate", "residual", "out"))
     if activation not in _ACTS:
