@@ -546,17 +546,22 @@ int gdn_expert_mlp(const void* x, int64_t ldx, const void* gate_up, const void* 
 #define GDN_ACT_GELU_TANH 4 /* its tanh form */
 #define GDN_ACT_SWIGLU 5    /* silu(gate) * up */
 
+/* Workspace bytes of gdn_linear_act (0 for sizes it needs none for). */
+size_t gdn_linear_act_workspace_bytes(int64_t M, int64_t N, int64_t K, int act);
+
 /*
  * out[M, N] = act(x[M, K] W^T + bias) * sigmoid(row_gate[m]) + residual[m], rounded once:
  *   W [N, K] row-major, or [2N, K] for SWIGLU (the gates' rows, then the ups')
  *   bias (NULL: none)      one value a row of W
  *   row_gate (NULL: none)  one value a row of x, ldg elements apart
  *   residual (NULL: none)  bf16 rows ldr elements apart; out may alias it
- * K and ldx multiples of 8, x and W 16-byte aligned.
+ * K and ldx multiples of 8, x and W 16-byte aligned.  A few hundred rows of a
+ * long K are summed in slices of K (in slice order) through the workspace;
+ * calls that overlap need one each.
  */
 int gdn_linear_act(const void* x, int64_t ldx, const void* W, const void* bias, int bias_dtype, int act,
                    const void* row_gate, int row_gate_dtype, int64_t ldg, const void* residual, int64_t ldr, void* out,
-                   int64_t ldo, int64_t M, int64_t N, int64_t K, void* stream);
+                   int64_t ldo, int64_t M, int64_t N, int64_t K, void* workspace, size_t workspace_bytes, void* stream);
 
 /* A KV cache's offsets: pos[b] = max(pos[b] + delta, lo) for B rows. */
 int gdn_pos_add(int32_t* pos, int64_t B, int32_t delta, int32_t lo, void* stream);

@@ -27,7 +27,7 @@ from .state_pool import PooledBatch, StatePool
 from . import prefix_state
 from .epilogue import gated_rms_norm, prepare_gated_rms_norm
 from .experts import SparseMLP, expert_mlp, expert_mlp_workspace_bytes, route_experts
-from .linear import DecodeWorkspace, gated_norm_linear_decode, linear_act, linear_decode
+from .linear import DecodeWorkspace, gated_norm_linear_decode, linear_act, linear_act_workspace_bytes, linear_decode
 from .mixer import GatedDeltaNet, commit_verified
 from .mixed_step import MixedStep
 from .attention import Attention, AttentionArgs, DecoderLayer, KVCache, MTPHead
@@ -48,6 +48,7 @@ __all__ = [
     "expert_mlp",
     "expert_mlp_workspace_bytes",
     "linear_act",
+    "linear_act_workspace_bytes",
     "route_experts",
     "Rotary",
     "attn_rope",

@@ -61,6 +61,7 @@ EXPORTS = (
     "gdn_route_experts",
     "gdn_expert_mlp_workspace_bytes",
     "gdn_expert_mlp",
+    "gdn_linear_act_workspace_bytes",
     "gdn_linear_act",
     "gdn_pos_add",
     "gdn_silu_mul",
@@ -225,9 +226,10 @@ _SIGNATURES = {
         c_int,
         [_P, _I64, _P, _P, _P, _P, _P, _I64, _P, _I64, _I64, _I64, _I64, _I64, _I64, _P, c_size_t, _P],
     ),
+    "gdn_linear_act_workspace_bytes": (c_size_t, [_I64, _I64, _I64, c_int]),
     "gdn_linear_act": (
         c_int,
-        [_P, _I64, _P, _P, c_int, c_int, _P, c_int, _I64, _P, _I64, _P, _I64, _I64, _I64, _I64, _P],
+        [_P, _I64, _P, _P, c_int, c_int, _P, c_int, _I64, _P, _I64, _P, _I64, _I64, _I64, _I64, _P, c_size_t, _P],
     ),
     "gdn_pos_add": (c_int, [_P, _I64, c_int32, c_int32, _P]),
     "gdn_silu_mul": (c_int, [_P, _P, _I64, _I64, _P]),

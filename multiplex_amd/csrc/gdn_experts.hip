@@ -25,7 +25,7 @@ constexpr int kMaxChoices = 64;
 // before counts each chunk's pairs by expert, so that a workgroup knows what lies in front of its own.  Where a pair
 // lies among its expert's goes by the atomics' order, which no result depends on.
 constexpr int kPlanThreads = 1024;
-constexpr int kChunk = 4096;  // pairs
+constexpr int kEach = 2, kChunk = kEach * kPlanThreads;  // pairs of a thread, of a workgroup
 
 struct PlanParams {
   const int* indices;
@@ -37,20 +37,25 @@ struct PlanParams {
   int* to;
 };
 
-__device__ __forceinline__ void count_pairs(const PlanParams& p, int* hist) {
+// The chunk's pairs by expert; each of the thread's pairs' expert (-1: none) and number among its chunk's.
+__device__ __forceinline__ void count_pairs(const PlanParams& p, int* hist, int (&expert)[kEach], int (&number)[kEach]) {
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    const int i = blockIdx.x * kChunk + j * kPlanThreads + threadIdx.x;
+    const int e = i < p.P ? p.indices[i] : -1;
+    expert[j] = e < p.E ? e : -1;
+  }
   for (int e = threadIdx.x; e < p.E; e += kPlanThreads) hist[e] = 0;
   __syncthreads();
-  const int first = blockIdx.x * kChunk, last = min(p.P - first, kChunk) + first;
-  for (int i = first + threadIdx.x; i < last; i += kPlanThreads) {
-    const int e = p.indices[i];
-    if (e >= 0 && e < p.E) atomicAdd(&hist[e], 1);
-  }
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) number[j] = expert[j] >= 0 ? atomicAdd(&hist[expert[j]], 1) : 0;
   __syncthreads();
 }
 
 __global__ __launch_bounds__(kPlanThreads) void plan_count_kernel(const PlanParams p) {
   __shared__ int hist[kMaxExperts];
-  count_pairs(p, hist);
+  int expert[kEach], number[kEach];
+  count_pairs(p, hist, expert, number);
   for (int e = threadIdx.x; e < p.E; e += kPlanThreads) p.counts[blockIdx.x * p.E + e] = hist[e];
 }
 
@@ -77,40 +82,39 @@ __device__ __forceinline__ int block_before(int x, int* waves, int* all) {
 }
 
 __global__ __launch_bounds__(kPlanThreads) void plan_place_kernel(const PlanParams p) {
-  __shared__ int next[kMaxExperts];
+  __shared__ int hist[kMaxExperts];
   __shared__ int waves[kPlanThreads / 64];
   static_assert(kMaxExperts <= kPlanThreads, "a thread an expert");
   const int e = threadIdx.x;
+  int expert[kEach], number[kEach];
+  count_pairs(p, hist, expert, number);
   int mine = 0, total = 0;  // pairs of expert e in the chunks before, and in all
-  if (p.chunks == 1) {
-    count_pairs(p, next);
-    if (e < p.E) total = next[e];
-  } else if (e < p.E) {
-    for (int c = 0; c < p.chunks; ++c) {
+  if (e < p.E) {
+    if (p.chunks == 1) total = hist[e];
+#pragma unroll 8
+    for (int c = 0; c < (p.chunks == 1 ? 0 : p.chunks); ++c) {
       const int n = p.counts[c * p.E + e];
       total += n;
-      if (c < static_cast<int>(blockIdx.x)) mine += n;
+      mine += c < static_cast<int>(blockIdx.x) ? n : 0;
     }
   }
   int all;
   const int first = block_before(total, waves, &all);
   const int tiles = (total + p.rows - 1) / p.rows;
   const int tile0 = block_before(tiles, waves, &all);
-  if (e < p.E) next[e] = first + mine;
+  if (e < p.E) hist[e] = first + mine;
   if (blockIdx.x == 0) {
     for (int i = 0; i < tiles; ++i)
       p.tiles[tile0 + i] = TileOf{e, first + i * p.rows, min(p.rows, total - i * p.rows), 0};
     if (e == 0) p.n_tiles[0] = all;
   }
   __syncthreads();
-  const int begin = blockIdx.x * kChunk, end = min(p.P - begin, kChunk) + begin;
-  for (int i = begin + threadIdx.x; i < end; i += kPlanThreads) {
-    const int x = p.indices[i];
-    if (x >= 0 && x < p.E) {
-      const int at = atomicAdd(&next[x], 1);
-      p.from[at] = i / p.k;
-      p.to[at] = i;
-    }
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    if (expert[j] < 0) continue;
+    const int i = blockIdx.x * kChunk + j * kPlanThreads + threadIdx.x, at = hist[expert[j]] + number[j];
+    p.from[at] = i / p.k;
+    p.to[at] = i;
   }
 }
 
@@ -270,7 +274,7 @@ ExpertLayout expert_layout(int64_t N, int64_t H, int64_t I, int64_t E, int64_t k
 
 bool expert_sizes_ok(int64_t N, int64_t H, int64_t I, int64_t E, int64_t k) {
   return N >= 0 && H > 0 && I > 0 && E > 0 && E <= kMaxExperts && k > 0 && k <= kMaxChoices && H % 8 == 0 &&
-         I % 8 == 0 && H <= INT32_MAX / 4 && I <= INT32_MAX / 4 && N <= INT32_MAX / k;
+         I % 8 == 0 && H <= INT32_MAX / 4 && I <= INT32_MAX / 4 && N <= (INT32_MAX - 2 * kChunk) / k;
 }
 
 }  // namespace

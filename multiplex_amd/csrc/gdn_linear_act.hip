@@ -64,53 +64,109 @@ void launch_few(const ProductParams& p, hipStream_t st) {
 
 namespace {
 
-// The tile of the least modelled time: rounds of tiles over the CUs times a tile's fixed part and its steps' (of 64
-// values of K, shared by WK groups of waves), which grow with the rows it works on, and below all the operands' bytes at
-// the rate the tile reaches.  Fitted to graph-replayed times of 165 sizes (11 products from 512 to 12288 in and 1000 to
-// 24576 weight rows, 5 to 4096 rows), each in all four; the choice is the slower one by 0.5% on average, by 16% at most
-// (5 to 16 rows of 4096 x 24576: 47 us in the second, 41 in the first).  E.g. 128 rows of 4096 x 4096, us:
-// 16.4, 30, 56, 56; 512 of 12288 x 4096: 142, 83, 154, 260; 4096 of 4096 x 24576: 2620, 1285, 700, 619.
+// The sum of the slices' sums and the epilogue, eight columns of a row a thread.  Bound by reading the sums.
+template <bool PAIR>
+__global__ __launch_bounds__(256) void finish_kernel(const ProductParams p) {
+  const int per = (p.N + CPL - 1) / CPL;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, row = i / per;
+  if (row >= p.M) return;
+  const int c = static_cast<int>(i % per) * CPL;
+  float v[CPL] = {}, up[CPL] = {};
+  auto add = [](float (&sum)[CPL], const float* at, bool both) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (h && !both) break;
+      const f32x4 x = *reinterpret_cast<const f32x4*>(at + 4 * h);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum[4 * h + j] += x[j];
+    }
+  };
+  const float* at = p.part + row * p.pitch + c;
+  const bool both = c + 4 < p.N;  // (the pitch's halves hold whole fours)
+  for (int s = 0; s < p.slices; ++s, at += static_cast<int64_t>(p.M) * p.pitch) {
+    add(v, at, both);
+    if (PAIR) add(up, at + p.pitch / 2, both);
+  }
+  finish8<PAIR>(p, v, up, row, c);
+}
+
+// The tile and slices of K of the least modelled time: rounds of tiles over the CUs times a tile's fixed part and its
+// steps' (of 64 values of K, shared by the groups of waves), which grow with the rows it works on, the slices' sums
+// written and read, and below all the operands' bytes at the rate that the tile reaches.  Fitted to graph-replayed times
+// of 165 sizes (11 products from 512 to 12288 in and 1000 to 24576 weight rows, 5 to 4096 rows), each in all four tiles;
+// without slices the choice is the slower one by 0.5% on average, by 16% at most (5 to 16 rows of 4096 x 24576: 47 us in
+// the second, 41 in the first).  E.g. 128 rows of 4096 x 4096, us: 16.4, 30, 56, 56; 512 of 12288 x 4096: 142, 83, 154,
+// 260; 4096 of 4096 x 24576: 2620, 1285, 700, 619.  Slices of K pay where a few tiles have many steps: 512 of 12288 x
+// 4096 in 4 slices 62, 128 of them in 8 41, 1024 of 4096 x 4096 in 2 46 (53 whole).
 struct Tiling {
   int rows, weight_rows, groups, block;  // block: rows that a step's work grows by
   float tile_us, step_us, rows_us;       // a tile's ends, a step, and a step of all rows on top
   float mb_us;                           // MB a us
+  int slices;
 };
 constexpr Tiling kTilings[4] = {
-    {64, 32, 4, 16, 3.7f, 0.0f, 0.63f, 3.5f},
-    {64, 128, 2, 16, 3.9f, 0.40f, 0.31f, 4.2f},
-    {128, 256, 1, 32, 4.0f, 0.40f, 0.40f, 3.1f},
-    {256, 256, 1, 32, 4.0f, 0.36f, 1.02f, 3.2f},
+    {64, 32, 4, 16, 3.7f, 0.0f, 0.63f, 3.5f, 1},
+    {64, 128, 2, 16, 3.9f, 0.40f, 0.31f, 4.2f, 1},
+    {128, 256, 1, 32, 4.0f, 0.40f, 0.40f, 3.1f, 1},
+    {256, 256, 1, 32, 4.0f, 0.36f, 1.02f, 3.2f, 1},
 };
+constexpr float kFinishUs = 4.0f, kPartMbUs = 4.0f;  // the slices' launch, and MB of their sums a us
 
-Tiling tiling(int64_t M, int64_t weight_rows, int64_t K, bool pair) {
-  const Tiling* best = nullptr;
+Tiling tiling(int64_t M, int64_t N, int64_t K, bool pair) {
+  const int64_t weight_rows = pair ? 2 * N : N;
+  const float mb = 2e-6f * (static_cast<float>(M) * K + static_cast<float>(weight_rows) * K + static_cast<float>(M) * N);
+  Tiling best = kTilings[0];
   float least = 0.0f;
+  bool any = false;
   for (const Tiling& t : kTilings) {
-    const int64_t tiles = ((M + t.rows - 1) / t.rows) * ((weight_rows + t.weight_rows - 1) / t.weight_rows);
-    const int64_t whole = (tiles + kCUs - 1) / kCUs;
-    const float rounds = whole > 3 ? static_cast<float>(tiles) / kCUs : static_cast<float>(whole);
-    int64_t rows = t.block;
-    while (rows < t.rows && rows < M) rows *= 2;
-    const float steps = static_cast<float>((K + 64 * t.groups - 1) / (64 * t.groups));
-    const float mb = 2e-6f * (static_cast<float>(M) * K + static_cast<float>(weight_rows) * K +
-                              static_cast<float>(M) * weight_rows / (pair ? 2 : 1));
-    float us = rounds * (t.tile_us + steps * (t.step_us + t.rows_us * static_cast<float>(rows) / t.rows));
-    us = us > mb / t.mb_us ? us : mb / t.mb_us;
-    if (!best || us < least) {
-      best = &t;
+    for (int slices = 1; slices <= 8; slices *= 2) {
+      const int64_t steps = ((K + 64 * t.groups - 1) / (64 * t.groups) + slices - 1) / slices;
+      if (slices > 1 && (t.groups > 1 || steps < 8 || M * weight_rows > (int64_t{1} << 28))) break;
+      const int64_t tiles = ((M + t.rows - 1) / t.rows) * ((weight_rows + t.weight_rows - 1) / t.weight_rows) * slices;
+      const int64_t whole = (tiles + kCUs - 1) / kCUs;
+      const float rounds = whole > 3 ? static_cast<float>(tiles) / kCUs : static_cast<float>(whole);
+      int64_t rows = t.block;
+      while (rows < t.rows && rows < M) rows *= 2;
+      float us = rounds * (t.tile_us + steps * (t.step_us + t.rows_us * static_cast<float>(rows) / t.rows));
+      us = us > mb / t.mb_us ? us : mb / t.mb_us;
+      if (slices > 1) us += kFinishUs + 8e-6f * slices * M * weight_rows / kPartMbUs;
+      if (any && us >= least) continue;
+      any = true;
       least = us;
+      best = t;
+      best.slices = slices;
     }
   }
-  return *best;
+  return best;
+}
+
+constexpr int kFewRows = 4;
+
+int64_t part_pitch(int64_t N, bool pair) { return (N + 3) / 4 * 4 * (pair ? 2 : 1); }
+
+int64_t part_bytes(int64_t M, int64_t N, int64_t K, bool pair) {
+  if (M <= kFewRows) return 0;
+  const Tiling t = tiling(M, N, K, pair);
+  return t.slices > 1 ? 4 * t.slices * M * part_pitch(N, pair) : 0;
+}
+
+template <class S, bool PAIR>
+void launch_slices(const ProductParams& p, int64_t m_tiles, hipStream_t st) {
+  launch_product<S, kPart, false>(p, m_tiles, st);
+  const int64_t threads = static_cast<int64_t>(p.M) * ((p.N + CPL - 1) / CPL);
+  hipLaunchKernelGGL((finish_kernel<PAIR>), dim3(static_cast<unsigned>((threads + 255) / 256)), dim3(256), 0, st, p);
 }
 
 template <bool PAIR>
-void launch_tiles(const ProductParams& p, const Tiling& t, int64_t m_tiles, bool bare, hipStream_t st) {
+void launch_tiles(const ProductParams& p, const Tiling& t, bool bare, hipStream_t st) {
+  const int64_t m_tiles = (p.M + t.rows - 1) / t.rows;
   if (t.rows == 256) {
-    if (bare) launch_product<Large<PAIR>, kBare, false>(p, m_tiles, st);
+    if (t.slices > 1) launch_slices<Large<PAIR>, PAIR>(p, m_tiles, st);
+    else if (bare) launch_product<Large<PAIR>, kBare, false>(p, m_tiles, st);
     else launch_product<Large<PAIR>, kFinish, false>(p, m_tiles, st);
   } else if (t.rows == 128) {
-    if (bare) launch_product<Wide<PAIR>, kBare, false>(p, m_tiles, st);
+    if (t.slices > 1) launch_slices<Wide<PAIR>, PAIR>(p, m_tiles, st);
+    else if (bare) launch_product<Wide<PAIR>, kBare, false>(p, m_tiles, st);
     else launch_product<Wide<PAIR>, kFinish, false>(p, m_tiles, st);
   } else if (t.groups == 2) {
     launch_product<Deep<PAIR>, kFinish, false>(p, m_tiles, st);
@@ -119,17 +175,26 @@ void launch_tiles(const ProductParams& p, const Tiling& t, int64_t m_tiles, bool
   }
 }
 
+bool linear_sizes_ok(int64_t M, int64_t N, int64_t K, int act) {
+  return M >= 0 && N > 0 && K > 0 && K % 8 == 0 && M <= INT32_MAX - 256 && N <= INT32_MAX / 4 && K <= INT32_MAX / 2 &&
+         act >= GDN_ACT_NONE && act <= GDN_ACT_SWIGLU;
+}
+
 }  // namespace
+
+extern "C" size_t gdn_linear_act_workspace_bytes(int64_t M, int64_t N, int64_t K, int act) {
+  return linear_sizes_ok(M, N, K, act) ? static_cast<size_t>(part_bytes(M, N, K, act == GDN_ACT_SWIGLU)) : 0;
+}
 
 extern "C" int gdn_linear_act(const void* x, int64_t ldx, const void* W, const void* bias, int bias_dtype, int act,
                               const void* row_gate, int row_gate_dtype, int64_t ldg, const void* residual, int64_t ldr,
-                              void* out, int64_t ldo, int64_t M, int64_t N, int64_t K, void* stream) {
+                              void* out, int64_t ldo, int64_t M, int64_t N, int64_t K, void* workspace,
+                              size_t workspace_bytes, void* stream) {
   using gdn_host::aligned;
   using gdn_host::fail;
-  if (M < 0 || N <= 0 || K <= 0 || K % 8 || M > INT32_MAX - 256 || N > INT32_MAX / 4)
-    return fail(GDN_ERR_INVALID, "gdn_linear_act: bad sizes M=%lld N=%lld K=%lld (K a multiple of 8)", (long long)M,
-                (long long)N, (long long)K);
-  if (act < GDN_ACT_NONE || act > GDN_ACT_SWIGLU) return fail(GDN_ERR_INVALID, "gdn_linear_act: unknown activation %d", act);
+  if (!linear_sizes_ok(M, N, K, act))
+    return fail(GDN_ERR_INVALID, "gdn_linear_act: bad sizes M=%lld N=%lld K=%lld (K a multiple of 8) or activation %d",
+                (long long)M, (long long)N, (long long)K, act);
   if (M == 0) return GDN_OK;
   if (!x || !W || !out) return fail(GDN_ERR_INVALID, "gdn_linear_act: null pointer");
   if ((bias && !gdn_host::dtype_ok(bias_dtype)) || (row_gate && !gdn_host::dtype_ok(row_gate_dtype)))
@@ -166,15 +231,25 @@ extern "C" int gdn_linear_act(const void* x, int64_t ldx, const void* W, const v
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const bool bare = !bias && !row_gate && !residual && (act == GDN_ACT_NONE || pair);
   // up to four rows: 12288 x 4096 at one 18.3 us (as tiles 25.8), at four 24.4 (27.2); 2048 x 1024 3.8 (4.8), 4.5 (4.8)
-  if (M <= 4) {
+  if (M <= kFewRows) {
     if (pair) launch_few<true>(p, st);
     else launch_few<false>(p, st);
-  } else {
-    const bool bare = !bias && !row_gate && !residual && (act == GDN_ACT_NONE || pair);
-    const Tiling t = tiling(M, pair ? 2 * N : N, K, pair);
-    const int64_t m = (M + t.rows - 1) / t.rows;
-    if (pair) launch_tiles<true>(p, t, m, bare, st);
-    else launch_tiles<false>(p, t, m, bare, st);
+    return gdn_host::check_launch("gdn_linear_act");
   }
+  const Tiling t = tiling(M, N, K, pair);
+  if (t.slices > 1) {
+    const int64_t need = part_bytes(M, N, K, pair), steps = (K + 63) / 64;
+    if (!workspace || workspace_bytes < static_cast<size_t>(need) || !aligned(workspace, 16))
+      return fail(GDN_ERR_INVALID, "gdn_linear_act: needs a 16-byte aligned workspace of %lld bytes (got %zu)",
+                  (long long)need, workspace_bytes);
+    p.slices = t.slices;
+    p.slice = static_cast<int>((steps + t.slices - 1) / t.slices * 64);
+    p.pitch = static_cast<int>(part_pitch(N, pair));
+    p.part = static_cast<float*>(workspace);
+    if (static_cast<int64_t>(p.slice) * (t.slices - 1) >= K)  // (no slice is empty)
+      p.slices = static_cast<int>((K + p.slice - 1) / p.slice);
+  }
+  if (pair) launch_tiles<true>(p, t, bare, st);
+  else launch_tiles<false>(p, t, bare, st);
   return gdn_host::check_launch("gdn_linear_act");
 }

@@ -42,6 +42,9 @@ struct ProductParams {
   int64_t ldo;
   int M, N, K;             // rows (no plan), columns of out
   int n_tiles;             // tiles of columns
+  // K in slices of `slice` values: slice i's sums go to part + i M pitch, a row's columns (its ups from pitch / 2 on)
+  int slices, slice, pitch;
+  float* part;
   // a plan: the tiles, how many; row r's row of x is from[r] (NULL: r itself), its row of out to[r] (NULL: r)
   const TileOf* tiles;
   const int* count;
@@ -234,11 +237,12 @@ enum Store {
   kBare,    // SwiGLU or nothing, to bf16
   kPacked,  // nothing, four sums in eight bytes
   kFinish,  // all of the epilogue
+  kPart,    // a slice of K's sums, as they are
 };
 
 // The epilogue of a tile's sums: lane (lr, lq) holds columns 4 lq + 0..3 of its 16-column blocks of row lr of its 16-row
-// blocks.  Where nothing but SwiGLU is to be done, straight from the registers.  The rest goes through LDS, WM blocks of
-// rows at a time, eight neighbouring columns a thread, so that its code stands there once and not for each of a lane's
+// blocks.  Where nothing but SwiGLU is to be done, straight from the registers.  The rest goes through LDS, as many
+// rows at a time as there is room for, eight neighbouring columns a thread, so that its code stands there once and not for each of a lane's
 // up to 128 sums: those had the experts' second product (4096 tokens, 2048 x 512, 8 of 256) wait 80 us for instructions.
 template <class S, int MB, Store ST>
 __device__ __forceinline__ void product_store(const ProductParams& p, f32x4 (&acc)[MB][S::NB], int n0, int row0, int rows,
@@ -252,24 +256,27 @@ __device__ __forceinline__ void product_store(const ProductParams& p, f32x4 (&ac
 
   if constexpr (ST == kFinish) {
     constexpr int PITCH = S::WR + 4;  // floats a row
-    constexpr int PASS = 16 * WM;     // rows at a time
-    static_assert(WK * PASS * PITCH * 4 <= S::LDS, "the sums fit");
+    constexpr int FIT = S::LDS / (WK * 16 * WM * PITCH * 4);  // blocks of rows a wave that there is room for
+    constexpr int PB = FIT >= MB ? MB : FIT >= 4 ? 4 : FIT >= 2 ? 2 : 1;
+    constexpr int PASS = 16 * WM * PB;  // rows at a time
+    static_assert(FIT >= 1 && MB % PB == 0, "the sums fit");
     float* sums = reinterpret_cast<float*>(smem);
-    for (int i = 0; i < MB; ++i) {
+    for (int i = 0; i < MB; i += PB) {
       if (16 * WM * i >= rows) break;
       __syncthreads();  // the stages, or the pass before, have been read
       unrolled<0, MB>([&](auto at) {
         constexpr int k = at;
-        if (i == k) {
+        if (i == k / PB * PB) {
 #pragma unroll
           for (int b = 0; b < NB; ++b)
-            *reinterpret_cast<f32x4*>(sums + (wk * PASS + 16 * wm + lr) * PITCH + (wn * NB + b) * 16 + 4 * lq) = acc[k][b];
+            *reinterpret_cast<f32x4*>(sums + (wk * PASS + 16 * (k % PB * WM + wm) + lr) * PITCH + (wn * NB + b) * 16 + 4 * lq) =
+                acc[k][b];
         }
       });
       __syncthreads();
       for (int at = threadIdx.x; at < PASS * S::COLS / CPL; at += S::NT) {
         const int r = at / (S::COLS / CPL), oc = at % (S::COLS / CPL) * CPL;
-        const int row = PASS * i + r, c = n0 + oc;
+        const int row = 16 * WM * i + r, c = n0 + oc;
         if (row >= rows || c >= p.N) continue;
         const float* from = sums + r * PITCH + (S::PAIR ? oc / (8 * NB) * (16 * NB) + oc % (8 * NB) : oc);
         float v[CPL], up[CPL];
@@ -284,6 +291,19 @@ __device__ __forceinline__ void product_store(const ProductParams& p, f32x4 (&ac
           }
         }
         finish8<S::PAIR>(p, v, up, p.to ? p.to[row0 + row] : row0 + row, c);
+      }
+    }
+  } else if constexpr (ST == kPart) {
+    static_assert(WK == 1, "groups sum up in LDS");
+#pragma unroll
+    for (int i = 0; i < MB; ++i) {
+      const int r = 16 * (i * WM + wm) + lr;
+      if (r >= rows) continue;
+      float* out = p.part + static_cast<int64_t>(row0 + r) * p.pitch;
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {  // (the pitch's halves hold whole fours)
+        const int c = n0 + (wn * OB + b % OB) * 16 + 4 * lq;
+        if (c < p.N) *reinterpret_cast<f32x4*>(out + c + (b < OB ? 0 : p.pitch / 2)) = acc[i][b];
       }
     }
   } else {
@@ -339,6 +359,7 @@ __device__ __forceinline__ void product_store(const ProductParams& p, f32x4 (&ac
 template <class S, int MB, Store ST>
 __device__ __forceinline__ void product_tile(const ProductParams& p, const uint16_t* w, int n0, int row0, int rows,
                                              unsigned char* smem) {
+  const int K = ST == kPart ? min(p.slice, p.K) : p.K;
   constexpr int NB = S::NB, WM = S::WM, WK = S::WK, NG = S::NG, WR = S::WR;
   constexpr int STAGE = (WR + 16 * MB * WM) * 128;      // bytes
   constexpr int FIT = S::LDS / (STAGE * WK), STAGES = FIT < 4 ? FIT : 4;
@@ -379,7 +400,7 @@ __device__ __forceinline__ void product_tile(const ProductParams& p, const uint1
   unsigned char* stages = smem + wk * (STAGES * STAGE);
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(stages));
   // the group's steps: wk, wk + WK, ... (groups that meet have as many each, which past K are of zeros)
-  const int nk = ((p.K + 63) / 64 - (NG > 1 ? 0 : wk) + WK - 1) / WK;
+  const int nk = ((K + 63) / 64 - (NG > 1 ? 0 : wk) + WK - 1) / WK;
 
   const uint16_t* wb = w + static_cast<int64_t>(n0) * p.K;
   auto load_part = [&](int s, int st, auto at) {
@@ -388,11 +409,11 @@ __device__ __forceinline__ void product_tile(const ProductParams& p, const uint1
     const uint32_t base = lds0 + st * STAGE;
     if constexpr (i < WI) {
       const int j = i * NG + wg;
-      lds_dma16(buf_words(wb + k0, kWhole), k0 + granule(j) * 8 < p.K ? w_off[i] : kOutside,
+      lds_dma16(buf_words(wb + k0, kWhole), k0 + granule(j) * 8 < K ? w_off[i] : kOutside,
                 __builtin_amdgcn_readfirstlane(base + j * 1024));
     } else {
       const int j = ((i - WI) * NG + wg) % XL;
-      lds_dma16(buf_words(x + k0, kWhole), k0 + granule(j) * 8 < p.K ? x_off[i - WI] : kOutside,
+      lds_dma16(buf_words(x + k0, kWhole), k0 + granule(j) * 8 < K ? x_off[i - WI] : kOutside,
                 __builtin_amdgcn_readfirstlane(base + WR * 128 + j * 1024));
     }
   };
@@ -465,14 +486,23 @@ __device__ __forceinline__ void product_rows(const ProductParams& p, const uint1
 
 // PLAN: an expert's tiles of the plan (whose rows vary), or the M rows of x.
 template <class S, Store ST, bool PLAN>
-__global__ __launch_bounds__(S::NT) void product_kernel(const ProductParams p) {
+__global__ __launch_bounds__(S::NT) void product_kernel(ProductParams p) {
   __shared__ __align__(1024) unsigned char smem[S::LDS];
   // Block b normally runs on XCD b % 8: each XCD takes neighbouring tiles, which read the same rows and weights, into
   // its L2.  (What a plan holds is only known here: the launch's blocks past it leave.)
   const uint32_t m_tiles = PLAN ? p.count[0] : (p.M + S::ROWS - 1) / S::ROWS;
-  const uint32_t total = m_tiles * p.n_tiles, per = (total + kXcds - 1) / kXcds, local = blockIdx.x / kXcds;
-  const uint32_t t = blockIdx.x % kXcds * per + local;
+  const uint32_t total = m_tiles * p.n_tiles * (ST == kPart ? p.slices : 1);
+  const uint32_t per = (total + kXcds - 1) / kXcds, local = blockIdx.x / kXcds;
+  uint32_t t = blockIdx.x % kXcds * per + local;
   if (local >= per || t >= total) return;
+  if constexpr (ST == kPart) {  // all tiles of a slice before the next one's
+    const int slice = static_cast<int>(t / (m_tiles * p.n_tiles)), k0 = slice * p.slice;
+    t %= m_tiles * p.n_tiles;
+    p.x += k0;
+    p.w += k0;
+    p.part += static_cast<int64_t>(slice) * p.M * p.pitch;
+    p.slice = min(p.slice, p.K - k0);
+  }
   if constexpr (PLAN) {
     const TileOf of = p.tiles[t / p.n_tiles];
     product_rows<S, ST, false, S::BY>(p, p.w + of.expert * p.expert_stride, static_cast<int>(t % p.n_tiles) * S::COLS,
@@ -488,7 +518,7 @@ __global__ __launch_bounds__(S::NT) void product_kernel(const ProductParams p) {
 template <class S, Store ST, bool PLAN>
 void launch_product(ProductParams p, int64_t m_tiles, hipStream_t st) {
   p.n_tiles = (p.N + S::COLS - 1) / S::COLS;
-  const int64_t blocks = (m_tiles * p.n_tiles + kXcds - 1) / kXcds * kXcds;
+  const int64_t blocks = (m_tiles * p.n_tiles * (ST == kPart ? p.slices : 1) + kXcds - 1) / kXcds * kXcds;
   hipLaunchKernelGGL((product_kernel<S, ST, PLAN>), dim3(static_cast<unsigned>(blocks)), dim3(S::NT), 0, st, p);
 }
 

@@ -7,9 +7,11 @@
 // Scores are formed in 64 bits: which of two experts is taken must not hang on how a score was rounded, and at a
 // token's few hundred experts the 64-bit exponentials (full rate on gfx950) are not what the time goes to.
 //
-// LPT lanes share a token, lane l holding its experts l, l + LPT, ...; the k rounds of an arg max are VALU row moves.
-// 64 lanes a token finish a decode step's few tokens soonest, 16 take the fewest instructions for many.
+// LPT lanes share a token, lane l holding its experts l, l + LPT, ...; the k rounds of an arg max, which bound it, are
+// VALU moves between lanes.  64 lanes a token finish a decode step's few tokens soonest, 32 take fewer instructions for
+// many.
 #include <climits>
+#include <cmath>
 
 #include "gdn_common.hpp"
 
@@ -36,29 +38,39 @@ struct RouteParams {
   double scale;
 };
 
-__device__ __forceinline__ int row_move(int x, int step) {
-  switch (step) {
+// The value of the lane that step s of a reduction meets: inside 16 lanes, then the other 16, then the other 32.
+__device__ __forceinline__ int partner(int x, int s) {
+  const bool odd = (threadIdx.x >> (s == 4 ? 4 : 5)) & 1;
+  switch (s) {
     case 0: return __builtin_amdgcn_mov_dpp(x, GDN_DPP_QUAD_XOR1, 0xF, 0xF, false);
     case 1: return __builtin_amdgcn_mov_dpp(x, GDN_DPP_QUAD_XOR2, 0xF, 0xF, false);
     case 2: return __builtin_amdgcn_mov_dpp(x, GDN_DPP_HALF_MIRROR, 0xF, 0xF, false);
     case 3: return __builtin_amdgcn_mov_dpp(x, GDN_DPP_ROW_MIRROR, 0xF, 0xF, false);
-    default: return __shfl_xor(x, step == 4 ? 16 : 32, 64);
+    case 4: {  // [0]: the even rows in both places, [1]: the odd ones
+      const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+      return odd ? r[0] : r[1];
+    }
+    default: {
+      const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+      return odd ? r[0] : r[1];
+    }
   }
 }
-__device__ __forceinline__ double row_move(double x, int step) {
+__device__ __forceinline__ double partner(double x, int s) {
   const int64_t b = __builtin_bit_cast(int64_t, x);
-  const uint32_t lo = row_move(static_cast<int>(b), step), hi = row_move(static_cast<int>(b >> 32), step);
+  const uint32_t lo = partner(static_cast<int>(b), s), hi = partner(static_cast<int>(b >> 32), s);
   return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
 }
 
 template <int LPT, class F, class X>
 __device__ __forceinline__ X over_lanes(X x, F f) {
 #pragma unroll
-  for (int s = 0; s < (LPT == 64 ? 6 : 4); ++s) x = f(x, row_move(x, s));
+  for (int s = 0; s < (LPT == 64 ? 6 : LPT == 32 ? 5 : 4); ++s) x = f(x, partner(x, s));
   return x;
 }
-// (neither operand is NaN where these are used)
-__device__ __forceinline__ double larger(double a, double b) { return a > b ? a : b; }
+__device__ __forceinline__ double larger(double a, double b) { return __builtin_fmax(a, b); }  // (of a number and NaN the number)
+__device__ __forceinline__ double added(double a, double b) { return a + b; }
+__device__ __forceinline__ int smaller(int a, int b) { return a < b ? a : b; }
 
 template <int LPT, int VPL>
 __global__ __launch_bounds__(kThreads) void route_kernel(const RouteParams p) {
@@ -81,14 +93,14 @@ __global__ __launch_bounds__(kThreads) void route_kernel(const RouteParams p) {
   if (!p.sigmoid) {
     top = -INFINITY;
 #pragma unroll
-    for (int v = 0; v < VPL; ++v) top = c[v] > top ? c[v] : top;
+    for (int v = 0; v < VPL; ++v) top = larger(top, c[v]);
     top = over_lanes<LPT>(top, larger);
     if (top == -INFINITY) top = 0.0;  // nothing but -inf (and NaN): scores of 0
     sum = 0.0;
 #pragma unroll
     for (int v = 0; v < VPL; ++v)
       if (lane + v * LPT < p.E) sum += exp(c[v] - top);
-    sum = over_lanes<LPT>(sum, [](double a, double b) { return a + b; });
+    sum = over_lanes<LPT>(sum, added);
     if (sum == 0.0) sum = 1.0;
   }
   auto score = [&](double x) { return p.sigmoid ? 1.0 / (1.0 + exp(-x)) : exp(x - top) / sum; };
@@ -105,59 +117,76 @@ __global__ __launch_bounds__(kThreads) void route_kernel(const RouteParams p) {
 
   if (p.top_groups < p.groups) {
     const int width = p.E / p.groups;
+    double* mine = group_s + slot * kMaxGroups;
     __syncthreads();
     for (int g = lane; g < p.groups; g += LPT) {
       const double* at = group_c + slot * (LPT * VPL) + g * width;
       double best = -INFINITY, second = -INFINITY;
-      for (int i = 0; i < width; ++i) {
-        const double x = at[i];  // (NaN is never larger)
-        if (x > best) {
-          second = best;
-          best = x;
-        } else if (x > second) {
-          second = x;
-        }
+      for (int i = 0; i < width; ++i) {  // (NaN counts as -inf)
+        const double x = larger(at[i], -INFINITY);
+        second = larger(second, x < best ? x : best);
+        best = larger(best, x);
       }
-      group_s[slot * kMaxGroups + g] = p.group_best > 1 && width > 1 ? best + second : best;
+      mine[g] = p.group_best > 1 && width > 1 ? best + second : best;
     }
     __syncthreads();
+    uint64_t stay = 0;  // a lane's groups that stay, then all lanes'
+    for (int g = lane; g < p.groups; g += LPT) {
+      const double s = mine[g];
+      int before = 0;  // groups that come first: larger, or as large with a lower index
+      for (int o = 0; o < p.groups; ++o) before += mine[o] > s || (mine[o] == s && o < g) ? 1 : 0;
+      stay |= static_cast<uint64_t>(before < p.top_groups) << g;
+    }
+    const uint32_t lo = over_lanes<LPT>(static_cast<int>(stay), [](int a, int b) { return a | b; });
+    const uint32_t hi = over_lanes<LPT>(static_cast<int>(stay >> 32), [](int a, int b) { return a | b; });
+    stay = static_cast<uint64_t>(hi) << 32 | lo;
 #pragma unroll
     for (int v = 0; v < VPL; ++v) {
-      const int e = lane + v * LPT, g = e / width;
-      if (e >= p.E) continue;
-      const double mine = group_s[slot * kMaxGroups + g];
-      int before = 0;  // groups that come first: larger, or as large with a lower index
-      for (int o = 0; o < p.groups; ++o) {
-        const double other = group_s[slot * kMaxGroups + o];
-        before += other > mine || (other == mine && o < g) ? 1 : 0;
-      }
-      if (before >= p.top_groups) left &= ~(1u << v);
+      const int e = lane + v * LPT;
+      if (e < p.E && !(stay >> (e / width) & 1)) left &= ~(1u << v);
     }
   }
 
   // k times the largest c that is left (NaN counts below every number), the lowest index of equals; choice j is lane j's
   int chosen = -1;
+  double w = 0.0;
+#pragma unroll
+  for (int v = 0; v < VPL; ++v)
+    if (!(left >> v & 1)) c[v] = -INFINITY;
   for (int j = 0; j < p.k; ++j) {
     double best = -INFINITY;
 #pragma unroll
-    for (int v = 0; v < VPL; ++v)
-      if (left >> v & 1 && c[v] > best) best = c[v];
+    for (int v = 0; v < VPL; ++v) best = larger(best, c[v]);
     best = over_lanes<LPT>(best, larger);
-    int at = INT_MAX, nan = INT_MAX;
+    int at = INT_MAX;
+    // (what cannot be chosen, or has been, is -inf, which only the last ones left may be too)
+    const uint32_t open = best > -INFINITY ? ~0u : left;
 #pragma unroll
-    for (int v = VPL - 1; v >= 0; --v) {
-      if (left >> v & 1 && c[v] == best) at = lane + v * LPT;
-      if (left >> v & 1 && c[v] != c[v]) nan = lane + v * LPT;
+    for (int v = VPL - 1; v >= 0; --v)
+      if (c[v] == best && open >> v & 1) at = lane + v * LPT;
+    at = over_lanes<LPT>(at, smaller);
+    if (at == INT_MAX) {  // nothing but NaN is left
+#pragma unroll
+      for (int v = VPL - 1; v >= 0; --v)
+        if (left >> v & 1) at = lane + v * LPT;
+      at = over_lanes<LPT>(at, smaller);
+      best = NAN;
     }
-    at = over_lanes<LPT>(at, [](int a, int b) { return a < b ? a : b; });
-    if (at == INT_MAX) at = over_lanes<LPT>(nan, [](int a, int b) { return a < b ? a : b; });
-    if (at % LPT == lane) left &= ~(1u << (at / LPT));
-    if (j == lane) chosen = at;  // (k <= LPT)
+    if (lane == j) {  // (k <= LPT)
+      chosen = at;
+      w = best;
+    }
+#pragma unroll
+    for (int v = 0; v < VPL; ++v) {
+      if (at != lane + v * LPT) continue;
+      c[v] = -INFINITY;
+      left &= ~(1u << v);
+    }
   }
-  double w = 0.0;
-  if (lane < p.k) w = score(static_cast<double>(load_any(p.logits, p.dt, row * p.ld + chosen)));
+  if (lane >= p.k) w = 0.0;
+  else if (p.bias) w = score(static_cast<double>(load_any(p.logits, p.dt, row * p.ld + chosen)));
   if (p.renormalize) {
-    const double all = over_lanes<LPT>(w, [](double a, double b) { return a + b; });
+    const double all = over_lanes<LPT>(w, added);
     w = all == 0.0 ? 0.0 : w / all;
   }
   if (n < p.N && lane < p.k) {
@@ -214,8 +243,21 @@ extern "C" int gdn_route_experts(const void* logits, int dtype, int64_t ld, cons
   p.renormalize = renormalize != 0;
   p.scale = scale;
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  if (E <= 64) launch<64, 1>(p, st);
-  else if (E <= 256) launch<64, 4>(p, st);
-  else launch<64, 16>(p, st);
+  // us with 64 and 32 lanes a token, 8 of 256: 1024 tokens 6.7, 8.9; 4096 12.7, 11.2; 16384 37.6, 29.4 (16 lanes: 14.0,
+  // 14.5, 28.4)
+  if (p.N >= 3500 && k <= 32 && E <= 256) {
+    if (E <= 64) launch<32, 2>(p, st);
+    else launch<32, 8>(p, st);
+  } else if (E <= 64) {
+    launch<64, 1>(p, st);
+  } else if (E <= 128) {
+    launch<64, 2>(p, st);
+  } else if (E <= 256) {
+    launch<64, 4>(p, st);
+  } else if (E <= 512) {
+    launch<64, 8>(p, st);
+  } else {
+    launch<64, 16>(p, st);
+  }
   return gdn_host::check_launch("gdn_route_experts");
 }

@@ -30,6 +30,7 @@ each).
 
 from __future__ import annotations
 
+import functools
 from typing import Optional
 
 import torch
@@ -38,7 +39,7 @@ import torch.autograd.forward_ad as forward_ad
 from . import _lib
 from .gated_delta import _dtype_code, _ptr, _require_device, _stream
 
-__all__ = ["linear", "linear_act", "DECODE_MAX_ROWS", "FUSED_NORM_MAX_ROWS", "DecodeWorkspace", "linear_decode",
+__all__ = ["linear", "linear_act", "linear_act_workspace_bytes", "DECODE_MAX_ROWS", "FUSED_NORM_MAX_ROWS", "DecodeWorkspace", "linear_decode",
            "gated_norm_linear_decode", "linear_decode_workspace_bytes", "decode_shape_ok"]
 
 DECODE_MAX_ROWS = 64
@@ -265,7 +266,8 @@ def _out_rows(out: torch.Tensor, shape, added: Optional[torch.Tensor], reads, na
 
 def linear_act(x: torch.Tensor, weight: torch.Tensor, *, bias: Optional[torch.Tensor] = None,
                activation: Optional[str] = None, row_gate: Optional[torch.Tensor] = None,
-               residual: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+               residual: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+               workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``act(x @ weight.T + bias) * sigmoid(row_gate) + residual`` in one launch
     (``gdn_linear_act``), rounded once.
 
@@ -275,12 +277,14 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, *, bias: Optional[torch.Te
     bias ``[rows of weight]``, row_gate ``[...]`` (one logit per row of x, such as
     a column of another product) in bf16, fp16 or fp32; residual ``[..., N]`` bf16.
     x and residual may be column slices of wider buffers.  ``out`` may be the
-    residual itself.  There is no backward.
+    residual itself.  ``workspace``: bytes for the sums of K's slices, which some
+    sizes are formed in (:func:`linear_act_workspace_bytes`; allocated when absent
+    or too small); calls that overlap need one each.  There is no backward.
     """
     # a plain call's checks in a few operations; what is wrong, or laid out otherwise, is looked into below
     index, bf16, act = x.get_device(), torch.bfloat16, _ACTS.get(activation)
     if (index >= 0 and act is not None and x.dtype is bf16 and weight.dtype is bf16 and weight.dim() == 2 and x.dim() > 0
-            and bias is None and row_gate is None and out is None and weight.get_device() == index
+            and bias is None and row_gate is None and out is None and workspace is None and weight.get_device() == index
             and x.is_contiguous() and weight.is_contiguous()
             and not (torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
                                                   or residual is not None and residual.requires_grad))):
@@ -290,19 +294,27 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, *, bias: Optional[torch.Te
         if (x.shape[-1] == K and K > 0 and K % 8 == 0 and N > 0 and (act != 5 or rows % 2 == 0) and (xp | wp) % 16 == 0
                 and (residual is None or residual.dtype is bf16 and residual.get_device() == index
                      and residual.shape == shape and residual.is_contiguous())):
-            dev = x.device
+            dev, M = x.device, x.numel() // K
             out = torch.empty(shape, dtype=bf16, device=dev)
+            need = linear_act_workspace_bytes(M, N, K, activation)
+            ws = torch.empty(need, dtype=torch.uint8, device=dev).data_ptr() if need else None
             _lib.call(dev, "gdn_linear_act", xp, K, wp, None, 0, act, None, 0, 0,
-                      None if residual is None else residual.data_ptr(), N, out.data_ptr(), N, x.numel() // K, N, K,
+                      None if residual is None else residual.data_ptr(), N, out.data_ptr(), N, M, N, K, ws, need,
                       _stream(dev))
             return out
-    return _linear_act_general(x, weight, bias, activation, row_gate, residual, out)
+    return _linear_act_general(x, weight, bias, activation, row_gate, residual, out, workspace)
 
 
-def _linear_act_general(x, weight, bias, activation, row_gate, residual, out):
+@functools.lru_cache(maxsize=4096)
+def linear_act_workspace_bytes(rows: int, N: int, K: int, activation: Optional[str] = None) -> int:
+    """Bytes that :func:`linear_act` needs as its workspace (0 for most sizes)."""
+    return int(_lib.load().gdn_linear_act_workspace_bytes(rows, N, K, _ACTS[activation]))
+
+
+def _linear_act_general(x, weight, bias, activation, row_gate, residual, out, workspace):
     """:func:`linear_act` of any layout; raises what is wrong with its arguments."""
-    dev = _require_device((x, weight, bias, row_gate, residual, out),
-                          ("x", "weight", "bias", "row_gate", "residual", "out"))
+    dev = _require_device((x, weight, bias, row_gate, residual, out, workspace),
+                          ("x", "weight", "bias", "row_gate", "residual", "out", "workspace"))
     if activation not in _ACTS:
         raise ValueError(f"activation must be one of {[a for a in _ACTS]} (got {activation!r})")
     if x.dtype is not torch.bfloat16 or weight.dtype is not torch.bfloat16:
@@ -349,8 +361,15 @@ def _linear_act_general(x, weight, bias, activation, row_gate, residual, out):
         out = torch.empty(shape, dtype=torch.bfloat16, device=dev)
         ldo = N
     else:
-        _out_rows(out, shape, residual, (x, weight, bias, row_gate), ("x", "weight", "bias", "row_gate"))
+        _out_rows(out, shape, residual, (x, weight, bias, row_gate, workspace),
+                  ("x", "weight", "bias", "row_gate", "workspace"))
         ldo = _even_rows(out)
+    need = linear_act_workspace_bytes(M, N, K, activation)
+    if workspace is not None and not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous")
+    if workspace is None or workspace.numel() * workspace.element_size() < need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     _lib.call(dev, "gdn_linear_act", x.data_ptr(), ldx, weight.data_ptr(), _ptr(bias), bias_dt, act, _ptr(row_gate),
-              gate_dt, ldg, _ptr(residual), ldr, out.data_ptr(), ldo, M, N, K, _stream(dev))
+              gate_dt, ldg, _ptr(residual), ldr, out.data_ptr(), ldo, M, N, K, _ptr(workspace),
+              0 if workspace is None else workspace.numel() * workspace.element_size(), _stream(dev))
     return out

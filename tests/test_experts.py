@@ -129,7 +129,7 @@ def test_expert_mlp_workspace(lib):
 
 def _linear(lib, **kw):
     a = dict(x=FAKE, ldx=64, W=FAKE, bias=None, bdt=0, act=0, gate=None, gdt=0, ldg=0, res=None, ldr=0, out=FAKE, ldo=48,
-             M=4, N=48, K=64)
+             M=4, N=48, K=64, ws=None, bytes=0)
     a.update(kw)
     return lib.gdn_linear_act(*a.values(), None)
 
@@ -146,10 +146,22 @@ def _linear(lib, **kw):
     (dict(M=1 << 31), _lib.ERR_INVALID), (dict(N=1 << 30, ldo=1 << 30), _lib.ERR_INVALID),
     (dict(act=5, N=1 << 24, K=64, ldo=1 << 24), _lib.ERR_UNSUPPORTED),  # gate and up more than 2 GiB apart
     (dict(K=1 << 23, ldx=1 << 23), _lib.ERR_UNSUPPORTED), (dict(ldx=1 << 23), _lib.ERR_UNSUPPORTED),
+    (dict(M=512, N=4096, K=12288, ldx=12288, ldo=4096), _lib.ERR_INVALID),  # without its workspace
+    (dict(M=512, N=4096, K=12288, ldx=12288, ldo=4096, ws=FAKE, bytes=1000), _lib.ERR_INVALID),
+    (dict(M=512, N=4096, K=12288, ldx=12288, ldo=4096, ws=FAKE + 8, bytes=1 << 40), _lib.ERR_INVALID),
     (dict(M=0, x=None), _lib.OK),
 ])
 def test_linear_act_abi_refusals(lib, kw, status):
     assert _linear(lib, **kw) == status
+
+
+def test_linear_act_workspace(lib):
+    """None for most sizes; where K is summed in slices, four bytes a sum and slice."""
+    f = linear.linear_act_workspace_bytes
+    assert f(1, 4096, 12288) == 0 and f(4096, 12288, 4096, "swiglu") == 0 and f(128, 4096, 2048) == 0
+    assert f(512, 4096, 12288) % (512 * 4096 * 4) == 0 and f(512, 4096, 12288) >= 2 * 512 * 4096 * 4
+    assert lib.gdn_linear_act_workspace_bytes(512, 4096, 12289, 0) == 0
+    assert lib.gdn_linear_act_workspace_bytes(512, 4096, 12288, 9) == 0
 
 
 # --------------------------------------------------------------- the Python calls

@@ -99,6 +99,25 @@ def test_linear_act(M, N, K, act):
     _check_linear(y, x, w, bias, act, gate, res)
 
 
+@pytest.mark.parametrize("act", [None, "gelu", "swiglu"])
+@pytest.mark.parametrize("M,N,K", [(600, 1000, 8200), (64, 1026, 8192), (130, 517, 12296)])
+def test_linear_act_in_slices(M, N, K, act):
+    """Sizes whose K is summed in slices, through a workspace that holds NaN."""
+    need = mx.linear_act_workspace_bytes(M, N, K, act)
+    if not need:
+        pytest.skip("no slices at this size")
+    g = _gen(K)
+    rows = 2 * N if act == "swiglu" else N
+    x, w = _r(g, M, K), _r(g, rows, K, scale=K ** -0.5)
+    bias, gate, res = _r(g, rows), _r(g, M, dtype=torch.float32), _r(g, M, N)
+    ws = torch.full((need + 16,), 0xff, dtype=torch.uint8, device=DEV)
+    y = mx.linear_act(x, w, bias=bias, activation=act, row_gate=gate, residual=res, workspace=ws)
+    _check_linear(y, x, w, bias, act, gate, res)
+    assert (ws[need:] == 0xff).all()
+    assert torch.equal(y, mx.linear_act(x, w, bias=bias, activation=act, row_gate=gate, residual=res, workspace=ws[:16]))
+    _check_linear(mx.linear_act(x, w, activation=act), x, w, None, act, None, None)
+
+
 @pytest.mark.parametrize("M", [1, 3, 40, 400])
 @pytest.mark.parametrize("act", [None, "swiglu"])
 def test_linear_act_strided(M, act):
