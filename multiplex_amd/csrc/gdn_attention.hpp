@@ -508,14 +508,6 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buf_rsrc(const void* base, uin
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, static_cast<int>(bytes), 0x00020000);
 }
 
-// lds_dma16 for bytes that are read once: not kept in the caches.
-__device__ __forceinline__ void lds_dma16_once(u32x4 rsrc, uint32_t voff, uint32_t lds_base) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen nt lds"
-               :
-               : "v"(voff), "s"(rsrc), "s"(lds_base)
-               : "memory", "m0");
-}
-
 // Max / sum over the four 16-lane rows of a wave (lanes r, r + 16, r + 32, r + 48), by the
 // gfx950 row-swap moves (VALU, no LDS round trip): permlane16_swap(x, x) yields the even and the
 // odd rows, permlane32_swap(x, x) the low and the high halves, each in both places.

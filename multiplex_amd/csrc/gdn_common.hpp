@@ -381,6 +381,14 @@ __device__ __forceinline__ void lds_dma16(u32x4 rsrc, uint32_t voff, uint32_t ld
                : "v"(voff), "s"(rsrc), "s"(lds_base)
                : "memory", "m0");
 }
+// lds_dma16 for bytes that are read once: not kept in the caches.
+__device__ __forceinline__ void lds_dma16_once(u32x4 rsrc, uint32_t voff, uint32_t lds_base) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen nt lds"
+               :
+               : "v"(voff), "s"(rsrc), "s"(lds_base)
+               : "memory", "m0");
+}
+
 // ------------------------------------------- 8-element row slices
 
 constexpr int CPL = 8;  // channels per lane

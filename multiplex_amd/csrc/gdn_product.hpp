@@ -356,7 +356,8 @@ __device__ __forceinline__ void product_store(const ProductParams& p, f32x4 (&ac
   }
 }
 
-template <class S, int MB, Store ST>
+// ONCE: W is read once or a few times soon after each other: it does not stay in the caches.
+template <class S, int MB, Store ST, bool ONCE>
 __device__ __forceinline__ void product_tile(const ProductParams& p, const uint16_t* w, int n0, int row0, int rows,
                                              unsigned char* smem) {
   const int K = ST == kPart ? min(p.slice, p.K) : p.K;
@@ -409,8 +410,10 @@ __device__ __forceinline__ void product_tile(const ProductParams& p, const uint1
     const uint32_t base = lds0 + st * STAGE;
     if constexpr (i < WI) {
       const int j = i * NG + wg;
-      lds_dma16(buf_words(wb + k0, kWhole), k0 + granule(j) * 8 < K ? w_off[i] : kOutside,
-                __builtin_amdgcn_readfirstlane(base + j * 1024));
+      const uint32_t off = k0 + granule(j) * 8 < K ? w_off[i] : kOutside;
+      const uint32_t to = __builtin_amdgcn_readfirstlane(base + j * 1024);
+      if (ONCE) lds_dma16_once(buf_words(wb + k0, kWhole), off, to);
+      else lds_dma16(buf_words(wb + k0, kWhole), off, to);
     } else {
       const int j = ((i - WI) * NG + wg) % XL;
       lds_dma16(buf_words(x + k0, kWhole), k0 + granule(j) * 8 < K ? x_off[i - WI] : kOutside,
@@ -474,18 +477,18 @@ __device__ __forceinline__ void product_tile(const ProductParams& p, const uint1
 }
 
 // Runs the tile with a number of 16-row blocks a wave that holds its rows: MB, 2 MB, 3 MB, ... or (DOUBLE) 2 MB, 4 MB, ...
-template <class S, Store ST, bool DOUBLE, int MB>
+template <class S, Store ST, bool DOUBLE, bool ONCE, int MB>
 __device__ __forceinline__ void product_rows(const ProductParams& p, const uint16_t* w, int n0, int row0, int rows,
                                              unsigned char* smem) {
   constexpr int NEXT = DOUBLE ? 2 * MB : MB + S::BY;
   if constexpr (NEXT <= S::MAXB) {
-    if (rows > 16 * S::WM * MB) return product_rows<S, ST, DOUBLE, NEXT>(p, w, n0, row0, rows, smem);
+    if (rows > 16 * S::WM * MB) return product_rows<S, ST, DOUBLE, ONCE, NEXT>(p, w, n0, row0, rows, smem);
   }
-  product_tile<S, MB, ST>(p, w, n0, row0, rows, smem);
+  product_tile<S, MB, ST, ONCE>(p, w, n0, row0, rows, smem);
 }
 
 // PLAN: an expert's tiles of the plan (whose rows vary), or the M rows of x.
-template <class S, Store ST, bool PLAN>
+template <class S, Store ST, bool PLAN, bool ONCE>
 __global__ __launch_bounds__(S::NT) void product_kernel(ProductParams p) {
   __shared__ __align__(1024) unsigned char smem[S::LDS];
   // Block b normally runs on XCD b % 8: each XCD takes neighbouring tiles, which read the same rows and weights, into
@@ -505,21 +508,21 @@ __global__ __launch_bounds__(S::NT) void product_kernel(ProductParams p) {
   }
   if constexpr (PLAN) {
     const TileOf of = p.tiles[t / p.n_tiles];
-    product_rows<S, ST, false, S::BY>(p, p.w + of.expert * p.expert_stride, static_cast<int>(t % p.n_tiles) * S::COLS,
+    product_rows<S, ST, false, ONCE, S::BY>(p, p.w + of.expert * p.expert_stride, static_cast<int>(t % p.n_tiles) * S::COLS,
                                       __builtin_amdgcn_readfirstlane(of.row), __builtin_amdgcn_readfirstlane(of.rows), smem);
   } else {
     // eight tiles of rows by all columns at a time
     const uint32_t band = 8 * p.n_tiles, first = t / band * 8, high = min(m_tiles - first, 8u), in = t % band;
     const int row0 = static_cast<int>(first + in % high) * S::ROWS;
-    product_rows<S, ST, true, 1>(p, p.w, static_cast<int>(in / high) * S::COLS, row0, min(p.M - row0, S::ROWS), smem);
+    product_rows<S, ST, true, ONCE, 1>(p, p.w, static_cast<int>(in / high) * S::COLS, row0, min(p.M - row0, S::ROWS), smem);
   }
 }
 
-template <class S, Store ST, bool PLAN>
+template <class S, Store ST, bool PLAN, bool ONCE = false>
 void launch_product(ProductParams p, int64_t m_tiles, hipStream_t st) {
   p.n_tiles = (p.N + S::COLS - 1) / S::COLS;
   const int64_t blocks = (m_tiles * p.n_tiles * (ST == kPart ? p.slices : 1) + kXcds - 1) / kXcds * kXcds;
-  hipLaunchKernelGGL((product_kernel<S, ST, PLAN>), dim3(static_cast<unsigned>(blocks)), dim3(S::NT), 0, st, p);
+  hipLaunchKernelGGL((product_kernel<S, ST, PLAN, ONCE>), dim3(static_cast<unsigned>(blocks)), dim3(S::NT), 0, st, p);
 }
 
 template <bool PAIR> using Thin = Shape<2, 1, 1, 4, 4, 1, 144, PAIR>;    // 64 rows by 32 weight rows
