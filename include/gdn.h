@@ -516,7 +516,7 @@ int gdn_rms_norm(const void* x, const void* res, void* h_out, const void* w, int
  */
 int gdn_route_experts(const void* logits, int dtype, int64_t ld, const float* bias, const int32_t* n_new,
                       int32_t* indices, float* weights, int64_t B, int64_t T, int64_t E, int64_t k, int sigmoid,
-                      int64_t groups, int64_t top_groups, int64_t group_best, int renormalize, float scale,
+                      int64_t groups, int64_t top_groups, int64_t group_best, int renormalize, double scale,
                       void* stream);
 
 /* Workspace bytes of gdn_expert_mlp (0 for sizes it does not take). */

@@ -10,7 +10,7 @@ import ctypes
 import os
 import struct
 import threading
-from ctypes import POINTER, Structure, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
+from ctypes import POINTER, Structure, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
 from pathlib import Path
 
 import torch
@@ -219,7 +219,7 @@ _SIGNATURES = {
     "gdn_rms_norm": (c_int, [_P, _P, _P, _P, c_int, _P, _I64, _I64, _I64, c_float, _P]),
     "gdn_route_experts": (
         c_int,
-        [_P, c_int, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _I64, c_int, _I64, _I64, _I64, c_int, c_float, _P],
+        [_P, c_int, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _I64, c_int, _I64, _I64, _I64, c_int, c_double, _P],
     ),
     "gdn_expert_mlp_workspace_bytes": (c_size_t, [_I64, _I64, _I64, _I64, _I64]),
     "gdn_expert_mlp": (

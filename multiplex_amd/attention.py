@@ -77,6 +77,7 @@ class AttentionArgs:
     shared_expert_intermediate_size: int = 0  # 0: no shared expert
     norm_topk_prob: bool = True
     scoring_func: str = "softmax"
+    router_bias: bool = False
     n_group: int = 1
     topk_group: int = 1
     routed_scaling_factor: float = 1.0

@@ -206,7 +206,7 @@ void launch(const RouteParams& p, hipStream_t st) {
 extern "C" int gdn_route_experts(const void* logits, int dtype, int64_t ld, const float* bias, const int32_t* n_new,
                                  int32_t* indices, float* weights, int64_t B, int64_t T, int64_t E, int64_t k,
                                  int sigmoid, int64_t groups, int64_t top_groups, int64_t group_best, int renormalize,
-                                 float scale, void* stream) {
+                                 double scale, void* stream) {
   using gdn_host::fail;
   if (B < 0 || T < 0 || E < 1 || E > kMaxExperts || k < 1 || k > kMaxChoices)
     return fail(GDN_ERR_INVALID, "gdn_route_experts: bad sizes B=%lld T=%lld E=%lld k=%lld (E up to %d, k up to %d)",

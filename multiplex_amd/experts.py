@@ -124,13 +124,14 @@ def expert_mlp(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor, indic
 
     ``workspace``: :func:`expert_mlp_workspace_bytes` bytes (allocated when absent
     or too small); calls that overlap need one each.  ``out`` may be the base
-    itself.  There is no backward.
+    itself, and otherwise lies apart from all that is read (other columns of one
+    buffer are refused too).  There is no backward.
     """
     index, bf16 = x.get_device(), torch.bfloat16
     E, H, I = down.shape if down.dim() == 3 else (0, 0, 0)
     lead, k = x.shape[:-1], indices.shape[-1] if indices.dim() else 0
     # a plain call's checks in a few operations; what is wrong, or laid out otherwise, is looked into below
-    if not (index >= 0 and out is None and x.dtype is bf16 and gate_up.dtype is bf16 and down.dtype is bf16
+    if not (index >= 0 and (out is None or out is base) and x.dtype is bf16 and gate_up.dtype is bf16 and down.dtype is bf16
             and indices.dtype is torch.int32 and weights.dtype is torch.float32 and gate_up.get_device() == index
             and down.get_device() == index and indices.get_device() == index and weights.get_device() == index
             and gate_up.shape == (E, 2 * I, H) and x.dim() > 0 and x.shape[-1] == H and indices.shape[:-1] == lead
@@ -143,7 +144,8 @@ def expert_mlp(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor, indic
                                                   weights.requires_grad or base is not None and base.requires_grad))):
         return _expert_mlp_general(x, gate_up, down, indices, weights, base, out, workspace)
     dev = x.device
-    return _expert_mlp_call(dev, x, H, gate_up, down, indices, weights, base, H, torch.empty_like(x), H, workspace,
+    return _expert_mlp_call(dev, x, H, gate_up, down, indices, weights, base, H,
+                            torch.empty_like(x) if out is None else out, H, workspace,
                             x.numel() // H if H else 0, H, I, E, k)
 
 
@@ -216,7 +218,7 @@ class SparseMLP(torch.nn.Module):
 
     The router's and the shared gate's rows are one weight (``router``: E rows,
     then the shared gate's), so both come from one product.  With
-    ``router_bias`` (set by :meth:`load`) the choice goes by scores plus it.
+    ``args.router_bias`` the choice goes by the scores plus ``router_bias``.
     """
 
     def __init__(self, args, device=None, dtype=torch.bfloat16):
@@ -230,7 +232,8 @@ class SparseMLP(torch.nn.Module):
         self.args = args
         self.E = E
         self.router = _weight(E + (1 if S else 0), H, device=device, dtype=dtype)
-        self.router_bias: Optional[torch.nn.Parameter] = None
+        self.router_bias = (torch.nn.Parameter(torch.zeros(E, device=device), requires_grad=False)
+                            if args.router_bias else None)
         self.gate_up_proj = _weight(E, 2 * I, H, device=device, dtype=dtype)
         self.down_proj = _weight(E, H, I, device=device, dtype=dtype)
         self.shared_gate_up_proj = _weight(2 * S, H, device=device, dtype=dtype) if S else None
@@ -245,23 +248,27 @@ class SparseMLP(torch.nn.Module):
         shared = (shared_gate_proj, shared_up_proj, shared_down_proj, shared_expert_gate)
         if any((t is None) != (self.shared_down_proj is None) for t in shared):
             raise ValueError("the shared expert's weights go with shared_expert_intermediate_size > 0, all of them")
+        if (router_bias is None) != (self.router_bias is None):
+            raise ValueError("a router bias goes with args.router_bias")
         self.router.copy_(gate if shared_expert_gate is None else torch.cat([gate, shared_expert_gate.view(1, -1)]))
         self.gate_up_proj.copy_(torch.cat([gate_proj, up_proj], 1))
         self.down_proj.copy_(down_proj)
         if self.shared_down_proj is not None:
             self.shared_gate_up_proj.copy_(torch.cat([shared_gate_proj, shared_up_proj]))
             self.shared_down_proj.copy_(shared_down_proj)
-        self.router_bias = None if router_bias is None else torch.nn.Parameter(
-            router_bias.to(self.router.device, torch.float32), requires_grad=False)
+        if router_bias is not None:
+            self.router_bias.copy_(router_bias)
 
     def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None,
                 n_new: Optional[torch.Tensor] = None) -> torch.Tensor:
         """The MLP of x ``[..., H]``, plus ``residual`` where given.  With x ``[B, T, H]``,
         ``n_new`` ``[B]`` int32: the experts pass over the tokens past it."""
-        a = self.args
+        a, bias = self.args, self.router_bias
+        if bias is not None and bias.dtype is not torch.float32:  # the module was cast
+            bias = bias.float()
         both = linear_act(x, self.router)
         indices, weights = route_experts(both[..., : self.E], a.num_experts_per_tok, scoring=a.scoring_func,
-                                         bias=self.router_bias, groups=a.n_group, top_groups=a.topk_group,
+                                         bias=bias, groups=a.n_group, top_groups=a.topk_group,
                                          renormalize=a.norm_topk_prob, scale=a.routed_scaling_factor, n_new=n_new)
         base = residual
         if self.shared_down_proj is not None:

@@ -277,7 +277,8 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, *, bias: Optional[torch.Te
     bias ``[rows of weight]``, row_gate ``[...]`` (one logit per row of x, such as
     a column of another product) in bf16, fp16 or fp32; residual ``[..., N]`` bf16.
     x and residual may be column slices of wider buffers.  ``out`` may be the
-    residual itself.  ``workspace``: bytes for the sums of K's slices, which some
+    residual itself, and otherwise lies apart from all that is read (other columns
+    of one buffer are refused too).  ``workspace``: bytes for the sums of K's slices, which some
     sizes are formed in (:func:`linear_act_workspace_bytes`; allocated when absent
     or too small); calls that overlap need one each.  There is no backward.
     """

@@ -321,6 +321,12 @@ def test_layers_take_a_sparse_mlp():
     m = experts.SparseMLP(_args())
     assert m.router.shape == (7, 64) and set(m.state_dict()) == {"router", "gate_up_proj", "down_proj",
                                                                  "shared_gate_up_proj", "shared_down_proj"}
+    m = experts.SparseMLP(_args(router_bias=True))
+    assert m.state_dict()["router_bias"].dtype is torch.float32
+    other = experts.SparseMLP(_args(router_bias=True))
+    other.load_state_dict(m.state_dict())
+    with pytest.raises(ValueError):  # it comes with one
+        m.load(*(torch.zeros(s) for s in ((6, 64), (6, 16, 64), (6, 16, 64), (6, 64, 16), (24, 64), (24, 64), (64, 24), (1, 64))))
     m = experts.SparseMLP(_args(shared_expert_intermediate_size=0))
     assert m.router.shape == (6, 64) and set(m.state_dict()) == {"router", "gate_up_proj", "down_proj"}
 

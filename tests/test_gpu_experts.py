@@ -341,6 +341,15 @@ def test_expert_mlp(N, H, I, E, k, base):
     assert torch.equal(y, mx.expert_mlp(*args[:5], base=args[5]))  # whatever order the pairs came in
 
 
+# rows of 128 and of 256 a tile; 157 MB of weights, which pass by the caches, in tiles of 64 and of 128
+@pytest.mark.parametrize("N,H,I,E,k", [(2048, 72, 1000, 8, 2), (4096, 72, 1000, 8, 2), (200, 512, 200, 256, 6),
+                                       (1400, 512, 200, 256, 6)])
+def test_expert_mlp_other_tiles(N, H, I, E, k):
+    args = _experts(_gen(N), N, H, I, E, k, True)
+    args[3][N - 5:] = -1
+    _check_experts(mx.expert_mlp(*args[:5], base=args[5]), *args)
+
+
 @pytest.mark.parametrize("N", [1, 4, 50, 700])
 def test_expert_mlp_choices(N):
     """Choices outside the experts add nothing, doubled ones add twice, tokens may have none."""
@@ -453,13 +462,13 @@ def _check_block(m, x, y, residual=None, n_new=None):
 
 
 @pytest.mark.parametrize("kw", [dict(), dict(shared_expert_intermediate_size=0, norm_topk_prob=False),
-                                dict(scoring_func="sigmoid", n_group=4, topk_group=2, routed_scaling_factor=2.5)])
+                                dict(scoring_func="sigmoid", n_group=4, topk_group=2, routed_scaling_factor=2.446, router_bias=True)])
 @pytest.mark.parametrize("B,T", [(1, 1), (3, 2), (2, 70)])
 def test_sparse_mlp(B, T, kw):
     torch.manual_seed(1)
     m = mx.SparseMLP(_args(**kw), DEV)
     if "n_group" in kw:
-        m.router_bias = torch.nn.Parameter(torch.randn(24, device=DEV) * 0.1, requires_grad=False)
+        m.router_bias.copy_(torch.randn(24, device=DEV) * 0.1)
     x, res = torch.randn(B, T, 256, device=DEV).bfloat16(), torch.randn(B, T, 256, device=DEV).bfloat16()
     kept = res.clone()
     _check_block(m, x, m(x))
@@ -502,6 +511,45 @@ def test_sparse_mlp_in_a_graph():
         got = y.clone()
         want = m(x)
         assert torch.equal(got, want)
+
+
+def test_expert_mlp_in_two_graphs():
+    """Graphs with workspaces of their own, captured and replayed in turn, and with eager calls between."""
+    args = _experts(_gen(12), 40, 264, 136, 12, 3, True)
+    few = _experts(_gen(13), 2, 264, 136, 12, 3, True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for a in (args, few):
+            mx.expert_mlp(*a[:5], base=a[5])
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs = [], []
+    for a in (args, few):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(mx.expert_mlp(*a[:5], base=a[5]))
+        graphs.append(g)
+    for i in range(3):
+        for a, g in zip((args, few), graphs):
+            a[0].copy_(torch.randn(a[0].shape, device=DEV))
+            a[3].copy_(torch.rand(a[0].shape[0], 12, device=DEV).argsort(-1)[:, :3])
+            g.replay()
+        torch.cuda.synchronize()
+        for a, o in zip((args, few), outs):
+            got = o.clone()
+            assert torch.equal(got, mx.expert_mlp(*a[:5], base=a[5]))
+
+
+def test_one_row_tensors():
+    """x of one dimension, as a row."""
+    g = _gen(14)
+    x, w = _r(g, 136), _r(g, 24, 136)
+    y = mx.linear_act(x, w)
+    assert y.shape == (24,) and torch.equal(y, mx.linear_act(x[None], w)[0])
+    i, wt = mx.route_experts(y, 2)
+    assert i.shape == (2,) and torch.equal(i, mx.route_experts(y[None], 2)[0][0])
+    a = _experts(g, 1, 136, 72, 6, 2)
+    assert torch.equal(mx.expert_mlp(a[0][0], *a[1:3], a[3][0], a[4][0]), mx.expert_mlp(*a[:5])[0])
 
 
 def test_calls_on_two_streams():
