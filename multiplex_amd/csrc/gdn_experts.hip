@@ -25,7 +25,9 @@ constexpr int kMaxChoices = 64;
 // before counts each chunk's pairs by expert, so that a workgroup knows what lies in front of its own.  Where a pair
 // lies among its expert's goes by the atomics' order, which no result depends on.
 constexpr int kPlanThreads = 1024;
-constexpr int kEach = 2, kChunk = kEach * kPlanThreads;  // pairs of a thread, of a workgroup
+// Pairs of a thread and of a workgroup: 2048 pairs a chunk, but up to 4096 in one (2331 pairs 2 + 5 us in two launches,
+// 5.5 in one).
+constexpr int kChunk = 2 * kPlanThreads, kOneChunk = 2 * kChunk;
 
 struct PlanParams {
   const int* indices;
@@ -38,23 +40,24 @@ struct PlanParams {
 };
 
 // The chunk's pairs by expert; each of the thread's pairs' expert (-1: none) and number among its chunk's.
-__device__ __forceinline__ void count_pairs(const PlanParams& p, int* hist, int (&expert)[kEach], int (&number)[kEach]) {
+template <int EACH>
+__device__ __forceinline__ void count_pairs(const PlanParams& p, int* hist, int (&expert)[EACH], int (&number)[EACH]) {
 #pragma unroll
-  for (int j = 0; j < kEach; ++j) {
-    const int i = blockIdx.x * kChunk + j * kPlanThreads + threadIdx.x;
+  for (int j = 0; j < EACH; ++j) {
+    const int i = blockIdx.x * (EACH * kPlanThreads) + j * kPlanThreads + threadIdx.x;
     const int e = i < p.P ? p.indices[i] : -1;
     expert[j] = e < p.E ? e : -1;
   }
   for (int e = threadIdx.x; e < p.E; e += kPlanThreads) hist[e] = 0;
   __syncthreads();
 #pragma unroll
-  for (int j = 0; j < kEach; ++j) number[j] = expert[j] >= 0 ? atomicAdd(&hist[expert[j]], 1) : 0;
+  for (int j = 0; j < EACH; ++j) number[j] = expert[j] >= 0 ? atomicAdd(&hist[expert[j]], 1) : 0;
   __syncthreads();
 }
 
 __global__ __launch_bounds__(kPlanThreads) void plan_count_kernel(const PlanParams p) {
   __shared__ int hist[kMaxExperts];
-  int expert[kEach], number[kEach];
+  int expert[kChunk / kPlanThreads], number[kChunk / kPlanThreads];
   count_pairs(p, hist, expert, number);
   for (int e = threadIdx.x; e < p.E; e += kPlanThreads) p.counts[blockIdx.x * p.E + e] = hist[e];
 }
@@ -81,12 +84,13 @@ __device__ __forceinline__ int block_before(int x, int* waves, int* all) {
   return before + s - x;
 }
 
+template <int EACH>
 __global__ __launch_bounds__(kPlanThreads) void plan_place_kernel(const PlanParams p) {
   __shared__ int hist[kMaxExperts];
   __shared__ int waves[kPlanThreads / 64];
   static_assert(kMaxExperts <= kPlanThreads, "a thread an expert");
   const int e = threadIdx.x;
-  int expert[kEach], number[kEach];
+  int expert[EACH], number[EACH];
   count_pairs(p, hist, expert, number);
   int mine = 0, total = 0;  // pairs of expert e in the chunks before, and in all
   if (e < p.E) {
@@ -110,9 +114,9 @@ __global__ __launch_bounds__(kPlanThreads) void plan_place_kernel(const PlanPara
   }
   __syncthreads();
 #pragma unroll
-  for (int j = 0; j < kEach; ++j) {
+  for (int j = 0; j < EACH; ++j) {
     if (expert[j] < 0) continue;
-    const int i = blockIdx.x * kChunk + j * kPlanThreads + threadIdx.x, at = hist[expert[j]] + number[j];
+    const int i = blockIdx.x * (EACH * kPlanThreads) + j * kPlanThreads + threadIdx.x, at = hist[expert[j]] + number[j];
     p.from[at] = i / p.k;
     p.to[at] = i;
   }
@@ -271,7 +275,7 @@ ExpertLayout expert_layout(int64_t N, int64_t H, int64_t I, int64_t E, int64_t k
   const int64_t P = N * k;
   l.rows = tile_rows(P, I, E);
   l.max_tiles = P / l.rows + (E < P ? E : P);
-  l.chunks = (P + kChunk - 1) / kChunk;
+  l.chunks = P <= kOneChunk ? 1 : (P + kChunk - 1) / kChunk;
   l.n_tiles = 0;
   l.tiles = 16;
   l.counts = l.tiles + l.max_tiles * sizeof(TileOf);
@@ -384,9 +388,16 @@ extern "C" int gdn_expert_mlp(const void* x, int64_t ldx, const void* gate_up, c
   plan.n_tiles = reinterpret_cast<int*>(ws + l.n_tiles);
   plan.from = reinterpret_cast<int*>(ws + l.from);
   plan.to = reinterpret_cast<int*>(ws + l.to);
-  const dim3 chunks(static_cast<unsigned>(l.chunks));
-  if (l.chunks > 1) hipLaunchKernelGGL(plan_count_kernel, chunks, dim3(kPlanThreads), 0, st, plan);
-  hipLaunchKernelGGL(plan_place_kernel, chunks, dim3(kPlanThreads), 0, st, plan);
+  const dim3 chunks(static_cast<unsigned>(l.chunks)), threads(kPlanThreads);
+  constexpr int kEach = kChunk / kPlanThreads;
+  if (l.chunks > 1) {
+    hipLaunchKernelGGL(plan_count_kernel, chunks, threads, 0, st, plan);
+    hipLaunchKernelGGL(plan_place_kernel<kEach>, chunks, threads, 0, st, plan);
+  } else if (plan.P > kChunk) {
+    hipLaunchKernelGGL(plan_place_kernel<kOneChunk / kPlanThreads>, chunks, threads, 0, st, plan);
+  } else {
+    hipLaunchKernelGGL(plan_place_kernel<kEach>, chunks, threads, 0, st, plan);
+  }
 
   const bool once = weights_once(N * k, H, I, E);
   ProductParams p = {};

@@ -22,12 +22,11 @@ import torch
 
 from . import _lib
 from .gated_delta import _dtype_code, _ptr, _require_device, _stream
-from .linear import _even_rows, _forward_only, _out_rows, linear_act
+from .linear import _FLOATS, _even_rows, _forward_only, _out_rows, linear_act
 
 __all__ = ["route_experts", "expert_mlp", "expert_mlp_workspace_bytes", "SparseMLP"]
 
 _SCORING = {"softmax": 0, "sigmoid": 1}
-_FLOATS = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
 
 
 def route_experts(logits: torch.Tensor, k: int, *, scoring: str = "softmax", bias: Optional[torch.Tensor] = None,
@@ -51,20 +50,24 @@ def route_experts(logits: torch.Tensor, k: int, *, scoring: str = "softmax", bia
     Computed in 64 bits, so that scores that differ at all are told apart.
     """
     # a plain call's checks in a few operations; what is wrong, or laid out otherwise, is looked into below
-    index = logits.get_device()
-    code = _FLOATS.get(logits.dtype)
-    if not (index >= 0 and code is not None and logits.dim() > 1 and k.__class__ is int and k > 0 and scoring in _SCORING
-            and not (torch.is_grad_enabled() and (logits.requires_grad or bias is not None and bias.requires_grad))
-            and logits.is_contiguous() and n_new is None
-            and (bias is None or bias.dtype is torch.float32 and bias.get_device() == index and bias.is_contiguous()
-                 and bias.shape == logits.shape[-1:])):
+    index, code, d = logits.get_device(), _FLOATS.get(logits.dtype), logits.dim()
+    ld = _even_rows(logits) if d > 1 else None
+    if (index < 0 or code is None or ld is None or k.__class__ is not int or k <= 0 or scoring not in _SCORING
+            or torch.is_grad_enabled() and (logits.requires_grad or bias is not None and bias.requires_grad)
+            or n_new is not None and not (d == 3 and n_new.dtype is torch.int32 and n_new.get_device() == index
+                                          and n_new.shape == logits.shape[:1] and n_new.is_contiguous())
+            or bias is not None and not (bias.dtype is torch.float32 and bias.get_device() == index
+                                         and bias.is_contiguous() and bias.shape == logits.shape[-1:])):
         return _route_general(logits, k, scoring, bias, groups, top_groups, group_best, renormalize, scale, n_new)
-    dev, E = logits.device, logits.shape[-1]
-    shape = (*logits.shape[:-1], k)
-    indices = torch.empty(shape, dtype=torch.int32, device=dev)
-    weights = torch.empty(shape, dtype=torch.float32, device=dev)
-    _lib.call(dev, "gdn_route_experts", logits.data_ptr(), code, E, None if bias is None else bias.data_ptr(), None,
-              indices.data_ptr(), weights.data_ptr(), indices.numel() // k, 1, E, k, _SCORING[scoring], int(groups),
+    dev, *lead = logits.device, *logits.shape
+    E = lead[-1]
+    lead[-1] = k
+    indices = torch.empty(lead, dtype=torch.int32, device=dev)
+    weights = torch.empty(lead, dtype=torch.float32, device=dev)
+    T = lead[1] if n_new is not None else 1
+    _lib.call(dev, "gdn_route_experts", logits.data_ptr(), code, ld, None if bias is None else bias.data_ptr(),
+              None if n_new is None else n_new.data_ptr(), indices.data_ptr(), weights.data_ptr(),
+              lead[0] if n_new is not None else indices.numel() // k, T, E, k, _SCORING[scoring], int(groups),
               int(top_groups), int(group_best), 1 if renormalize else 0, float(scale), _stream(dev))
     return indices, weights
 

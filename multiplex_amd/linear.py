@@ -208,15 +208,20 @@ def gated_norm_linear_decode(y: torch.Tensor, z: torch.Tensor, norm_weight: Opti
 
 # -------------------------------------------------- products with an epilogue
 
+_FLOATS = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
 _ACTS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4, "swiglu": 5}
 
 
 def _even_rows(t: torch.Tensor) -> Optional[int]:
     """Elements from a row of ``[..., D]`` to the next where the rows are contiguous
     and evenly spaced (a column slice of a wider buffer), else None."""
-    if t.is_contiguous():
-        return t.shape[-1]
     D = t.shape[-1]
+    if t.is_contiguous():
+        return D
+    if t.dim() == 3:  # the usual column slice of [B, T, width]
+        (_, T, _), (b, ld, one) = t.shape, t.stride()
+        if one == 1 and T > 1 and b == T * ld and ld >= D:
+            return ld
     if t.stride(-1) != 1 and D != 1:
         return None
     ld, rows = 0, 1
@@ -285,21 +290,34 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, *, bias: Optional[torch.Te
     # a plain call's checks in a few operations; what is wrong, or laid out otherwise, is looked into below
     index, bf16, act = x.get_device(), torch.bfloat16, _ACTS.get(activation)
     if (index >= 0 and act is not None and x.dtype is bf16 and weight.dtype is bf16 and weight.dim() == 2 and x.dim() > 0
-            and bias is None and row_gate is None and out is None and workspace is None and weight.get_device() == index
+            and out is None and workspace is None and weight.get_device() == index
             and x.is_contiguous() and weight.is_contiguous()
             and not (torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
+                                                  or bias is not None and bias.requires_grad
+                                                  or row_gate is not None and row_gate.requires_grad
                                                   or residual is not None and residual.requires_grad))):
         rows, K = weight.shape
         N = rows // 2 if act == 5 else rows
-        shape, xp, wp = x.shape[:-1] + (N,), x.data_ptr(), weight.data_ptr()
+        lead, xp, wp = x.shape[:-1], x.data_ptr(), weight.data_ptr()
+        shape = lead + (N,)
+        bias_dt = gate_dt = 0
+        if bias is not None:
+            bias_dt = _FLOATS.get(bias.dtype, -1) if (bias.shape == (rows,) and bias.get_device() == index
+                                                      and bias.is_contiguous()) else -1
+        if row_gate is not None:  # (of one dimension: any stride; otherwise contiguous)
+            gate_dt = _FLOATS.get(row_gate.dtype, -1) if (row_gate.shape == lead and row_gate.get_device() == index and
+                                                          (len(lead) == 1 or row_gate.is_contiguous())) else -1
         if (x.shape[-1] == K and K > 0 and K % 8 == 0 and N > 0 and (act != 5 or rows % 2 == 0) and (xp | wp) % 16 == 0
+                and bias_dt >= 0 and gate_dt >= 0
                 and (residual is None or residual.dtype is bf16 and residual.get_device() == index
                      and residual.shape == shape and residual.is_contiguous())):
             dev, M = x.device, x.numel() // K
             out = torch.empty(shape, dtype=bf16, device=dev)
             need = linear_act_workspace_bytes(M, N, K, activation)
             ws = torch.empty(need, dtype=torch.uint8, device=dev).data_ptr() if need else None
-            _lib.call(dev, "gdn_linear_act", xp, K, wp, None, 0, act, None, 0, 0,
+            _lib.call(dev, "gdn_linear_act", xp, K, wp, None if bias is None else bias.data_ptr(), bias_dt, act,
+                      None if row_gate is None else row_gate.data_ptr(), gate_dt,
+                      0 if row_gate is None else row_gate.stride(0) if len(lead) == 1 else 1,
                       None if residual is None else residual.data_ptr(), N, out.data_ptr(), N, M, N, K, ws, need,
                       _stream(dev))
             return out
