@@ -121,7 +121,7 @@ Tiling tiling(int64_t M, int64_t N, int64_t K, bool pair) {
   for (const Tiling& t : kTilings) {
     for (int slices = 1; slices <= 8; slices *= 2) {
       const int64_t steps = ((K + 64 * t.groups - 1) / (64 * t.groups) + slices - 1) / slices;
-      if (slices > 1 && (t.groups > 1 || steps < 8 || M * weight_rows > (int64_t{1} << 28))) break;
+      if (slices > 1 && (steps * t.groups < 8 || M * weight_rows > (int64_t{1} << 28))) break;
       const int64_t tiles = ((M + t.rows - 1) / t.rows) * ((weight_rows + t.weight_rows - 1) / t.weight_rows) * slices;
       const int64_t whole = (tiles + kCUs - 1) / kCUs;
       const float rounds = whole > 3 ? static_cast<float>(tiles) / kCUs : static_cast<float>(whole);
@@ -169,9 +169,11 @@ void launch_tiles(const ProductParams& p, const Tiling& t, bool bare, hipStream_
     else if (bare) launch_product<Wide<PAIR>, kBare, false>(p, m_tiles, st);
     else launch_product<Wide<PAIR>, kFinish, false>(p, m_tiles, st);
   } else if (t.groups == 2) {
-    launch_product<Deep<PAIR>, kFinish, false>(p, m_tiles, st);
+    if (t.slices > 1) launch_slices<Deep<PAIR>, PAIR>(p, m_tiles, st);
+    else launch_product<Deep<PAIR>, kFinish, false>(p, m_tiles, st);
   } else {
-    launch_product<Thin<PAIR>, kFinish, false>(p, m_tiles, st);
+    if (t.slices > 1) launch_slices<Thin<PAIR>, PAIR>(p, m_tiles, st);
+    else launch_product<Thin<PAIR>, kFinish, false>(p, m_tiles, st);
   }
 }
 

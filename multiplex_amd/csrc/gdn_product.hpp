@@ -72,61 +72,100 @@ __device__ __forceinline__ float activate(int act, float x) {
   }
 }
 
-// Eight neighbouring columns' sums (of SwiGLU's gates, and its ups) through the epilogue: row `at` of out, columns c on.
-template <bool PAIR>
-__device__ __forceinline__ void finish8(const ProductParams& p, float (&v)[CPL], const float (&up)[CPL], int64_t at, int c) {
-  const Epilogue& e = p.epi;
-  if (e.bias) {
+// Eight neighbouring bf16 values of which `n` are there, by the widest pieces that their place allows.
+__device__ __forceinline__ u32x4 load_bf16x8(const uint16_t* p, int n) {
+  if (n >= CPL && reinterpret_cast<uintptr_t>(p) % 16 == 0) return *reinterpret_cast<const u32x4*>(p);
+  u32x4 v = {0u, 0u, 0u, 0u};
+  if (n >= CPL && reinterpret_cast<uintptr_t>(p) % 4 == 0) {
 #pragma unroll
-    for (int j = 0; j < CPL; ++j) v[j] += load_any(e.bias, e.bias_dt, min(c + j, p.N - 1));
-  }
-  if constexpr (PAIR) {
-    if (e.bias) {
-#pragma unroll
-      for (int j = 0; j < CPL; ++j) v[j] = silu(v[j]) * (up[j] + load_any(e.bias, e.bias_dt, min(c + j, p.N - 1) + p.up));
-    } else {
-#pragma unroll
-      for (int j = 0; j < CPL; ++j) v[j] = silu(v[j]) * up[j];
-    }
-  } else {
-    if (e.act != GDN_ACT_NONE) {
-#pragma unroll 1
-      for (int j = 0; j < CPL; ++j) {  // the values pass by one copy of the code
-        float x = v[0];
-        x = activate(e.act, x);
-#pragma unroll
-        for (int m = 1; m < CPL; ++m) v[m - 1] = v[m];
-        v[CPL - 1] = x;
-      }
-    }
-  }
-  if (e.gate) {
-    const float g = sigmoid(load_any(e.gate, e.gate_dt, at * e.gate_ld));
-#pragma unroll
-    for (int j = 0; j < CPL; ++j) v[j] *= g;
-  }
-  const bool all = c + CPL <= p.N;
-  if (e.residual) {
-    const uint16_t* r = e.residual + at * e.ldr + c;
-    if (all && reinterpret_cast<uintptr_t>(r) % 16 == 0) {
-      float x[CPL];
-      unpack8<GDN_DTYPE_BF16>(load_raw8<GDN_DTYPE_BF16>(r, 0), x);
-#pragma unroll
-      for (int j = 0; j < CPL; ++j) v[j] += x[j];
-    } else {
-#pragma unroll
-      for (int j = 0; j < CPL; ++j)
-        if (c + j < p.N) v[j] += bf16_to_f32(r[j]);
-    }
-  }
-  uint16_t* o = p.out + at * p.ldo + c;
-  if (all && reinterpret_cast<uintptr_t>(o) % 16 == 0) {
-    store8<GDN_DTYPE_BF16>(o, 0, v);
+    for (int j = 0; j < 4; ++j) v[j] = reinterpret_cast<const uint32_t*>(p)[j];
   } else {
 #pragma unroll
     for (int j = 0; j < CPL; ++j)
-      if (c + j < p.N) o[j] = f32_to_bf16(v[j]);
+      if (j < n) v[j / 2] |= static_cast<uint32_t>(p[j]) << (16 * (j % 2));
   }
+  return v;
+}
+__device__ __forceinline__ void store_bf16x8(uint16_t* p, int n, const u32x4& v) {
+  if (n >= CPL && reinterpret_cast<uintptr_t>(p) % 16 == 0) {
+    *reinterpret_cast<u32x4*>(p) = v;
+  } else if (n >= CPL && reinterpret_cast<uintptr_t>(p) % 4 == 0) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) reinterpret_cast<uint32_t*>(p)[j] = v[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < CPL; ++j)
+      if (j < n) p[j] = static_cast<uint16_t>(v[j / 2] >> (16 * (j % 2)));
+  }
+}
+
+__device__ __forceinline__ void load_bias8(const Epilogue& e, int c, int n, float (&b)[CPL]) {
+  if (e.bias_dt == GDN_DTYPE_F32) {
+#pragma unroll
+    for (int j = 0; j < CPL; ++j) b[j] = j < n ? static_cast<const float*>(e.bias)[c + j] : 0.0f;
+  } else {
+    const u32x4 v = load_bf16x8(static_cast<const uint16_t*>(e.bias) + c, n);
+#pragma unroll
+    for (int j = 0; j < CPL; ++j) {
+      const uint16_t h = static_cast<uint16_t>(v[j / 2] >> (16 * (j % 2)));
+      b[j] = e.bias_dt == GDN_DTYPE_BF16 ? bf16_to_f32(h) : f16_to_f32(h);
+    }
+  }
+}
+
+// Eight neighbouring columns' sums (of SwiGLU's gates, and its ups) through the epilogue: row `at` of out, columns c on.
+template <bool PAIR>
+__device__ __forceinline__ void finish8(const ProductParams& p, float (&v)[CPL], float (&up)[CPL], int64_t at, int c) {
+  const Epilogue& e = p.epi;
+  const int n = p.N - c;  // columns that are there
+  // what is read is on its way before the activation
+  u32x4 residual = {0u, 0u, 0u, 0u};
+  if (e.residual) residual = load_bf16x8(e.residual + at * e.ldr + c, n);
+  const float gate = e.gate ? load_any(e.gate, e.gate_dt, at * e.gate_ld) : 0.0f;
+  if (e.bias) {
+    float b[CPL];
+    load_bias8(e, c, n, b);
+#pragma unroll
+    for (int j = 0; j < CPL; ++j) v[j] += b[j];
+    if (PAIR) {
+      load_bias8(e, c + p.up, n, b);
+#pragma unroll
+      for (int j = 0; j < CPL; ++j) up[j] += b[j];
+    }
+  }
+  if constexpr (PAIR) {
+#pragma unroll
+    for (int j = 0; j < CPL; ++j) v[j] = silu(v[j]) * up[j];
+  } else if (e.act == GDN_ACT_GELU) {  // (the others are short: all eight at a time)
+#pragma unroll 1
+    for (int j = 0; j < CPL; ++j) {  // the values pass by one copy of the code
+      const float x = activate(GDN_ACT_GELU, v[0]);
+#pragma unroll
+      for (int m = 1; m < CPL; ++m) v[m - 1] = v[m];
+      v[CPL - 1] = x;
+    }
+  } else if (e.act == GDN_ACT_RELU) {
+#pragma unroll
+    for (int j = 0; j < CPL; ++j) v[j] = activate(GDN_ACT_RELU, v[j]);
+  } else if (e.act == GDN_ACT_SILU) {
+#pragma unroll
+    for (int j = 0; j < CPL; ++j) v[j] = activate(GDN_ACT_SILU, v[j]);
+  } else if (e.act == GDN_ACT_GELU_TANH) {
+#pragma unroll
+    for (int j = 0; j < CPL; ++j) v[j] = activate(GDN_ACT_GELU_TANH, v[j]);
+  }
+  if (e.gate) {
+    const float g = sigmoid(gate);
+#pragma unroll
+    for (int j = 0; j < CPL; ++j) v[j] *= g;
+  }
+  if (e.residual) {
+#pragma unroll
+    for (int j = 0; j < CPL; ++j)
+      v[j] += __uint_as_float(j % 2 ? residual[j / 2] & 0xffff0000u : residual[j / 2] << 16);
+  }
+  store_bf16x8(p.out + at * p.ldo + c, n,
+               u32x4{pk_bf16(v[0], v[1]), pk_bf16(v[2], v[3]), pk_bf16(v[4], v[5]), pk_bf16(v[6], v[7])});
 }
 
 // ------------------------------------------------- four sums in eight bytes
@@ -254,7 +293,7 @@ __device__ __forceinline__ void product_store(const ProductParams& p, f32x4 (&ac
   const int wk = wave / NG, wg = wave % NG, wm = wg % WM, wn = wg / WM;
   const int lr = lane & 15, lq = lane >> 4;
 
-  if constexpr (ST == kFinish) {
+  if constexpr (ST == kFinish || (ST == kPart && WK > 1)) {
     constexpr int PITCH = S::WR + 4;  // floats a row
     constexpr int FIT = S::LDS / (WK * 16 * WM * PITCH * 4);  // blocks of rows a wave that there is room for
     constexpr int PB = FIT >= MB ? MB : FIT >= 4 ? 4 : FIT >= 2 ? 2 : 1;
@@ -290,11 +329,21 @@ __device__ __forceinline__ void product_store(const ProductParams& p, f32x4 (&ac
             if (S::PAIR) up[j] += from[g * PASS * PITCH + 8 * NB + j];
           }
         }
-        finish8<S::PAIR>(p, v, up, p.to ? p.to[row0 + row] : row0 + row, c);
+        if constexpr (ST == kPart) {  // (the pitch's halves hold whole fours)
+          float* part = p.part + static_cast<int64_t>(row0 + row) * p.pitch + c;
+          const bool both = c + 4 < p.N;
+          *reinterpret_cast<f32x4*>(part) = f32x4{v[0], v[1], v[2], v[3]};
+          if (both) *reinterpret_cast<f32x4*>(part + 4) = f32x4{v[4], v[5], v[6], v[7]};
+          if (S::PAIR) {
+            *reinterpret_cast<f32x4*>(part + p.pitch / 2) = f32x4{up[0], up[1], up[2], up[3]};
+            if (both) *reinterpret_cast<f32x4*>(part + p.pitch / 2 + 4) = f32x4{up[4], up[5], up[6], up[7]};
+          }
+        } else {
+          finish8<S::PAIR>(p, v, up, p.to ? p.to[row0 + row] : row0 + row, c);
+        }
       }
     }
   } else if constexpr (ST == kPart) {
-    static_assert(WK == 1, "groups sum up in LDS");
 #pragma unroll
     for (int i = 0; i < MB; ++i) {
       const int r = 16 * (i * WM + wm) + lr;
