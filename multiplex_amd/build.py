@@ -15,18 +15,18 @@ from pathlib import Path
 PKG_DIR = Path(__file__).resolve().parent
 CSRC = PKG_DIR / "csrc"
 LIB_PATH = PKG_DIR / "libgdn.so"
-SOURCES = [
-    "gdn_api.hip",
+SOURCES = [  # those that take longest first
+    "gdn_linear_act.hip",
+    "gdn_experts.hip",
+    "gdn_chunk.hip",
     "gdn_recurrent.hip",
     "gdn_prologue.hip",
-    "gdn_chunk.hip",
-    "gdn_epilogue.hip",
-    "gdn_attention.hip",
     "gdn_paged.hip",
+    "gdn_attention.hip",
     "gdn_linear.hip",
+    "gdn_epilogue.hip",
     "gdn_route.hip",
-    "gdn_experts.hip",
-    "gdn_linear_act.hip",
+    "gdn_api.hip",
 ]
 ARCH = "gfx950"
 
