@@ -40,7 +40,7 @@ struct ProductParams {
   int up;                  // SwiGLU: weight rows from a column's gate to its up (0: one row a column)
   uint16_t* out;
   int64_t ldo;
-  int M, N, K;             // rows (no plan), columns of out
+  int M, N, K;             // rows (without a plan), columns of out
   int n_tiles;             // tiles of columns
   // K in slices of `slice` values: slice i's sums go to part + i M pitch, a row's columns (its ups from pitch / 2 on)
   int slices, slice, pitch;
@@ -172,8 +172,8 @@ __device__ __forceinline__ void finish8(const ProductParams& p, float (&v)[CPL],
 //
 // An expert's results wait in memory for the sum over a token's experts.  Rounded to bf16 they would be off by as much
 // as the output's own rounding is.  In the same bytes, four neighbouring columns share an exponent: 8 bits, and 14 for
-// each column's signed multiple of 2^(exponent - 12), off by at most 2^-12 of the largest of the four (16 times less than bf16
-// at its own).  8191, -8191 and -8192 stand for +inf, -inf and NaN.
+// each column's signed multiple of 2^(exponent - 12), off by at most 2^-12 of the largest of the four (16 times less than
+// bf16 at its own).  8191, -8191 and -8192 stand for +inf, -inf and NaN.
 constexpr int kInf14 = 8191, kNan14 = -8192, kMost14 = 8190;
 
 __device__ __forceinline__ u32x2 pack4(const f32x4& v) {
@@ -280,9 +280,10 @@ enum Store {
 };
 
 // The epilogue of a tile's sums: lane (lr, lq) holds columns 4 lq + 0..3 of its 16-column blocks of row lr of its 16-row
-// blocks.  Where nothing but SwiGLU is to be done, straight from the registers.  The rest goes through LDS, as many
-// rows at a time as there is room for, eight neighbouring columns a thread, so that its code stands there once and not for each of a lane's
-// up to 128 sums: those had the experts' second product (4096 tokens, 2048 x 512, 8 of 256) wait 80 us for instructions.
+// blocks.  Where nothing but SwiGLU is to be done, straight from the registers.  The rest goes through LDS, as many rows at
+// a time as there is room for, eight neighbouring columns a thread, so that its code stands there once and not for each
+// of a lane's up to 128 sums (the experts' second product of 4096 tokens, 2048 x 512, 8 of 256, 246 us with all of it in
+// the unrolled stores, 176 as here).
 template <class S, int MB, Store ST>
 __device__ __forceinline__ void product_store(const ProductParams& p, f32x4 (&acc)[MB][S::NB], int n0, int row0, int rows,
                                               unsigned char* smem) {

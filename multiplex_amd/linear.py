@@ -312,7 +312,7 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, *, bias: Optional[torch.Te
                 and (residual is None or residual.dtype is bf16 and residual.get_device() == index
                      and residual.shape == shape and residual.is_contiguous())):
             dev, M = x.device, x.numel() // K
-            out = torch.empty(shape, dtype=bf16, device=dev)
+            out = x.new_empty(shape)
             need = linear_act_workspace_bytes(M, N, K, activation)
             ws = torch.empty(need, dtype=torch.uint8, device=dev).data_ptr() if need else None
             _lib.call(dev, "gdn_linear_act", xp, K, wp, None if bias is None else bias.data_ptr(), bias_dt, act,

@@ -540,6 +540,21 @@ def test_expert_mlp_in_two_graphs():
             assert torch.equal(got, mx.expert_mlp(*a[:5], base=a[5]))
 
 
+def test_gradients_are_refused():
+    """On the calls' short way too; without recording they run."""
+    g = _gen(15)
+    x, w = _r(g, 4, 136), _r(g, 24, 136)
+    a = _experts(g, 4, 136, 72, 6, 2)
+    logits = _r(g, 4, 16, dtype=torch.float32)
+    calls = [lambda: mx.linear_act(x.requires_grad_(), w), lambda: mx.route_experts(logits.requires_grad_(), 2),
+             lambda: mx.expert_mlp(*a[:4], a[4].requires_grad_())]
+    for call in calls:
+        with pytest.raises(ValueError, match="gradient"):
+            call()
+        with torch.no_grad():
+            call()
+
+
 def test_one_row_tensors():
     """x of one dimension, as a row."""
     g = _gen(14)
