@@ -92,43 +92,50 @@ __global__ __launch_bounds__(256) void finish_kernel(const ProductParams p) {
 
 // The tile and slices of K of the least modelled time: rounds of tiles over the CUs times a tile's fixed part and its
 // steps' (of 64 values of K, shared by the groups of waves), which grow with the rows it works on, the slices' sums
-// written and read, and below all the operands' bytes at the rate that the tile reaches.  Fitted to graph-replayed times
-// of 165 sizes (11 products from 512 to 12288 in and 1000 to 24576 weight rows, 5 to 4096 rows), each in all four tiles;
-// without slices the choice is the slower one by 0.5% on average, by 16% at most (5 to 16 rows of 4096 x 24576: 47 us in
-// the second, 41 in the first).  E.g. 128 rows of 4096 x 4096, us: 16.4, 30, 56, 56; 512 of 12288 x 4096: 142, 83, 154,
-// 260; 4096 of 4096 x 24576: 2620, 1285, 700, 619.  Slices of K pay where a few tiles have many steps: 512 of 12288 x
-// 4096 in 4 slices 62, 128 of them in 8 41, 1024 of 4096 x 4096 in 2 46 (53 whole).
+// written and read, and below all the operands' bytes at the rate that the tile reaches.  Where K is no multiple of 64,
+// rows start inside cache lines and a step's loads take two lines a row.  Fitted to graph-replayed times of 140 sizes (16
+// products from 512 to 12288 in and 700 to 24576 weight rows, seven of them with such K; 8 to 4096 rows) in up to 12
+// ways each; the choice is 2.8% slower than the best of them on average, at most 59% (8 x 3320 x 9244: 31 us in the second
+// tile, 20 in the first).  E.g. 128 rows of 4096 x 4096, us in the four tiles: 16.4, 30, 56, 56; 512 of 12288 x 4096: 142,
+// 83, 154, 260; 4096 of 4096 x 24576: 2620, 1285, 700, 619.  Slices of K pay where a few tiles have many steps: 512 of
+// 12288 x 4096 in 4 slices 62, 128 of them in 8 41, 1024 of 4096 x 4096 in 2 46 (53 whole).
 struct Tiling {
   int rows, weight_rows, groups, block;  // block: rows that a step's work grows by
   float tile_us, step_us, rows_us;       // a tile's ends, a step, and a step of all rows on top
   float mb_us;                           // MB a us
+  float across_step, across_mb;          // what step_us and mb_us are times where rows start inside lines
   int slices;
 };
 constexpr Tiling kTilings[4] = {
-    {64, 32, 4, 16, 3.7f, 0.0f, 0.63f, 3.5f, 1},
-    {64, 128, 2, 16, 3.9f, 0.40f, 0.31f, 4.2f, 1},
-    {128, 256, 1, 32, 4.0f, 0.40f, 0.40f, 3.1f, 1},
-    {256, 256, 1, 32, 4.0f, 0.36f, 1.02f, 3.2f, 1},
+    {64, 32, 4, 16, 1.6f, 0.28f, 0.40f, 3.5f, 1.48f, 0.71f, 1},
+    {64, 128, 2, 16, 2.2f, 0.52f, 0.24f, 4.1f, 1.50f, 0.72f, 1},
+    {128, 256, 1, 32, 2.9f, 0.46f, 0.38f, 4.0f, 1.67f, 0.73f, 1},
+    {256, 256, 1, 32, 3.2f, 0.40f, 1.04f, 4.0f, 1.82f, 0.74f, 1},
 };
-constexpr float kFinishUs = 4.0f, kPartMbUs = 4.0f;  // the slices' launch, and MB of their sums a us
+constexpr float kFinishUs = 5.5f, kPartMbUs = 6.1f;  // the slices' launch, and MB of their sums a us
 
 Tiling tiling(int64_t M, int64_t N, int64_t K, bool pair) {
   const int64_t weight_rows = pair ? 2 * N : N;
   const float mb = 2e-6f * (static_cast<float>(M) * K + static_cast<float>(weight_rows) * K + static_cast<float>(M) * N);
+  const bool across = K % 64 != 0;
   Tiling best = kTilings[0];
   float least = 0.0f;
   bool any = false;
   for (const Tiling& t : kTilings) {
+    const float step_us = t.step_us * (across ? t.across_step : 1.0f), mb_us = t.mb_us * (across ? t.across_mb : 1.0f);
     for (int slices = 1; slices <= 8; slices *= 2) {
       const int64_t steps = ((K + 64 * t.groups - 1) / (64 * t.groups) + slices - 1) / slices;
-      if (slices > 1 && (steps * t.groups < 8 || M * weight_rows > (int64_t{1} << 28))) break;
+      // (as few steps, and as many slices of the tiles whose groups share K, as were measured)
+      if (slices > 1 && (steps * t.groups < 16 || slices > (t.groups > 1 ? 4 : 8) ||
+                         M * weight_rows > (int64_t{1} << 28)))
+        break;
       const int64_t tiles = ((M + t.rows - 1) / t.rows) * ((weight_rows + t.weight_rows - 1) / t.weight_rows) * slices;
       const int64_t whole = (tiles + kCUs - 1) / kCUs;
       const float rounds = whole > 3 ? static_cast<float>(tiles) / kCUs : static_cast<float>(whole);
       int64_t rows = t.block;
       while (rows < t.rows && rows < M) rows *= 2;
-      float us = rounds * (t.tile_us + steps * (t.step_us + t.rows_us * static_cast<float>(rows) / t.rows));
-      us = us > mb / t.mb_us ? us : mb / t.mb_us;
+      float us = rounds * (t.tile_us + steps * (step_us + t.rows_us * static_cast<float>(rows) / t.rows));
+      us = us > mb / mb_us ? us : mb / mb_us;
       if (slices > 1) us += kFinishUs + 8e-6f * slices * M * weight_rows / kPartMbUs;
       if (any && us >= least) continue;
       any = true;
