@@ -1,8 +1,8 @@
 """Float64 CPU restatement of the sparse MLP's operators: routing to experts, the
 experts' products, and dense products with an epilogue.
 
-TEST INFRASTRUCTURE ONLY.  Only ``tests/`` may import this module, and only as the
-checker.  The product package ``multiplex_amd`` never imports it.
+TEST INFRASTRUCTURE ONLY.  Only ``tests/`` may import this module.  The product
+package ``multiplex_amd`` never imports it.
 
 What it restates: mlx-lm's sparse block of the ``qwen3_5`` layers (softmax over all
 experts, top-k, renormalised weights, SwiGLU experts, a shared expert times the
