@@ -314,12 +314,13 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, *, bias: Optional[torch.Te
             dev, M = x.device, x.numel() // K
             out = x.new_empty(shape)
             need = linear_act_workspace_bytes(M, N, K, activation)
-            ws = torch.empty(need, dtype=torch.uint8, device=dev).data_ptr() if need else None
+            # (bound until the call returns: its memory may be another thread's as soon as the tensor is gone)
+            ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
             _lib.call(dev, "gdn_linear_act", xp, K, wp, None if bias is None else bias.data_ptr(), bias_dt, act,
                       None if row_gate is None else row_gate.data_ptr(), gate_dt,
                       0 if row_gate is None else row_gate.stride(0) if len(lead) == 1 else 1,
-                      None if residual is None else residual.data_ptr(), N, out.data_ptr(), N, M, N, K, ws, need,
-                      _stream(dev))
+                      None if residual is None else residual.data_ptr(), N, out.data_ptr(), N, M, N, K,
+                      None if ws is None else ws.data_ptr(), need, _stream(dev))
             return out
     return _linear_act_general(x, weight, bias, activation, row_gate, residual, out, workspace)
 

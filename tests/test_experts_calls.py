@@ -1,0 +1,65 @@
+"""What the sparse MLP's Python calls hand to the library, without a GPU: the calls' short
+ways run on CPU tensors that claim a device, and the launch is a stand-in."""
+
+from __future__ import annotations
+
+import weakref
+
+import pytest
+import torch
+
+from multiplex_amd import _lib, attention, experts, linear
+
+
+class OnDevice(torch.Tensor):
+    """A host tensor that the calls' short ways take for one of device 0."""
+
+    def get_device(self):
+        return 0
+
+
+def _b(*shape, dtype=torch.bfloat16):
+    return torch.zeros(*shape, dtype=dtype).as_subclass(OnDevice)
+
+
+def _i(*shape):
+    return _b(*shape, dtype=torch.int32)
+
+
+def _f(*shape):
+    return _b(*shape, dtype=torch.float32)
+
+
+@pytest.fixture
+def made(monkeypatch):
+    """(name, arguments) of the launches."""
+    calls = []
+    for mod in (experts, linear):
+        monkeypatch.setattr(mod, "_stream", lambda dev: 0)
+        monkeypatch.setattr(mod, "_require_device", lambda tensors, names: torch.device("cpu"))
+    monkeypatch.setattr(_lib, "call", lambda dev, name, *args: calls.append((name, args)))
+    return calls
+
+
+def test_a_workspace_lives_until_its_launch(made, monkeypatch):
+    """(Another thread may be given its memory otherwise: the library's call lets go of the interpreter.)"""
+    x, w = _b(14, 12144), _b(494, 12144)
+    assert linear.linear_act_workspace_bytes(14, 494, 12144) > 0
+    made_here, alive = [], []
+    empty = torch.empty
+
+    def recorded(*args, **kw):
+        t = empty(*args, **kw)
+        made_here.append(weakref.ref(t))
+        return t
+
+    def launched(dev, name, *args):
+        alive.extend(r() is not None and r().data_ptr() in args for r in made_here)
+
+    monkeypatch.setattr(torch, "empty", recorded)
+    monkeypatch.setattr(_lib, "call", launched)
+    linear.linear_act(x, w)
+    assert alive == [True]
+    made_here.clear(), alive.clear()
+    experts.expert_mlp(_b(4, 16), _b(3, 16, 16), _b(3, 16, 8), _i(4, 2), _f(4, 2))
+    assert alive == [True]
