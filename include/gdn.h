@@ -529,7 +529,9 @@ size_t gdn_expert_mlp_workspace_bytes(int64_t N, int64_t H, int64_t I, int64_t E
  *   gate_up [E, 2I, H] (G_e's rows, then U_e's), down [E, H, I], contiguous
  *   indices, weights [N, k]; a choice outside [0, E) adds nothing, one that
  *   stands twice is added twice
- * silu(..) * .. and an expert's result are rounded to bf16, the sum of the k once.
+ * silu(..) * .. is rounded to bf16 (an operand of the second product); an expert's
+ * result is off by at most 2^-12 of itself (rounded to 12 bits of significand, or,
+ * for few pairs, not at all); the sum of the k is formed in fp32 and rounded once.
  * out may alias base.  Calls that overlap need a workspace each.
  * H and I multiples of 8, strides too; pointers 16-byte aligned; x spans less
  * than 2 GiB, an expert's gate_up too.

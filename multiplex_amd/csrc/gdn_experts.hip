@@ -7,8 +7,9 @@
 // rows, and one launch runs all tiles of all experts: a workgroup finds its expert, rows and columns in the plan.  The
 // launch has as many workgroups as the pairs can need at most; those past the plan's end leave.
 // SwiGLU happens in the first product's epilogue (a wave forms a column of the gate and the same column of up), its
-// result is rounded to bf16 as the second product's operand; the k results of a token wait in packed fours and are summed
-// in fp32 in the order of its choices: a result does not depend on where a pair came to lie in the plan.
+// result is rounded to bf16 as the second product's operand: the matrix units multiply bf16, and a second product of what
+// the rounding leaves would double theirs.  The k results of a token wait in 20 bits a column and are summed in fp32 in the
+// order of its choices: a result does not depend on where a pair came to lie in the plan.
 #include <cmath>
 
 #include "gdn_dot.hpp"
@@ -125,7 +126,8 @@ __global__ __launch_bounds__(kPlanThreads) void plan_place_kernel(const PlanPara
 // ------------------------------------------------------------------- combine
 
 struct CombineParams {
-  const uint16_t* y;  // [N k][H], packed fours
+  const uint16_t* y;        // [N k][H], the sums' upper halves
+  const uint32_t* nibbles;  // [N k][H / 8], their next four bits
   const int* indices;
   const float* weights;
   const uint16_t* base;
@@ -147,6 +149,7 @@ __global__ __launch_bounds__(256) void combine_kernel(const CombineParams p) {
   if (p.base) unpack8<GDN_DTYPE_BF16>(load_raw8<GDN_DTYPE_BF16>(p.base, t * p.ldb + c), sum);
   for (int j0 = 0; j0 < p.k; j0 += 4) {  // four rows on their way at a time (those of no expert hold anything)
     u32x4 q[4];
+    uint32_t q4[4];
     float w[4];
     bool in[4];
 #pragma unroll
@@ -156,11 +159,12 @@ __global__ __launch_bounds__(256) void combine_kernel(const CombineParams p) {
       in[m] = j0 + m < p.k && e >= 0 && e < p.E;
       w[m] = p.weights[j];
       q[m] = *reinterpret_cast<const u32x4*>(p.y + j * p.H + c);
+      q4[m] = p.nibbles[(j * p.H + c) / 8];
     }
 #pragma unroll
     for (int m = 0; m < 4; ++m) {
       if (!in[m]) continue;
-      const f32x4 y[2] = {unpack4(q[m][0], q[m][1]), unpack4(q[m][2], q[m][3])};
+      const f32x4 y[2] = {joined4(q[m][0], q[m][1], q4[m] << 4 & 0xf0f0f0f0u), joined4(q[m][2], q[m][3], q4[m] & 0xf0f0f0f0u)};
 #pragma unroll
       for (int i = 0; i < CPL; ++i) sum[i] += w[m] * y[i / 4][i % 4];
     }
@@ -267,7 +271,7 @@ bool few_pairs(int64_t P, int64_t H, int64_t I, int64_t E) {
 
 struct ExpertLayout {  // byte offsets in the workspace
   int64_t rows, max_tiles, chunks;
-  int64_t tiles, n_tiles, counts, from, to, act, y, bytes;
+  int64_t tiles, n_tiles, counts, from, to, act, y, nibbles, bytes;
 };
 
 ExpertLayout expert_layout(int64_t N, int64_t H, int64_t I, int64_t E, int64_t k) {
@@ -283,7 +287,8 @@ ExpertLayout expert_layout(int64_t N, int64_t H, int64_t I, int64_t E, int64_t k
   l.to = l.from + round16(P * 4);
   l.act = l.to + round16(P * 4);
   l.y = l.act + P * I * 2;
-  l.bytes = l.y + P * H * 2;
+  l.nibbles = l.y + P * H * 2;
+  l.bytes = l.nibbles + P * H / 2;
   return l;
 }
 
@@ -350,6 +355,7 @@ extern "C" int gdn_expert_mlp(const void* x, int64_t ldx, const void* gate_up, c
   unsigned char* ws = static_cast<unsigned char*>(workspace);
   CombineParams c = {};
   c.y = reinterpret_cast<const uint16_t*>(ws + l.y);
+  c.nibbles = reinterpret_cast<const uint32_t*>(ws + l.nibbles);
   c.indices = indices;
   c.weights = weights;
   c.base = static_cast<const uint16_t*>(base);
@@ -421,12 +427,13 @@ extern "C" int gdn_expert_mlp(const void* x, int64_t ldx, const void* gate_up, c
   p.expert_stride = H * I;
   p.up = 0;
   p.out = reinterpret_cast<uint16_t*>(ws + l.y);
+  p.nibbles = reinterpret_cast<uint32_t*>(ws + l.nibbles);
   p.ldo = H;
   p.N = static_cast<int>(H);
   p.K = static_cast<int>(I);
   p.from = nullptr;
   p.to = plan.to;
-  launch_experts<false, kPacked>(p, l, once, st);
+  launch_experts<false, kSplit>(p, l, once, st);
 
   hipLaunchKernelGGL(combine_kernel, dim3(static_cast<unsigned>((N * (H / 8) + 255) / 256)), dim3(256), 0, st, c);
   return gdn_host::check_launch("gdn_expert_mlp");

@@ -39,6 +39,7 @@ struct ProductParams {
   int64_t expert_stride;   // elements from an expert's weights to the next's
   int up;                  // SwiGLU: weight rows from a column's gate to its up (0: one row a column)
   uint16_t* out;
+  uint32_t* nibbles;       // kSplit: the sums' next four bits, eight columns a word, rows as out's
   int64_t ldo;
   int M, N, K;             // rows (without a plan), columns of out
   int n_tiles;             // tiles of columns
@@ -168,67 +169,37 @@ __device__ __forceinline__ void finish8(const ProductParams& p, float (&v)[CPL],
                u32x4{pk_bf16(v[0], v[1]), pk_bf16(v[2], v[3]), pk_bf16(v[4], v[5]), pk_bf16(v[6], v[7])});
 }
 
-// ------------------------------------------------- four sums in eight bytes
+// ------------------------------------------------- a sum in 20 bits
 //
 // An expert's results wait in memory for the sum over a token's experts.  Rounded to bf16 they would be off by as much
-// as the output's own rounding is.  In the same bytes, four neighbouring columns share an exponent: 8 bits, and 14 for
-// each column's signed multiple of 2^(exponent - 12), off by at most 2^-12 of the largest of the four (16 times less than
-// bf16 at its own).  8191, -8191 and -8192 stand for +inf, -inf and NaN.
-constexpr int kInf14 = 8191, kNan14 = -8192, kMost14 = 8190;
-
-__device__ __forceinline__ u32x2 pack4(const f32x4& v) {
-  // the exponent of 1.0005 times the largest, so that no multiple is over 8190 (below 2^-107 all count as there)
-  auto exponent = [](float top) { return max(__float_as_uint(top * 1.0005f) >> 23, 20u); };
-  auto bits = [](const uint32_t (&q)[4], uint32_t e) {
-    const uint32_t lo = (q[0] & 0x3fffu) | q[1] << 14, hi = (q[2] << 4 & 0x3ffffu) | q[3] << 18;
-    return u32x2{(lo & 0xfffffffu) | e << 28, e >> 4 | (hi & ~0xfu)};
-  };
-  uint32_t q[4];
-  if (fabsf(v[0] + v[1] + v[2] + v[3]) < INFINITY) {
-    const uint32_t e = exponent(fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3]))));
-    const float scale = __uint_as_float((266u - e) << 23);  // 2^(12 - (e - 127))
-    // added to 3 * 2^22 the multiple stands, rounded to nearest even, in the sum's low bits
+// as the output's own rounding is (2^-8 of a column); in fp32 they would be 60% more bytes.  So: the upper 20 bits of the
+// fp32 sum, rounded, 16 in a plane of bf16's width and four in a plane of nibbles.  A column is off by at most 2^-12 of itself
+// whatever lies beside it.  Half of the last bit is added to all: what carries runs into the exponent, as it should, and
+// leaves infinities and NaN as they are (a NaN is a bf16 operand's or the default one, whose lower half is zeros).
+__device__ __forceinline__ f32x4 half_added(const f32x4& v) {
+  f32x4 r;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) q[j] = __float_as_uint(__builtin_fmaf(v[j], scale, 12582912.0f));
-    return bits(q, e);
-  }
-  // an infinity or NaN among them (or a sum that overflows): the others keep their exponent
-  float top = 0.0f;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) top = fmaxf(top, fabsf(v[j]) < INFINITY ? fabsf(v[j]) : 0.0f);
-  const uint32_t e = min(exponent(top), 254u);
-  const float scale = __uint_as_float((266u - e) << 23);
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int x = v[j] != v[j] ? kNan14 : fabsf(v[j]) < INFINITY
-        ? static_cast<int>(__builtin_rintf(__builtin_amdgcn_fmed3f(v[j] * scale, -8190.0f, 8190.0f)))
-        : v[j] > 0.0f ? kInf14 : -kInf14;
-    q[j] = static_cast<uint32_t>(x);
-  }
-  return bits(q, e);
+  for (int j = 0; j < 4; ++j) r[j] = __uint_as_float(__float_as_uint(v[j]) + 0x800u);
+  return r;
 }
-
-__device__ __forceinline__ f32x4 unpack4(uint32_t lo, uint32_t hi) {
-  const uint32_t e = lo >> 28 | (hi & 0xfu) << 4;
-  const float scale = __uint_as_float((e - 12u) << 23);  // 2^((e - 127) - 12); e is from 20 on
-  const int q[4] = {static_cast<int>(lo << 18) >> 18, static_cast<int>(lo << 4) >> 18, static_cast<int>(hi << 14) >> 18,
-                    static_cast<int>(hi) >> 18};
-  f32x4 v;
-  bool odd = false;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    v[j] = static_cast<float>(q[j]) * scale;
-    odd |= q[j] > kMost14 || q[j] < -kMost14;
-  }
-  if (odd) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (q[j] == kNan14) v[j] = __uint_as_float(0x7fc00000u);
-      if (q[j] == kInf14) v[j] = INFINITY;
-      if (q[j] == -kInf14) v[j] = -INFINITY;
-    }
-  }
-  return v;
+__device__ __forceinline__ u32x2 upper16(const f32x4& v) {
+  return u32x2{__builtin_amdgcn_perm(__float_as_uint(v[1]), __float_as_uint(v[0]), 0x07060302u),
+               __builtin_amdgcn_perm(__float_as_uint(v[3]), __float_as_uint(v[2]), 0x07060302u)};
+}
+// The four columns' third bytes, whose upper nibbles count; those of eight columns: column j's is nibble 2 j, 4 + j's 2 j + 1.
+__device__ __forceinline__ uint32_t third8(const f32x4& v) {
+  return __builtin_amdgcn_perm(__float_as_uint(v[1]), __float_as_uint(v[0]), 0x0c0c0501u) |
+         __builtin_amdgcn_perm(__float_as_uint(v[3]), __float_as_uint(v[2]), 0x05010c0cu);
+}
+__device__ __forceinline__ uint32_t nibbles8(uint32_t first, uint32_t second) {
+  return (first >> 4 & 0x0f0f0f0fu) | (second & 0xf0f0f0f0u);
+}
+// Four sums back from their upper halves and third bytes.
+__device__ __forceinline__ f32x4 joined4(uint32_t lo, uint32_t hi, uint32_t third) {
+  return f32x4{__uint_as_float(__builtin_amdgcn_perm(lo, third, 0x0504000cu)),
+               __uint_as_float(__builtin_amdgcn_perm(lo, third, 0x0706010cu)),
+               __uint_as_float(__builtin_amdgcn_perm(hi, third, 0x0504020cu)),
+               __uint_as_float(__builtin_amdgcn_perm(hi, third, 0x0706030cu))};
 }
 
 // ------------------------------------------------------------------ product
@@ -274,7 +245,7 @@ __device__ __forceinline__ void wait_loads() {  // until at most N loads are on 
 
 enum Store {
   kBare,    // SwiGLU or nothing, to bf16
-  kPacked,  // nothing, four sums in eight bytes
+  kSplit,   // nothing, a sum in 20 bits (N and ldo multiples of 8)
   kFinish,  // all of the epilogue
   kPart,    // a slice of K's sums, as they are
 };
@@ -367,6 +338,7 @@ __device__ __forceinline__ void product_store(const ProductParams& p, f32x4 (&ac
       const int r = 16 * (i * WM + wm) + lr, row = min(r, rows - 1);
       const int64_t at = p.to ? p.to[row0 + row] : row0 + row;
       u32x2 y[OB];  // the blocks' four columns
+      uint32_t third[ST == kSplit ? OB : 1];
 #pragma unroll
       for (int b = 0; b < OB; ++b) {
         f32x4 v = acc[i][b];
@@ -374,10 +346,17 @@ __device__ __forceinline__ void product_store(const ProductParams& p, f32x4 (&ac
 #pragma unroll
           for (int j = 0; j < 4; ++j) v[j] = silu(v[j]) * acc[i][b + OB][j];
         }
-        if constexpr (ST == kPacked) y[b] = pack4(v);
-        else y[b] = u32x2{pk_bf16(v[0], v[1]), pk_bf16(v[2], v[3])};
+        if constexpr (ST == kSplit) {
+          v = half_added(v);
+          y[b] = upper16(v);
+          third[b] = third8(v);
+        } else {
+          y[b] = u32x2{pk_bf16(v[0], v[1]), pk_bf16(v[2], v[3])};
+        }
       }
       uint16_t* out = p.out + at * p.ldo + first;
+      uint32_t* nibbles = nullptr;
+      if constexpr (ST == kSplit) nibbles = p.nibbles + (at * p.ldo + first) / 8;
       if (whole) {
         // two blocks' halves change hands between the 16-lane rows: a lane then has 8 neighbouring columns of one
 #pragma unroll
@@ -386,12 +365,20 @@ __device__ __forceinline__ void product_store(const ProductParams& p, f32x4 (&ac
           const auto hi = __builtin_amdgcn_permlane16_swap(y[b][1], y[b + 1][1], false, false);
           if (r < rows)
             *reinterpret_cast<u32x4*>(out + (b + (lq & 1)) * 16 + (lq >> 1) * 8) = u32x4{lo[0], hi[0], lo[1], hi[1]};
+          if constexpr (ST == kSplit) {
+            const auto t = __builtin_amdgcn_permlane16_swap(third[b], third[b + 1], false, false);
+            if (r < rows) nibbles[(b + (lq & 1)) * 2 + (lq >> 1)] = nibbles8(t[0], t[1]);
+          }
         }
       } else {
 #pragma unroll
         for (int b = 0; b < OB; ++b) {
           const int c = first + b * 16 + 4 * lq;
           uint16_t* o = out + b * 16 + 4 * lq;
+          if constexpr (ST == kSplit) {  // of the 16-lane rows' pairs the even one has a word's first four columns
+            const auto t = __builtin_amdgcn_permlane16_swap(third[b], third[b], false, false);
+            if (r < rows && c < p.N && lq % 2 == 0) nibbles[b * 2 + lq / 2] = nibbles8(t[0], t[1]);
+          }
           if (r >= rows || c >= p.N) continue;
           if (wide) {
             *reinterpret_cast<u32x2*>(o) = y[b];

@@ -123,7 +123,8 @@ def expert_mlp(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor, indic
     ``[..., k]`` int32 and weights ``[..., k]`` fp32 as :func:`route_experts` returns
     them.  A choice outside ``[0, E)`` adds nothing, one that stands twice is
     added twice; a token without any is its base, or 0.  An expert's inner values
-    and its result are rounded to bf16, their sum once.
+    are rounded to bf16, its result to 12 bits of significand or not at all (off by
+    at most 2^-12 of itself), their fp32 sum once.
 
     ``workspace``: :func:`expert_mlp_workspace_bytes` bytes (allocated when absent
     or too small); calls that overlap need one each.  ``out`` may be the base

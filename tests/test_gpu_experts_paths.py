@@ -1,0 +1,79 @@
+"""The sparse MLP's operators on each of their kernels' paths: every tile that the sizes' rules
+can choose, the planned experts where they are read in place, captured or overlapped, and
+columns of one result that are far apart in size.
+
+Tolerances as in ``test_gpu_experts``, from whose helpers they come; an expert's result
+is rounded to 12 bits of significand on its way to the sum: off by at most 2^-12 of itself,
+whatever lies beside it.
+"""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+import multiplex_amd as mx
+from oracle import experts as ox
+from test_gpu_experts import DEV, U, _experts, _gen, _np, _sums, _within
+
+pytestmark = pytest.mark.gpu
+
+
+def _check_columns(y, x, gate_up, down, indices, weights, base):
+    """Each column within what its own sums and roundings come to."""
+    x, gate_up, down, weights, base = map(_np, (x, gate_up, down, weights, base))
+    indices = indices.cpu().numpy()
+    E, H, I = down.shape
+    ref = np.zeros_like(x) if base is None else base.copy()
+    tol = np.full_like(ref, 1e-36) + 2.0 ** -23 * np.abs(ref)
+    for e in np.unique(indices):
+        if not 0 <= e < E:
+            continue
+        t, j = np.nonzero(indices == e)
+        s, es = x[t] @ gate_up[e].T, _sums(x[t], gate_up[e])
+        g, up = s[:, :I], s[:, I:]
+        a = ox.silu(g) * up
+        ea = 1.13 * es[:, :I] * (np.abs(up) + es[:, I:]) + np.abs(ox.silu(g)) * es[:, I:] + (U + 2.0 ** -20) * np.abs(a)
+        r = a @ down[e].T
+        er = ea @ np.abs(down[e]).T + _sums(np.abs(a) + ea, down[e])
+        er += 2.0 ** -12 * (np.abs(r) + er)
+        w = weights[t, j][:, None]
+        np.add.at(ref, t, w * r)
+        np.add.at(tol, t, np.abs(w) * er + 2.0 ** -22 * np.abs(w * r))
+    _within(y, ref, tol + U * (np.abs(ref) + tol))
+
+
+# few pairs; tiles of 64 rows, of 128 and of 256; 157 MB of weights, which pass by the caches, in tiles of 64 and of 128
+PATHS = [(3, 136, 72, 4, 2), (600, 136, 72, 4, 2), (2048, 72, 1000, 8, 2), (4096, 72, 1000, 8, 2), (200, 512, 200, 256, 6),
+         (1400, 512, 200, 256, 6)]
+
+
+@pytest.mark.parametrize("base", [False, True])
+@pytest.mark.parametrize("N,H,I,E,k", PATHS)
+def test_expert_mlp_columns_far_apart(N, H, I, E, k, base):
+    """Columns a thousand and a million times their neighbours, as hidden states have them."""
+    x, gate_up, down, indices, weights, b = _experts(_gen(N), N, H, I, E, k, base)
+    scale = torch.ones(H, device=DEV)
+    scale[1::8], scale[6::16], scale[3::16] = 2.0 ** 10, 2.0 ** 20, 2.0 ** -10
+    down = (down * scale[:, None]).bfloat16()
+    y = mx.expert_mlp(x, gate_up, down, indices, weights, base=b)
+    _check_columns(y, x, gate_up, down, indices, weights, b)
+
+
+@pytest.mark.parametrize("N,H,I,E,k", PATHS[:3] + PATHS[4:5])
+def test_expert_mlp_every_nan_stays_one(N, H, I, E, k):
+    """NaNs of all sorts of bits among the weights: none becomes a number, and other columns are as without."""
+    x, gate_up, down, indices, weights, _ = _experts(_gen(N), N, H, I, E, k)
+    clean = mx.expert_mlp(x, gate_up, down, indices, weights)
+    bits = torch.tensor([0x7fff, -1, 0x7f81, 0x7fc0, -0x7f, -0x40], dtype=torch.int16, device=DEV).view(torch.bfloat16)
+    bad, cols = down.clone(), [0, 5, 18, 31, 44, H - 1]
+    for c, v in zip(cols, bits):
+        bad[:, c, I // 2] = v
+    y = mx.expert_mlp(x, gate_up, bad, indices, weights)
+    keep = [c for c in range(H) if c not in cols]
+    assert torch.isnan(y[:, cols]).all() and torch.equal(y[:, keep], clean[:, keep])
+    bad = x.clone()
+    bad[1, :6] = bits
+    y = mx.expert_mlp(bad, gate_up, down, indices, weights)
+    assert torch.isnan(y[1]).all() and torch.equal(y[2:], clean[2:]) and torch.equal(y[0], clean[0])
