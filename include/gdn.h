@@ -506,7 +506,8 @@ int gdn_rms_norm(const void* x, const void* res, void* h_out, const void* w, int
  *   s       softmax of the logits, or (sigmoid != 0) 1 / (1 + exp(-logit))
  *   c       s + bias[e] (NULL: s); the choice goes by c, the weights are s
  *   groups  equal ranges of experts: only the top_groups with the largest sums
- *           of their group_best (1 or 2) largest c can be chosen from
+ *           of their group_best (1 or 2) largest c can be chosen from (+inf and
+ *           -inf together count as -inf)
  *   indices [B*T, k]  the experts in the order of falling c, of equals the lowest
  *           index first; a NaN counts below every number
  *   weights [B*T, k]  s, divided by their sum (renormalize != 0), times scale;

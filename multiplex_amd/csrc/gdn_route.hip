@@ -127,7 +127,8 @@ __global__ __launch_bounds__(kThreads) void route_kernel(const RouteParams p) {
         second = larger(second, x < best ? x : best);
         best = larger(best, x);
       }
-      mine[g] = p.group_best > 1 && width > 1 ? best + second : best;
+      // (+inf and -inf, of biases, have no sum: NaN, which would stand before no other group and behind none)
+      mine[g] = p.group_best > 1 && width > 1 ? larger(best + second, -INFINITY) : best;
     }
     __syncthreads();
     uint64_t stay = 0;  // a lane's groups that stay, then all lanes'

@@ -39,7 +39,8 @@ def route_experts(logits: torch.Tensor, k: int, *, scoring: str = "softmax", bia
     ``scoring``: "softmax" over the experts or "sigmoid" of each.  The choice goes
     by the score plus ``bias [E]`` (fp32), the weights are the scores alone.  With
     ``groups`` > 1, equal ranges of experts, only the ``top_groups`` ranges with the
-    largest sums of their ``group_best`` (1 or 2) best can be chosen from.
+    largest sums of their ``group_best`` (1 or 2) best can be chosen from (+inf and
+    -inf, of biases, together count as -inf).
     ``renormalize`` divides the weights by their sum, ``scale`` multiplies them.
 
     The experts stand in the order of falling score, of equals the lowest index

@@ -75,7 +75,7 @@ def route(logits, k, scoring="softmax", bias=None, groups=1, top_groups=1, group
             for g in range(groups):
                 best = sorted((v for v in c[g * width:(g + 1) * width] if not np.isnan(v)), reverse=True)
                 best = (best + [-np.inf] * group_best)[: min(group_best, width)]
-                of.append(sum(best))
+                of.append(-np.inf if np.inf in best and -np.inf in best else sum(best))  # (a sum that is none)
             first = sorted(range(groups), key=lambda g: (-of[g], g))[:top_groups]
             allowed = [e for e in range(E) if e // width in first]
         order = sorted(allowed, key=lambda e: (-key[e][0], -key[e][1], e))[:k]

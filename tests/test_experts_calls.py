@@ -5,10 +5,12 @@ from __future__ import annotations
 
 import weakref
 
+import numpy as np
 import pytest
 import torch
 
 from multiplex_amd import _lib, attention, experts, linear
+from oracle import experts as ox
 
 
 class OnDevice(torch.Tensor):
@@ -63,3 +65,13 @@ def test_a_workspace_lives_until_its_launch(made, monkeypatch):
     made_here.clear(), alive.clear()
     experts.expert_mlp(_b(4, 16), _b(3, 16, 16), _b(3, 16, 8), _i(4, 2), _f(4, 2))
     assert alive == [True]
+
+
+def test_oracle_groups_of_infinite_biases():
+    """A group whose two best are +inf and -inf has no sum: it counts as -inf."""
+    inf = np.inf
+    bias = np.array([inf, -inf, -inf, -inf, 0.5, 0, 0, 0, 0.4, 0, 0, 0, 0, 0, 0, 0])
+    i, _ = ox.route(np.zeros((1, 16)), 4, scoring="sigmoid", bias=bias, groups=4, top_groups=2)
+    assert i.tolist() == [[4, 8, 5, 6]]
+    i, _ = ox.route(np.zeros((1, 16)), 4, scoring="sigmoid", bias=bias, groups=4, top_groups=2, group_best=1)
+    assert i.tolist() == [[0, 4, 5, 6]]

@@ -15,7 +15,7 @@ import torch
 
 import multiplex_amd as mx
 from oracle import experts as ox
-from test_gpu_experts import DEV, U, _experts, _gen, _np, _sums, _within
+from test_gpu_experts import DEV, U, _check_route, _experts, _gen, _np, _r, _sums, _within
 
 pytestmark = pytest.mark.gpu
 
@@ -77,3 +77,26 @@ def test_expert_mlp_every_nan_stays_one(N, H, I, E, k):
     bad[1, :6] = bits
     y = mx.expert_mlp(bad, gate_up, down, indices, weights)
     assert torch.isnan(y[1]).all() and torch.equal(y[2:], clean[2:]) and torch.equal(y[0], clean[0])
+
+
+# --------------------------------------------------------------- routing
+
+@pytest.mark.parametrize("times", [1, 200])  # of 20 tokens: 64 lanes a token, 32
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("E,groups,top_groups,k", [(16, 4, 2, 4), (256, 8, 4, 8), (60, 3, 1, 20)])
+def test_route_infinite_biases(E, groups, top_groups, k, scoring, times):
+    """Experts that are always (+inf) or never (-inf) to be taken: as many groups stay as are asked for, one with
+    both among its two best counting as -inf."""
+    g = _gen(E)
+    logits = _r(g, 20, E, dtype=torch.float32)
+    width = E // groups
+    for taken, never in (((0,), range(1, width)), ((1, width + 2), range(0, 0)), ((), range(E - width, E)),
+                         ((), range(0, E)), ((E - 1,), range(0, E - 1))):
+        bias = _r(g, E, dtype=torch.float32, scale=0.1)
+        bias[list(never)] = float("-inf")
+        bias[list(taken)] = float("inf")
+        for group_best in (1, 2):
+            kw = dict(scoring=scoring, bias=bias, groups=groups, top_groups=top_groups, group_best=group_best)
+            indices, weights = mx.route_experts(logits.repeat(times, 1), k, **kw)
+            _check_route((indices[:20], weights[:20]), logits, k, **kw)
+            assert torch.equal(indices, indices[:20].repeat(times, 1))
