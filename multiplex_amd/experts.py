@@ -22,7 +22,7 @@ import torch
 
 from . import _lib
 from .gated_delta import _dtype_code, _ptr, _require_device, _stream
-from .linear import _FLOATS, _even_rows, _forward_only, _out_rows, linear_act
+from .linear import _FLOATS, _even_rows, _forward_only, _out_rows, _watched, linear_act
 
 __all__ = ["route_experts", "expert_mlp", "expert_mlp_workspace_bytes", "SparseMLP"]
 
@@ -54,7 +54,7 @@ def route_experts(logits: torch.Tensor, k: int, *, scoring: str = "softmax", bia
     index, code, d = logits.get_device(), _FLOATS.get(logits.dtype), logits.dim()
     ld = _even_rows(logits) if d > 1 else None
     if (index < 0 or code is None or ld is None or k.__class__ is not int or k <= 0 or scoring not in _SCORING
-            or torch.is_grad_enabled() and (logits.requires_grad or bias is not None and bias.requires_grad)
+            or _watched() or torch.is_grad_enabled() and (logits.requires_grad or bias is not None and bias.requires_grad)
             or n_new is not None and not (d == 3 and n_new.dtype is torch.int32 and n_new.get_device() == index
                                           and n_new.shape == logits.shape[:1] and n_new.is_contiguous())
             or bias is not None and not (bias.dtype is torch.float32 and bias.get_device() == index
@@ -144,7 +144,7 @@ def expert_mlp(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor, indic
             and down.is_contiguous() and indices.is_contiguous() and weights.is_contiguous() and x.data_ptr() % 16 == 0
             and (base is None or base.dtype is bf16 and base.get_device() == index and base.shape == x.shape
                  and base.is_contiguous() and base.data_ptr() % 16 == 0)
-            and (workspace is None or workspace.get_device() == index and workspace.is_contiguous())
+            and (workspace is None or workspace.get_device() == index and workspace.is_contiguous()) and not _watched()
             and not (torch.is_grad_enabled() and (x.requires_grad or gate_up.requires_grad or down.requires_grad or
                                                   weights.requires_grad or base is not None and base.requires_grad))):
         return _expert_mlp_general(x, gate_up, down, indices, weights, base, out, workspace)

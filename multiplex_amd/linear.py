@@ -31,6 +31,7 @@ each).
 from __future__ import annotations
 
 import functools
+import sys
 from typing import Optional
 
 import torch
@@ -236,12 +237,31 @@ def _even_rows(t: torch.Tensor) -> Optional[int]:
     return (D if rows == 1 else ld) if rows == 1 or ld >= D else None
 
 
+_jit_tracing = getattr(torch._C, "_is_tracing", torch.jit.is_tracing)
+
+
+def _watched() -> bool:
+    """Whether something may follow the call that these calls do not serve
+    (:func:`_forward_only` looks closer): a trace, a dispatch mode, a forward-mode level."""
+    return bool(_jit_tracing() or getattr(forward_ad, "_current_level", 0) >= 0 or _dispatch_modes is None
+                or _dispatch_modes())
+
+
 def _forward_only(tensors, names) -> None:
-    """These calls have no backward: a gradient asked for is an error, not lost."""
+    """These calls have no backward and are no operators of torch's: a gradient or a
+    tangent asked for is an error, not lost, and so is a trace, which would hold the
+    result as a constant."""
     if torch.is_grad_enabled():
         for t, n in zip(tensors, names):
             if t is not None and t.requires_grad:
                 raise ValueError(f"{n} requires a gradient, which this call does not form (use torch.no_grad())")
+    proxies = sys.modules.get("torch.fx.experimental.proxy_tensor")  # (there is no such trace before it is imported)
+    if torch.jit.is_tracing() or proxies is not None and proxies.get_proxy_mode() is not None:
+        raise ValueError("this call cannot be traced: the trace would hold its result as a constant")
+    if getattr(forward_ad, "_current_level", 0) >= 0:  # (outside a dual level, -1, no tensor has a tangent)
+        for t, n in zip(tensors, names):
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise ValueError(f"{n} has a forward-mode tangent, which this call does not carry on")
 
 
 def _apart(out: torch.Tensor, others, names) -> None:
@@ -291,7 +311,7 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, *, bias: Optional[torch.Te
     index, bf16, act = x.get_device(), torch.bfloat16, _ACTS.get(activation)
     if (index >= 0 and act is not None and x.dtype is bf16 and weight.dtype is bf16 and weight.dim() == 2 and x.dim() > 0
             and out is None and workspace is None and weight.get_device() == index
-            and x.is_contiguous() and weight.is_contiguous()
+            and x.is_contiguous() and weight.is_contiguous() and not _watched()
             and not (torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
                                                   or bias is not None and bias.requires_grad
                                                   or row_gate is not None and row_gate.requires_grad

@@ -8,6 +8,8 @@ import weakref
 import numpy as np
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
+from torch.fx.experimental.proxy_tensor import make_fx
 
 from multiplex_amd import _lib, attention, experts, linear
 from oracle import experts as ox
@@ -75,3 +77,46 @@ def test_oracle_groups_of_infinite_biases():
     assert i.tolist() == [[4, 8, 5, 6]]
     i, _ = ox.route(np.zeros((1, 16)), 4, scoring="sigmoid", bias=bias, groups=4, top_groups=2, group_best=1)
     assert i.tolist() == [[0, 4, 5, 6]]
+
+
+# Each call as a function of one of its inputs.
+CALLS = {
+    "linear_act": (lambda x: linear.linear_act(x, _b(8, 16)), lambda: _b(4, 16)),
+    "linear_act's weight": (lambda w: linear.linear_act(_b(4, 16), w), lambda: _b(8, 16)),
+    "linear_act's row gate": (lambda r: linear.linear_act(_b(4, 16), _b(8, 16), row_gate=r), lambda: _f(4)),
+    "route_experts": (lambda l: experts.route_experts(l, 2)[1], lambda: _f(4, 16)),
+    "expert_mlp": (lambda x: experts.expert_mlp(x, _b(3, 16, 16), _b(3, 16, 8), _i(4, 2), _f(4, 2)), lambda: _b(4, 16)),
+    "expert_mlp's weights": (lambda w: experts.expert_mlp(_b(4, 16), _b(3, 16, 16), _b(3, 16, 8), _i(4, 2), w),
+                             lambda: _f(4, 2)),
+}
+
+
+@pytest.mark.parametrize("call", CALLS)
+def test_a_tangent_is_refused(made, call):
+    f, t = CALLS[call]
+    with forward_ad.dual_level():
+        f(t())  # none of its tensors has one
+        assert len(made) == 1
+        with pytest.raises(ValueError, match="tangent"):
+            f(forward_ad.make_dual(t(), torch.ones_like(t())))
+    assert len(made) == 1
+
+
+@pytest.mark.parametrize("call", CALLS)
+def test_a_trace_is_refused(made, call):
+    """It would hold the result as a constant."""
+    f, t = CALLS[call]
+    plain = t().as_subclass(torch.Tensor)
+    for trace in (lambda: torch.jit.trace(f, (plain,), check_trace=False), lambda: make_fx(f)(plain)):
+        with pytest.raises(ValueError, match="traced"):
+            trace()
+    assert not made
+
+
+def test_a_mode_that_only_looks_on_is_served(made):
+    from torch.utils.flop_counter import FlopCounterMode
+
+    with FlopCounterMode(display=False):
+        for f, t in CALLS.values():
+            f(t())
+    assert len(made) == len(CALLS)

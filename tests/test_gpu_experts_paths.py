@@ -12,6 +12,8 @@ from __future__ import annotations
 import numpy as np
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
+from torch.fx.experimental.proxy_tensor import make_fx
 
 import multiplex_amd as mx
 from oracle import experts as ox
@@ -100,3 +102,23 @@ def test_route_infinite_biases(E, groups, top_groups, k, scoring, times):
             indices, weights = mx.route_experts(logits.repeat(times, 1), k, **kw)
             _check_route((indices[:20], weights[:20]), logits, k, **kw)
             assert torch.equal(indices, indices[:20].repeat(times, 1))
+
+
+# ------------------------------------------------- what follows an operator
+
+def test_tangents_and_traces_are_refused():
+    g = _gen(3)
+    x, w, logits = _r(g, 8, 64), _r(g, 16, 64), _r(g, 8, 16, dtype=torch.float32)
+    a = _experts(g, 8, 64, 32, 6, 2)
+    calls = [(lambda t: mx.linear_act(t, w), x), (lambda t: mx.route_experts(t, 2)[1], logits),
+             (lambda t: mx.expert_mlp(t, *a[1:5]), a[0])]
+    for f, t in calls:
+        want = f(t)
+        with forward_ad.dual_level():
+            assert torch.equal(f(t), want)
+            with pytest.raises(ValueError, match="tangent"):
+                f(forward_ad.make_dual(t, torch.ones_like(t)))
+        for trace in (lambda: torch.jit.trace(f, (t,), check_trace=False), lambda: make_fx(f)(t)):
+            with pytest.raises(ValueError, match="traced"):
+                trace()
+        assert torch.equal(f(t), want)
