@@ -535,7 +535,7 @@ size_t gdn_expert_mlp_workspace_bytes(int64_t N, int64_t H, int64_t I, int64_t E
  * for few pairs, not at all); the sum of the k is formed in fp32 and rounded once.
  * out may alias base.  Calls that overlap need a workspace each.
  * H and I multiples of 8, strides too; pointers 16-byte aligned; x spans less
- * than 2 GiB, an expert's gate_up too.
+ * than 2 GiB, an expert's gate_up too; I up to 2^22.
  */
 int gdn_expert_mlp(const void* x, int64_t ldx, const void* gate_up, const void* down, const int32_t* indices,
                    const float* weights, const void* base, int64_t ldb, void* out, int64_t ldo, int64_t N, int64_t H,

@@ -18,6 +18,8 @@ namespace {
 
 constexpr int kMaxExperts = 1024;
 constexpr int kMaxChoices = 64;
+// The second product's rows, the inner values, are 32-bit byte offsets from a tile's first one of up to 256, below 2 GiB.
+constexpr int64_t kMostInner = (int64_t{1} << 30) / 256;
 
 // -------------------------------------------------------------------- plan
 //
@@ -343,6 +345,8 @@ extern "C" int gdn_expert_mlp(const void* x, int64_t ldx, const void* gate_up, c
     return fail(GDN_ERR_UNSUPPORTED, "gdn_expert_mlp: x spans more than 2 GiB (pass fewer tokens a call)");
   if (!weights_fit(2 * I + 256, H) || !weights_fit(H, I))
     return fail(GDN_ERR_UNSUPPORTED, "gdn_expert_mlp: an expert's weights exceed 2 GiB");
+  if (I > kMostInner)
+    return fail(GDN_ERR_UNSUPPORTED, "gdn_expert_mlp: I=%lld exceeds %lld", (long long)I, (long long)kMostInner);
   const ExpertLayout l = expert_layout(N, H, I, E, k);
   if (!workspace || workspace_bytes < static_cast<size_t>(l.bytes) || !aligned(workspace, 16))
     return fail(GDN_ERR_INVALID, "gdn_expert_mlp: needs a 16-byte aligned workspace of %lld bytes (got %zu)",

@@ -120,3 +120,16 @@ def test_a_mode_that_only_looks_on_is_served(made):
         for f, t in CALLS.values():
             f(t())
     assert len(made) == len(CALLS)
+
+
+@pytest.mark.parametrize("N", [1, 300, 1 << 13])
+def test_inner_rows_past_a_tiles_offsets_are_refused(N):
+    """A tile's rows of inner values are found by 32-bit byte offsets: 256 of more than 2^22 values pass 2 GiB."""
+    fake = 0x10000  # only ever compared, never read
+    lib = _lib.load()
+
+    def call(I):
+        return lib.gdn_expert_mlp(fake, 8, fake, fake, fake, fake, None, 0, fake, 8, N, 8, I, 1, 1, fake + 8, 1 << 60, None)
+
+    assert call((1 << 22) + 8) == _lib.ERR_UNSUPPORTED
+    assert call(1 << 22) == _lib.ERR_INVALID  # as far as the workspace, which is misaligned
