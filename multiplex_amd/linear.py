@@ -247,6 +247,25 @@ def _watched() -> bool:
                 or _dispatch_modes())
 
 
+def _spacing(t: torch.Tensor) -> Optional[int]:
+    """Elements from a value of ``[...]`` to the next where they are evenly spaced (0: one
+    value for all), else None."""
+    if t.dim() == 1:
+        return t.stride(0)
+    if t.is_contiguous():
+        return 1
+    step, values = 1, 1
+    for n, s in zip(reversed(t.shape), reversed(t.stride())):
+        if n == 1:
+            continue
+        if values == 1:
+            step = s
+        elif s != values * step:
+            return None
+        values *= n
+    return step
+
+
 def _forward_only(tensors, names) -> None:
     """These calls have no backward and are no operators of torch's: a gradient or a
     tangent asked for is an error, not lost, and so is a trace, which would hold the
@@ -324,9 +343,11 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, *, bias: Optional[torch.Te
         if bias is not None:
             bias_dt = _FLOATS.get(bias.dtype, -1) if (bias.shape == (rows,) and bias.get_device() == index
                                                       and bias.is_contiguous()) else -1
-        if row_gate is not None:  # (of one dimension: any stride; otherwise contiguous)
-            gate_dt = _FLOATS.get(row_gate.dtype, -1) if (row_gate.shape == lead and row_gate.get_device() == index and
-                                                          (len(lead) == 1 or row_gate.is_contiguous())) else -1
+        ldg = 0
+        if row_gate is not None:
+            ldg = _spacing(row_gate)
+            gate_dt = _FLOATS.get(row_gate.dtype, -1) if (row_gate.shape == lead and row_gate.get_device() == index
+                                                          and ldg is not None) else -1
         if (x.shape[-1] == K and K > 0 and K % 8 == 0 and N > 0 and (act != 5 or rows % 2 == 0) and (xp | wp) % 16 == 0
                 and bias_dt >= 0 and gate_dt >= 0
                 and (residual is None or residual.dtype is bf16 and residual.get_device() == index
@@ -337,8 +358,7 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, *, bias: Optional[torch.Te
             # (bound until the call returns: its memory may be another thread's as soon as the tensor is gone)
             ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
             _lib.call(dev, "gdn_linear_act", xp, K, wp, None if bias is None else bias.data_ptr(), bias_dt, act,
-                      None if row_gate is None else row_gate.data_ptr(), gate_dt,
-                      0 if row_gate is None else row_gate.stride(0) if len(lead) == 1 else 1,
+                      None if row_gate is None else row_gate.data_ptr(), gate_dt, ldg,
                       None if residual is None else residual.data_ptr(), N, out.data_ptr(), N, M, N, K,
                       None if ws is None else ws.data_ptr(), need, _stream(dev))
             return out
@@ -386,7 +406,7 @@ def _linear_act_general(x, weight, bias, activation, row_gate, residual, out, wo
         if row_gate.shape != lead:
             raise ValueError(f"row_gate must be {list(lead)}, one value per row of x (got {list(row_gate.shape)})")
         gate_dt = _dtype_code(row_gate, "row_gate")
-        ldg = _even_rows(row_gate.unsqueeze(-1))
+        ldg = _spacing(row_gate)
         if ldg is None:
             row_gate, ldg = row_gate.contiguous(), 1
     if residual is not None:

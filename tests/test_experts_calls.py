@@ -133,3 +133,34 @@ def test_inner_rows_past_a_tiles_offsets_are_refused(N):
 
     assert call((1 << 22) + 8) == _lib.ERR_UNSUPPORTED
     assert call(1 << 22) == _lib.ERR_INVALID  # as far as the workspace, which is misaligned
+
+
+def _layer(**kw):
+    a = dict(hidden_size=64, num_attention_heads=2, num_key_value_heads=1, head_dim=128, intermediate_size=32,
+             num_experts=6, num_experts_per_tok=2, moe_intermediate_size=16, shared_expert_intermediate_size=24)
+    return attention.AttentionArgs(**{**a, **kw})
+
+
+@pytest.mark.parametrize("lead", [(5,), (4, 1), (1, 6), (2, 3), (2, 3, 4)])
+def test_the_layers_calls_take_the_short_way(made, monkeypatch, lead):
+    """(A row gate that is a column of a wider product, of any number of dimensions, among them.)"""
+    for mod, name in ((linear, "_linear_act_general"), (experts, "_route_general"), (experts, "_expert_mlp_general")):
+        monkeypatch.setattr(mod, name, lambda *a, name=name: pytest.fail(name))
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda self: 0)
+    m = experts.SparseMLP(_layer())
+    m(_b(*lead, 64), residual=_b(*lead, 64))
+    assert [n for n, _ in made] == ["gdn_linear_act", "gdn_route_experts", "gdn_linear_act", "gdn_linear_act", "gdn_expert_mlp"]
+    gate, ld = made[3][1][6], made[3][1][8]
+    assert gate - made[0][1][11] == 6 * 2 and ld == 7  # the seventh column of what the router's product wrote
+
+
+def test_row_gates_of_other_layouts(made):
+    """Evenly spaced ones are read in place (one value for all among them), others copied."""
+    x, w = _b(2, 3, 16), _b(8, 16)
+    for gate, ld in ((_f(2, 3), 1), (_f(2, 3, 5)[..., 2], 5), (_f(1).expand(2, 3), 0), (_f(3, 2).T, None),
+                     (_f(2, 1).expand(2, 3), None), (_f(2, 4)[:, :3], None)):
+        made.clear()
+        linear.linear_act(x, w, row_gate=gate)
+        (_, args), = made
+        assert args[8] == (1 if ld is None else ld)
+        assert (args[6] == gate.data_ptr()) == (ld is not None)
