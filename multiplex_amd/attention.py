@@ -528,10 +528,11 @@ class Attention(torch.nn.Module):
         return ranges if block_us * (blocks - of_range) > 3.5 + mb_us * partials else 1
 
     def forward(self, x: torch.Tensor, cache: "KVCache | PagedKVCache",
-                n_new: Optional[Sequence[int]] = None) -> torch.Tensor:
+                n_new: Optional[Sequence[int]] = None, counts: Optional[torch.Tensor] = None) -> torch.Tensor:
         """The layer's output for T new tokens a row, appended to ``cache``.  With
         a :class:`PagedKVCache`, ``n_new`` (host counts) says how many of the T a
-        row has; the rest is padding, whose outputs are unspecified."""
+        row has; the rest is padding, whose outputs are unspecified.  ``counts`` is
+        n_new on the device (:meth:`PagedKVCache.counts`), where the caller has it."""
         B, T, _ = x.shape
         Hq, Hkv, D = self.Hq, self.Hkv, self.D
         pool = getattr(cache, "pool", None)
@@ -542,7 +543,7 @@ class Attention(torch.nn.Module):
         if pool is not None and B * T == 0:
             return linear(x.new_empty(B, T, Hq * D), self.o_proj)
         if pool is not None:
-            counts = None if n_new is None else cache.counts(n_new)
+            counts = None if n_new is None else cache.counts(n_new) if counts is None else counts
             slots = cache.reserve(T, n_new, counts)
             q = attn_rope(qg, k, v, self.q_norm.weight, self.k_norm.weight, self.args.rms_norm_eps, cache.pos0,
                           pool.keys, pool.values, self.rotary, slots=slots)
@@ -622,7 +623,7 @@ class DecoderLayer(torch.nn.Module):
         else:
             xin, y0 = self.input_layernorm(x, residual=residual)
         # the residual add in front of the second norm is fused into it
-        h, y = self.post_attention_layernorm(xin, residual=self.self_attn(y0, cache, n_new))
+        h, y = self.post_attention_layernorm(xin, residual=self.self_attn(y0, cache, n_new, counts))
         return h, y, counts
 
 

@@ -122,3 +122,29 @@ def test_tangents_and_traces_are_refused():
             with pytest.raises(ValueError, match="traced"):
                 trace()
         assert torch.equal(f(t), want)
+
+
+# ------------------------------------------------------------------ layers
+
+def _layer_args(**kw):
+    a = dict(hidden_size=256, num_attention_heads=4, num_key_value_heads=2, head_dim=128, intermediate_size=0,
+             num_experts=24, num_experts_per_tok=4, moe_intermediate_size=72, shared_expert_intermediate_size=136)
+    return mx.AttentionArgs(**{**a, **kw})
+
+
+@pytest.mark.parametrize("experts", [24, 0])
+def test_a_padded_step_uploads_its_counts_once(monkeypatch, experts):
+    torch.manual_seed(5)
+    layer = mx.DecoderLayer(_layer_args(num_experts=experts, intermediate_size=72), DEV)
+    made, counts = [], mx.PagedKVCache.counts
+    monkeypatch.setattr(mx.PagedKVCache, "counts", lambda self, n_new: made.append(counts(self, n_new)) or made[-1])
+    x = torch.randn(2, 5, 256, device=DEV).bfloat16()
+    cache = mx.PagedKVCache(mx.BlockPool(16, 2, 128, device=DEV), 2)
+    layer(x, cache, n_new=[5, 2])
+    assert len(made) == 1 and cache.lengths == [5, 2] and cache.pos0.tolist() == [5, 2]
+    layer.forward_parts(x, None, cache, [0, 5])
+    assert len(made) == 2 and cache.lengths == [5, 7] and cache.pos0.tolist() == [5, 7]
+    for bad in ([1], [1, 6], [-1, 2]):
+        with pytest.raises(ValueError):
+            layer(x, cache, n_new=bad)
+        assert cache.lengths == [5, 7] and cache.pos0.tolist() == [5, 7]
