@@ -81,6 +81,7 @@ class AttentionArgs:
     n_group: int = 1
     topk_group: int = 1
     routed_scaling_factor: float = 1.0
+    group_best: int = 2  # a group's score is the sum of its one or two best experts'
 
     @property
     def rot(self) -> int:

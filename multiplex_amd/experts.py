@@ -274,7 +274,8 @@ class SparseMLP(torch.nn.Module):
         both = linear_act(x, self.router)
         indices, weights = route_experts(both[..., : self.E], a.num_experts_per_tok, scoring=a.scoring_func,
                                          bias=bias, groups=a.n_group, top_groups=a.topk_group,
-                                         renormalize=a.norm_topk_prob, scale=a.routed_scaling_factor, n_new=n_new)
+                                         group_best=a.group_best, renormalize=a.norm_topk_prob,
+                                         scale=a.routed_scaling_factor, n_new=n_new)
         base = residual
         if self.shared_down_proj is not None:
             s = linear_act(x, self.shared_gate_up_proj, activation="swiglu")

@@ -164,3 +164,14 @@ def test_row_gates_of_other_layouts(made):
         (_, args), = made
         assert args[8] == (1 if ld is None else ld)
         assert (args[6] == gate.data_ptr()) == (ld is not None)
+
+
+def test_the_layers_routing_is_its_arguments(made, monkeypatch):
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda self: 0)
+    for kw, want in ((dict(), (0, 1, 1, 2, 1, 1.0)),
+                     (dict(scoring_func="sigmoid", n_group=3, topk_group=2, group_best=1, norm_topk_prob=False,
+                           routed_scaling_factor=2.5), (1, 3, 2, 1, 0, 2.5))):
+        made.clear()
+        experts.SparseMLP(_layer(**kw))(_b(4, 64))
+        (args,) = [a for n, a in made if n == "gdn_route_experts"]
+        assert args[11:17] == want
