@@ -255,6 +255,15 @@ class SparseMLP(torch.nn.Module):
             raise ValueError("the shared expert's weights go with shared_expert_intermediate_size > 0, all of them")
         if (router_bias is None) != (self.router_bias is None):
             raise ValueError("a router bias goes with args.router_bias")
+        E, H, I = self.down_proj.shape
+        S = 0 if self.shared_down_proj is None else self.shared_down_proj.shape[1]
+        for name, t, shape in (("gate", gate, (E, H)), ("gate_proj", gate_proj, (E, I, H)), ("up_proj", up_proj, (E, I, H)),
+                               ("down_proj", down_proj, (E, H, I)), ("shared_gate_proj", shared_gate_proj, (S, H)),
+                               ("shared_up_proj", shared_up_proj, (S, H)), ("shared_down_proj", shared_down_proj, (H, S)),
+                               ("shared_expert_gate", None if shared_expert_gate is None else
+                                shared_expert_gate.reshape(1, -1), (1, H)), ("router_bias", router_bias, (E,))):
+            if t is not None and tuple(t.shape) != shape:
+                raise ValueError(f"{name} must be {list(shape)} (got {list(t.shape)})")
         self.router.copy_(gate if shared_expert_gate is None else torch.cat([gate, shared_expert_gate.view(1, -1)]))
         self.gate_up_proj.copy_(torch.cat([gate_proj, up_proj], 1))
         self.down_proj.copy_(down_proj)

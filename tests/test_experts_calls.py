@@ -175,3 +175,32 @@ def test_the_layers_routing_is_its_arguments(made, monkeypatch):
         experts.SparseMLP(_layer(**kw))(_b(4, 64))
         (args,) = [a for n, a in made if n == "gdn_route_experts"]
         assert args[11:17] == want
+
+
+@pytest.mark.parametrize("name,shape", [
+    ("gate", (1, 64)), ("gate", (64,)), ("gate", (5, 64)), ("gate_proj", (1, 16, 64)), ("up_proj", (6, 16, 1)),
+    ("up_proj", (6, 8, 64)), ("down_proj", (1, 64, 16)), ("down_proj", (64, 16)), ("shared_gate_proj", (23, 64)),
+    ("shared_down_proj", (64, 1)), ("shared_expert_gate", (2, 64)), ("router_bias", (1,)),
+])
+def test_loading_other_shapes_is_refused(name, shape):
+    """(A weight of one expert would be spread over all of them, halves of other sizes make a whole.)"""
+    shapes = dict(gate=(6, 64), gate_proj=(6, 16, 64), up_proj=(6, 16, 64), down_proj=(6, 64, 16), shared_gate_proj=(24, 64),
+                  shared_up_proj=(24, 64), shared_down_proj=(64, 24), shared_expert_gate=(1, 64), router_bias=(6,))
+    m = experts.SparseMLP(_layer(router_bias=True))
+    w = {n: torch.ones(s) for n, s in shapes.items()}
+    before = {n: p.clone() for n, p in m.state_dict().items()}
+    other = {"gate_proj": "up_proj", "up_proj": "gate_proj", "shared_gate_proj": "shared_up_proj"}.get(name)
+    if shape == (1, 16, 64):  # both halves, as they would be given
+        w[other] = torch.ones(shape)
+    if shape in ((6, 8, 64), (23, 64)):  # the other half makes up for it
+        w[other] = torch.ones(6, 24, 64) if len(shape) == 3 else torch.ones(25, 64)
+    with pytest.raises(ValueError):
+        m.load(**{**w, name: torch.ones(shape)})
+    assert all(torch.equal(p, before[n]) for n, p in m.state_dict().items())
+
+
+def test_loading_takes_the_shapes_that_it_names():
+    m = experts.SparseMLP(_layer())
+    w = [torch.randn(s).bfloat16() for s in ((6, 64), (6, 16, 64), (6, 16, 64), (6, 64, 16), (24, 64), (24, 64), (64, 24), (64,))]
+    m.load(*w)
+    assert torch.equal(m.router, torch.cat([w[0], w[7][None]])) and torch.equal(m.gate_up_proj[:, 16:], w[2])
