@@ -129,8 +129,8 @@ def expert_mlp(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor, indic
 
     ``workspace``: :func:`expert_mlp_workspace_bytes` bytes (allocated when absent
     or too small); calls that overlap need one each.  ``out`` may be the base
-    itself, and otherwise lies apart from all that is read (other columns of one
-    buffer are refused too).  There is no backward.
+    itself (which may be x), and otherwise lies apart from all that is read (other
+    columns of one buffer are refused too).  There is no backward.
     """
     index, bf16 = x.get_device(), torch.bfloat16
     E, H, I = down.shape if down.dim() == 3 else (0, 0, 0)
@@ -202,7 +202,10 @@ def _expert_mlp_general(x, gate_up, down, indices, weights, base, out, workspace
     if out is None:
         out, ldo = torch.empty(x.shape, dtype=bf16, device=dev), H
     else:
-        _out_rows(out, x.shape, base, (x, gate_up, down, indices, weights, workspace),
+        # (x is read before anything is written, so it may be the rows of the base that out is)
+        place = [(t.data_ptr(), _even_rows(t)) for t in (out, x, base) if t is not None]
+        in_place = len(place) == 3 and place[0] == place[1] == place[2]
+        _out_rows(out, x.shape, base, (None if in_place else x, gate_up, down, indices, weights, workspace),
                   ("x", "gate_up", "down", "indices", "weights", "workspace"))
         ldo = _even_rows(out)
     if workspace is not None and not workspace.is_contiguous():

@@ -204,3 +204,18 @@ def test_loading_takes_the_shapes_that_it_names():
     w = [torch.randn(s).bfloat16() for s in ((6, 64), (6, 16, 64), (6, 16, 64), (6, 64, 16), (24, 64), (24, 64), (64, 24), (64,))]
     m.load(*w)
     assert torch.equal(m.router, torch.cat([w[0], w[7][None]])) and torch.equal(m.gate_up_proj[:, 16:], w[2])
+
+
+def test_in_place_of_x_and_base(made):
+    """out = base = x on the short way and on the long one alike; x alone, or other rows of it, are refused."""
+    a = dict(gate_up=_b(3, 16, 16), down=_b(3, 16, 8), indices=_i(4, 2), weights=_f(4, 2))
+    for x in (_b(4, 16), _b(4, 24)[:, :16], _b(4, 16).as_subclass(torch.Tensor)):
+        assert experts.expert_mlp(x, **a, base=x, out=x) is x
+        view = x[:]
+        assert experts.expert_mlp(view, **a, base=x, out=x) is x
+        with pytest.raises(ValueError, match="overlaps x"):
+            experts.expert_mlp(x, **a, base=_b(4, 16), out=x)
+    assert [n for n, _ in made] == ["gdn_expert_mlp"] * 6
+    buf = _b(6, 24)
+    with pytest.raises(ValueError, match="overlaps x"):
+        experts.expert_mlp(buf[1:5, :16], **a, base=buf[:4, :16], out=buf[:4, :16])

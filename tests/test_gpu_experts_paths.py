@@ -81,6 +81,20 @@ def test_expert_mlp_every_nan_stays_one(N, H, I, E, k):
     assert torch.isnan(y[1]).all() and torch.equal(y[2:], clean[2:]) and torch.equal(y[0], clean[0])
 
 
+@pytest.mark.parametrize("N,H,I,E,k", PATHS[:3])
+def test_expert_mlp_in_place(N, H, I, E, k):
+    """x, base and out the same rows."""
+    x, gate_up, down, indices, weights, _ = _experts(_gen(N), N, H, I, E, k)
+    want = mx.expert_mlp(x, gate_up, down, indices, weights, base=x)
+    wide = torch.full((N, H + 16), 7.0, dtype=torch.bfloat16, device=DEV)
+    rows = wide[:, 8:8 + H]
+    rows.copy_(x)
+    assert mx.expert_mlp(rows, gate_up, down, indices, weights, base=rows, out=rows) is rows
+    assert torch.equal(rows, want) and (wide[:, :8] == 7).all() and (wide[:, 8 + H:] == 7).all()
+    assert mx.expert_mlp(x, gate_up, down, indices, weights, base=x, out=x) is x
+    assert torch.equal(x, want)
+
+
 # --------------------------------------------------------------- routing
 
 @pytest.mark.parametrize("times", [1, 200])  # of 20 tokens: 64 lanes a token, 32
