@@ -524,6 +524,13 @@ int gdn_route_experts(const void* logits, int dtype, int64_t ld, const float* bi
 size_t gdn_expert_mlp_workspace_bytes(int64_t N, int64_t H, int64_t I, int64_t E, int64_t k);
 
 /*
+ * The way gdn_expert_mlp takes for these sizes: rows of x a tile (64, 128 or 256),
+ * 0 where the pairs are few and run without a plan; a GDN_ERR_* for sizes it does
+ * not take.
+ */
+int gdn_expert_mlp_tile_rows(int64_t N, int64_t H, int64_t I, int64_t E, int64_t k);
+
+/*
  * out[t] = base[t] + sum_j weights[t][j] * mlp_e(x[t]) with e = indices[t][j] and
  * mlp_e(x) = (silu(x G_e^T) * (x U_e^T)) D_e^T:
  *   x [N, H], base (NULL: 0) and out [N, H]: rows ldx, ldb, ldo elements apart
@@ -551,6 +558,13 @@ int gdn_expert_mlp(const void* x, int64_t ldx, const void* gate_up, const void* 
 
 /* Workspace bytes of gdn_linear_act (0 for sizes it needs none for). */
 size_t gdn_linear_act_workspace_bytes(int64_t M, int64_t N, int64_t K, int act);
+
+/*
+ * The way gdn_linear_act takes for these sizes: tile[0] rows of x by tile[1] rows of
+ * W a tile, K in tile[2] slices (1: whole); 0, 0, 0 for the few rows that run
+ * without tiles.
+ */
+int gdn_linear_act_tile(int64_t M, int64_t N, int64_t K, int act, int32_t* tile);
 
 /*
  * out[M, N] = act(x[M, K] W^T + bias) * sigmoid(row_gate[m]) + residual[m], rounded once:

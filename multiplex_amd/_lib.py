@@ -60,8 +60,10 @@ EXPORTS = (
     "gdn_rms_norm",
     "gdn_route_experts",
     "gdn_expert_mlp_workspace_bytes",
+    "gdn_expert_mlp_tile_rows",
     "gdn_expert_mlp",
     "gdn_linear_act_workspace_bytes",
+    "gdn_linear_act_tile",
     "gdn_linear_act",
     "gdn_pos_add",
     "gdn_silu_mul",
@@ -222,11 +224,13 @@ _SIGNATURES = {
         [_P, c_int, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _I64, c_int, _I64, _I64, _I64, c_int, c_double, _P],
     ),
     "gdn_expert_mlp_workspace_bytes": (c_size_t, [_I64, _I64, _I64, _I64, _I64]),
+    "gdn_expert_mlp_tile_rows": (c_int, [_I64, _I64, _I64, _I64, _I64]),
     "gdn_expert_mlp": (
         c_int,
         [_P, _I64, _P, _P, _P, _P, _P, _I64, _P, _I64, _I64, _I64, _I64, _I64, _I64, _P, c_size_t, _P],
     ),
     "gdn_linear_act_workspace_bytes": (c_size_t, [_I64, _I64, _I64, c_int]),
+    "gdn_linear_act_tile": (c_int, [_I64, _I64, _I64, c_int, POINTER(c_int32)]),
     "gdn_linear_act": (
         c_int,
         [_P, _I64, _P, _P, c_int, c_int, _P, c_int, _I64, _P, _I64, _P, _I64, _I64, _I64, _I64, _P, c_size_t, _P],

@@ -323,6 +323,12 @@ extern "C" size_t gdn_expert_mlp_workspace_bytes(int64_t N, int64_t H, int64_t I
   return static_cast<size_t>(expert_layout(N, H, I, E, k).bytes);
 }
 
+extern "C" int gdn_expert_mlp_tile_rows(int64_t N, int64_t H, int64_t I, int64_t E, int64_t k) {
+  if (!expert_sizes_ok(N, H, I, E, k))
+    return gdn_host::fail(GDN_ERR_INVALID, "gdn_expert_mlp_tile_rows: sizes that gdn_expert_mlp does not take");
+  return few_pairs(N * k, H, I, E) ? 0 : static_cast<int>(tile_rows(N * k, I, E));
+}
+
 extern "C" int gdn_expert_mlp(const void* x, int64_t ldx, const void* gate_up, const void* down, const int32_t* indices,
                               const float* weights, const void* base, int64_t ldb, void* out, int64_t ldo, int64_t N,
                               int64_t H, int64_t I, int64_t E, int64_t k, void* workspace, size_t workspace_bytes,

@@ -149,6 +149,12 @@ Tiling tiling(int64_t M, int64_t N, int64_t K, bool pair) {
 
 constexpr int kFewRows = 4;
 
+// Values of K a slice (whole steps), and how many slices hold any.
+int64_t slice_values(const Tiling& t, int64_t K) { return ((K + 63) / 64 + t.slices - 1) / t.slices * 64; }
+int slices_of(const Tiling& t, int64_t K) {
+  return static_cast<int>((K + slice_values(t, K) - 1) / slice_values(t, K));
+}
+
 int64_t part_pitch(int64_t N, bool pair) { return (N + 3) / 4 * 4 * (pair ? 2 : 1); }
 
 int64_t part_bytes(int64_t M, int64_t N, int64_t K, bool pair) {
@@ -193,6 +199,18 @@ bool linear_sizes_ok(int64_t M, int64_t N, int64_t K, int act) {
 
 extern "C" size_t gdn_linear_act_workspace_bytes(int64_t M, int64_t N, int64_t K, int act) {
   return linear_sizes_ok(M, N, K, act) ? static_cast<size_t>(part_bytes(M, N, K, act == GDN_ACT_SWIGLU)) : 0;
+}
+
+extern "C" int gdn_linear_act_tile(int64_t M, int64_t N, int64_t K, int act, int32_t* tile) {
+  if (!linear_sizes_ok(M, N, K, act) || !tile)
+    return gdn_host::fail(GDN_ERR_INVALID, "gdn_linear_act_tile: sizes that gdn_linear_act does not take, or no place");
+  tile[0] = tile[1] = tile[2] = 0;
+  if (M <= kFewRows) return GDN_OK;
+  const Tiling t = tiling(M, N, K, act == GDN_ACT_SWIGLU);
+  tile[0] = t.rows;
+  tile[1] = t.weight_rows;
+  tile[2] = slices_of(t, K);
+  return GDN_OK;
 }
 
 extern "C" int gdn_linear_act(const void* x, int64_t ldx, const void* W, const void* bias, int bias_dtype, int act,
@@ -247,16 +265,14 @@ extern "C" int gdn_linear_act(const void* x, int64_t ldx, const void* W, const v
   }
   const Tiling t = tiling(M, N, K, pair);
   if (t.slices > 1) {
-    const int64_t need = part_bytes(M, N, K, pair), steps = (K + 63) / 64;
+    const int64_t need = part_bytes(M, N, K, pair);
     if (!workspace || workspace_bytes < static_cast<size_t>(need) || !aligned(workspace, 16))
       return fail(GDN_ERR_INVALID, "gdn_linear_act: needs a 16-byte aligned workspace of %lld bytes (got %zu)",
                   (long long)need, workspace_bytes);
-    p.slices = t.slices;
-    p.slice = static_cast<int>((steps + t.slices - 1) / t.slices * 64);
+    p.slices = slices_of(t, K);
+    p.slice = static_cast<int>(slice_values(t, K));
     p.pitch = static_cast<int>(part_pitch(N, pair));
     p.part = static_cast<float*>(workspace);
-    if (static_cast<int64_t>(p.slice) * (t.slices - 1) >= K)  // (no slice is empty)
-      p.slices = static_cast<int>((K + p.slice - 1) / p.slice);
   }
   if (pair) launch_tiles<true>(p, t, bare, st);
   else launch_tiles<false>(p, t, bare, st);

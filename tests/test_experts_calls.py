@@ -3,8 +3,12 @@ ways run on CPU tensors that claim a device, and the launch is a stand-in."""
 
 from __future__ import annotations
 
+import ctypes
+import math
+import random
 import weakref
 
+import linear_sizes
 import numpy as np
 import pytest
 import torch
@@ -219,3 +223,50 @@ def test_in_place_of_x_and_base(made):
     buf = _b(6, 24)
     with pytest.raises(ValueError, match="overlaps x"):
         experts.expert_mlp(buf[1:5, :16], **a, base=buf[:4, :16], out=buf[:4, :16])
+
+
+# ------------------------------------------------------------------ the sizes' rules
+
+def _linear_tile(M, N, K, act):
+    tile = (ctypes.c_int32 * 3)()
+    assert _lib.load().gdn_linear_act_tile(M, N, K, linear._ACTS[act], tile) == _lib.OK
+    return tuple(tile)
+
+
+@pytest.mark.parametrize("M,N,K,act,tile", linear_sizes.SIZES)
+def test_linear_act_runs_the_tile(M, N, K, act, tile):
+    """What the GPU tests run at these sizes is what they say (refit the sizes with the rule)."""
+    assert _linear_tile(M, N, K, act) == tile
+    need = linear.linear_act_workspace_bytes(M, N, K, act)
+    pitch = (N + 3) // 4 * 4 * (2 if act == "swiglu" else 1)
+    assert need == (4 * tile[2] * M * pitch if tile[2] > 1 else 0)
+
+
+@pytest.mark.parametrize("act", [None, "gelu", "swiglu"])
+@pytest.mark.parametrize("M,N,K", [(600, 1000, 8200), (64, 1026, 8192), (130, 517, 12296)])
+def test_the_sliced_sizes_are_sliced(M, N, K, act):
+    """Those of ``test_gpu_experts``, which passes over the ones that are not."""
+    assert _linear_tile(M, N, K, act)[2] > 1 and linear.linear_act_workspace_bytes(M, N, K, act) > 0
+
+
+def test_every_tile_is_run():
+    """Each tile whole, and in every number of slices that the rule gives it, with and without SwiGLU."""
+    run = {(act, tile) for *_, act, tile in linear_sizes.SIZES}
+    rng = random.Random(1)
+    for _ in range(20000):
+        M, N, K = (int(math.exp(rng.uniform(math.log(a), math.log(b)))) for a, b in ((5, 6000), (8, 30000), (1, 1600)))
+        for act in (None, "swiglu"):
+            assert (act, _linear_tile(M, N, 8 * K, act)) in run
+    for M in (1, 2, 3, 4):
+        assert _linear_tile(M, 1000, 4096, None) == (0, 0, 0)
+
+
+def test_the_tiles_calls_refuse_what_the_products_do():
+    lib = _lib.load()
+    tile = (ctypes.c_int32 * 3)()
+    for args in ((-1, 8, 8, 0), (8, 0, 8, 0), (8, 8, 12, 0), (8, 8, 8, 6)):
+        assert lib.gdn_linear_act_tile(*args, tile) == _lib.ERR_INVALID
+    assert lib.gdn_linear_act_tile(8, 8, 8, 0, None) == _lib.ERR_INVALID
+    assert lib.gdn_expert_mlp_tile_rows(8, 12, 8, 4, 2) == _lib.ERR_INVALID
+    assert lib.gdn_expert_mlp_tile_rows(1, 64, 32, 4, 2) == 0
+    assert lib.gdn_expert_mlp_tile_rows(4096, 2048, 512, 256, 8) in (64, 128, 256)
