@@ -572,9 +572,9 @@ int gdn_linear_act_tile(int64_t M, int64_t N, int64_t K, int act, int32_t* tile)
  *   bias (NULL: none)      one value a row of W
  *   row_gate (NULL: none)  one value a row of x, ldg elements apart
  *   residual (NULL: none)  bf16 rows ldr elements apart; out may alias it
- * K and ldx multiples of 8, x and W 16-byte aligned.  A few hundred rows of a
- * long K are summed in slices of K (in slice order) through the workspace;
- * calls that overlap need one each.
+ * K and ldx multiples of 8, x and W 16-byte aligned.  From five rows on a
+ * long K may be summed in slices (in slice order, a launch more) through the
+ * workspace; calls that overlap need one each.
  */
 int gdn_linear_act(const void* x, int64_t ldx, const void* W, const void* bias, int bias_dtype, int act,
                    const void* row_gate, int row_gate_dtype, int64_t ldg, const void* residual, int64_t ldr, void* out,

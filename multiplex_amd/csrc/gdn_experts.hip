@@ -251,9 +251,9 @@ int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
 
 // Rows of the experts' tiles.  128 by 256 weight rows use the matrix units and LDS best where the experts have the rows
 // for it and the tiles are enough for the CUs, 256 by 256 where they have more of both; us in 64-, 128-, 256-row tiles:
-//   2048 x 512, 8 of 256: 512 tokens (16 rows an expert) 314, 314, 318; 1024 (32) 342, 332, 348; 4096 (128) 539, 470, 494
-//   1024 x 512, 6 of 64: 1024 (96) 81, 86, 95; 2048 (192) 110, 93, 107; 4096 (384) 172, 150, 136
-//   1536 x 1000, 2 of 8: 512 (128; 96 tiles of 128 rows) 39, 50, 71; 4096 (1024) 147, 132, 123
+//   2048 x 512, 8 of 256: 512 tokens (16 rows an expert) 290, 315, 345; 1024 (32) 344, 340, 365; 4096 (128) 562, 490, 486
+//   1024 x 512, 6 of 64: 1024 (96) 81, 83, 101; 2048 (192) 116, 96, 125; 4096 (384) 179, 159, 142
+//   1536 x 1000, 2 of 8: 512 (128; 96 tiles of 128 rows) 42, 52, 75; 4096 (1024) 154, 134, 128
 int64_t tile_rows(int64_t P, int64_t I, int64_t E) {
   for (const int64_t rows : {256, 128}) {
     if (P >= (rows == 256 ? 256 : 32) * E && (P / rows + E / 2) * ((I + 127) / 128) >= kCUs) return rows;
@@ -263,8 +263,10 @@ int64_t tile_rows(int64_t P, int64_t I, int64_t E) {
 
 // Whether the pairs are few: each reads its own weights, without a plan, against those of the experts that are chosen at
 // all and a longer way.  Tokens at which the plan becomes the faster one, us without and with it:
-//   2048 x 512, 8 of 256: 8 67, 82; 16 130, 121.  4096 x 1536, 4 of 32: 4 97, 115; 8 184, 145
-//   1096 x 328, 3 of 12: 8 14.5, 20.4; 16 22.5, 20.7.  1536 x 1000, 2 of 8: 4 15, 22; 8 27, 23
+//   2048 x 512, 8 of 256: 8 63, 66; 16 125, 107.  4096 x 1536, 4 of 32: 4 96, 104; 8 187, 123 to 138
+//   1096 x 328, 3 of 12: 8 15, 20; 16 23.5, 20.5.  1536 x 1000, 2 of 8: 4 16.4, 22.5; 8 26.7, 24.7
+// (choices that crowd on some experts, as these did, leave the plan fewer weights to read than the rule expects: at 16
+// tokens of the first it still takes the pairs' way)
 bool few_pairs(int64_t P, int64_t H, int64_t I, int64_t E) {
   if (P > 1024) return false;
   const double mb = 6e-6 * H * I, chosen = E * (1.0 - std::pow(1.0 - 1.0 / E, static_cast<double>(P)));
@@ -296,8 +298,8 @@ ExpertLayout expert_layout(int64_t N, int64_t H, int64_t I, int64_t E, int64_t k
 
 // Whether the weights pass by the caches: where an expert has about one tile and the weights would not stay in the 256 MB
 // last-level cache until a model's next step in any case (us with and without, 2048 x 512, 8 of 256, 1.6 GB: 64 tokens
-// 196, 206; 512 290, 320; 2048 376, 390; but 4096, half of whose experts have a second tile, 510, 470; 1536 x 1000, 2 of 8,
-// 74 MB, which the next call finds there, 64 tokens 38, 29).
+// 195, 224; 512 288, 314; 2048 377, 380; but 4096, half of whose experts have a second tile, 523, 489; 1536 x 1000, 2 of 8,
+// 74 MB, which the next call finds there, 64 tokens 39, 27).
 bool weights_once(int64_t P, int64_t H, int64_t I, int64_t E) {
   return P <= 64 * E && 6e-6 * E * H * I >= 128.0;
 }

@@ -226,7 +226,9 @@ class SparseMLP(torch.nn.Module):
 
     The router's and the shared gate's rows are one weight (``router``: E rows,
     then the shared gate's), so both come from one product.  With
-    ``args.router_bias`` the choice goes by the scores plus ``router_bias``.
+    ``args.router_bias`` the choice goes by the scores plus ``router_bias``.  The
+    logits are rounded to bf16, as mlx-lm's router's are (its scores, as these, are
+    formed in a wider type from there on).
     """
 
     def __init__(self, args, device=None, dtype=torch.bfloat16):

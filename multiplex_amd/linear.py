@@ -19,7 +19,7 @@ is given alone.
 
 :func:`linear` is the layers' plain projection: a few rows by
 ``gdn_linear_rows16``, the library beyond.  :func:`linear_act` is a projection
-with its epilogue (bias, activation, row gate, residual) in the product's launch.
+with its epilogue (bias, activation, row gate, residual) in the product's own kernels.
 
 The sliced kernel sums its K slices through a workspace of fp32 partials and one
 ticket per output tile; the tickets must start at zero and every call
@@ -312,8 +312,8 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, *, bias: Optional[torch.Te
                activation: Optional[str] = None, row_gate: Optional[torch.Tensor] = None,
                residual: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
                workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """``act(x @ weight.T + bias) * sigmoid(row_gate) + residual`` in one launch
-    (``gdn_linear_act``), rounded once.
+    """``act(x @ weight.T + bias) * sigmoid(row_gate) + residual`` (``gdn_linear_act``), in
+    one launch or, where K is summed in slices, two, rounded once.
 
     x ``[..., K]`` and weight ``[N, K]`` bf16, K a multiple of 8; ``activation`` is
     None, "relu", "silu", "gelu" (erf), "gelu_tanh" or "swiglu" (``silu(gate) * up``:
@@ -323,8 +323,8 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, *, bias: Optional[torch.Te
     x and residual may be column slices of wider buffers.  ``out`` may be the
     residual itself, and otherwise lies apart from all that is read (other columns
     of one buffer are refused too).  ``workspace``: bytes for the sums of K's slices, which some
-    sizes are formed in (:func:`linear_act_workspace_bytes`; allocated when absent
-    or too small); calls that overlap need one each.  There is no backward.
+    sizes of five rows or more are formed in (:func:`linear_act_workspace_bytes`;
+    allocated when absent or too small); calls that overlap need one each.  There is no backward.
     """
     # a plain call's checks in a few operations; what is wrong, or laid out otherwise, is looked into below
     index, bf16, act = x.get_device(), torch.bfloat16, _ACTS.get(activation)
