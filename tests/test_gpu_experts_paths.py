@@ -243,6 +243,45 @@ def test_planned_in_two_graphs():
             assert torch.equal(got, mx.expert_mlp(*a[:5], base=a[5]))
 
 
+# ------------------------------------------------------------ far offsets
+
+def test_far_offsets_linear_act():
+    """x, residual and out that pass 4 GiB: their last rows."""
+    g = _gen(1)
+    M, K, N, tail = 70000, 64, 32776, 40
+    w = _r(g, N, K, scale=K ** -0.5)
+    x = torch.empty(M, 32800, dtype=torch.bfloat16, device=DEV)[:, 8:8 + K]
+    x.copy_(_r(g, M, K))
+    res = torch.zeros(M, N, dtype=torch.bfloat16, device=DEV)
+    res[-tail:] = _r(g, tail, N)
+    y = mx.linear_act(x, w, residual=res)
+    for rows in (slice(0, tail), slice(M // 2, M // 2 + tail), slice(M - tail, M)):
+        _check_linear(y[rows], x[rows], w, None, None, None, res[rows])
+
+
+def test_far_offsets_experts():
+    """Results of pairs that wait in more than 4 GiB: the last tokens'."""
+    g = _gen(2)
+    N, H, I, E, k, tail = 300000, 1024, 16, 8, 8, 40
+    gate_up, down = _r(g, E, 2 * I, H, scale=H ** -0.5), _r(g, E, H, I, scale=I ** -0.5)
+    x = torch.randn(N, H, device=DEV).bfloat16()
+    indices = torch.rand(N, E, device=DEV).argsort(-1).int()
+    weights = torch.rand(N, k, device=DEV)
+    y = mx.expert_mlp(x, gate_up, down, indices, weights)
+    for rows in (slice(0, tail), slice(N // 2, N // 2 + tail), slice(N - tail, N)):
+        _check_columns(y[rows], x[rows], gate_up, down, indices[rows], weights[rows], None)
+
+
+def test_far_offsets_routing():
+    """Logits that pass 4 GiB."""
+    N, E, tail = 2200000, 1000, 20
+    logits = torch.empty(N, 1024, dtype=torch.bfloat16, device=DEV)[:, 8:8 + E]
+    logits.normal_()
+    indices, weights = mx.route_experts(logits, 4)
+    for rows in (slice(0, tail), slice(N // 2, N // 2 + tail), slice(N - tail, N)):
+        _check_route((indices[rows], weights[rows]), logits[rows], 4)
+
+
 # ------------------------------------------------- what follows an operator
 
 def test_tangents_and_traces_are_refused():
