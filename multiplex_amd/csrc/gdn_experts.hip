@@ -318,6 +318,9 @@ bool expert_sizes_ok(int64_t N, int64_t H, int64_t I, int64_t E, int64_t k) {
          I % 8 == 0 && H <= INT32_MAX / 4 && I <= INT32_MAX / 4 && N <= (INT32_MAX - 2 * kChunk) / k;
 }
 
+// Whether 32-bit byte offsets reach an expert's weights and a tile's inner values.
+bool expert_fits(int64_t H, int64_t I) { return weights_fit(2 * I + 256, H) && weights_fit(H, I) && I <= kMostInner; }
+
 }  // namespace
 
 extern "C" size_t gdn_expert_mlp_workspace_bytes(int64_t N, int64_t H, int64_t I, int64_t E, int64_t k) {
@@ -328,6 +331,7 @@ extern "C" size_t gdn_expert_mlp_workspace_bytes(int64_t N, int64_t H, int64_t I
 extern "C" int gdn_expert_mlp_tile_rows(int64_t N, int64_t H, int64_t I, int64_t E, int64_t k) {
   if (!expert_sizes_ok(N, H, I, E, k))
     return gdn_host::fail(GDN_ERR_INVALID, "gdn_expert_mlp_tile_rows: sizes that gdn_expert_mlp does not take");
+  if (!expert_fits(H, I)) return gdn_host::fail(GDN_ERR_UNSUPPORTED, "gdn_expert_mlp_tile_rows: weights too large");
   return few_pairs(N * k, H, I, E) ? 0 : static_cast<int>(tile_rows(N * k, I, E));
 }
 
@@ -351,10 +355,9 @@ extern "C" int gdn_expert_mlp(const void* x, int64_t ldx, const void* gate_up, c
     return fail(GDN_ERR_INVALID, "gdn_expert_mlp: misaligned pointer");
   if (N > ((int64_t{1} << 30) - H) / ldx + 1)
     return fail(GDN_ERR_UNSUPPORTED, "gdn_expert_mlp: x spans more than 2 GiB (pass fewer tokens a call)");
-  if (!weights_fit(2 * I + 256, H) || !weights_fit(H, I))
-    return fail(GDN_ERR_UNSUPPORTED, "gdn_expert_mlp: an expert's weights exceed 2 GiB");
-  if (I > kMostInner)
-    return fail(GDN_ERR_UNSUPPORTED, "gdn_expert_mlp: I=%lld exceeds %lld", (long long)I, (long long)kMostInner);
+  if (!expert_fits(H, I))
+    return fail(GDN_ERR_UNSUPPORTED, "gdn_expert_mlp: an expert's weights exceed 2 GiB, or I=%lld is over %lld", (long long)I,
+                (long long)kMostInner);
   const ExpertLayout l = expert_layout(N, H, I, E, k);
   if (!workspace || workspace_bytes < static_cast<size_t>(l.bytes) || !aligned(workspace, 16))
     return fail(GDN_ERR_INVALID, "gdn_expert_mlp: needs a 16-byte aligned workspace of %lld bytes (got %zu)",

@@ -195,6 +195,9 @@ bool linear_sizes_ok(int64_t M, int64_t N, int64_t K, int act) {
          act >= GDN_ACT_NONE && act <= GDN_ACT_SWIGLU;
 }
 
+// Whether 32-bit byte offsets reach a tile's weights.
+bool linear_fits(int64_t N, int64_t K, int act) { return weights_fit(act == GDN_ACT_SWIGLU ? N + 256 : 256, K); }
+
 }  // namespace
 
 extern "C" size_t gdn_linear_act_workspace_bytes(int64_t M, int64_t N, int64_t K, int act) {
@@ -204,6 +207,8 @@ extern "C" size_t gdn_linear_act_workspace_bytes(int64_t M, int64_t N, int64_t K
 extern "C" int gdn_linear_act_tile(int64_t M, int64_t N, int64_t K, int act, int32_t* tile) {
   if (!linear_sizes_ok(M, N, K, act) || !tile)
     return gdn_host::fail(GDN_ERR_INVALID, "gdn_linear_act_tile: sizes that gdn_linear_act does not take, or no place");
+  if (!linear_fits(N, K, act))
+    return gdn_host::fail(GDN_ERR_UNSUPPORTED, "gdn_linear_act_tile: rows too long");
   tile[0] = tile[1] = tile[2] = 0;
   if (M <= kFewRows) return GDN_OK;
   const Tiling t = tiling(M, N, K, act == GDN_ACT_SWIGLU);
@@ -233,7 +238,7 @@ extern "C" int gdn_linear_act(const void* x, int64_t ldx, const void* W, const v
       !aligned(bias, size(bias_dtype)) || !aligned(row_gate, size(row_gate_dtype)))
     return fail(GDN_ERR_INVALID, "gdn_linear_act: misaligned pointer");
   const bool pair = act == GDN_ACT_SWIGLU;
-  if (!weights_fit(pair ? N + 256 : 256, K) || ldx > (int64_t{1} << 30) / 256 - 64)
+  if (!linear_fits(N, K, act) || ldx > (int64_t{1} << 30) / 256 - 64)
     return fail(GDN_ERR_UNSUPPORTED, "gdn_linear_act: rows too long");
   if ((M / 64 + 1) * (N / 16 + 1) > INT32_MAX / 2)
     return fail(GDN_ERR_UNSUPPORTED, "gdn_linear_act: problem too large");

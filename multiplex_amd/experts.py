@@ -120,9 +120,9 @@ def expert_mlp(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor, indic
     token's experts ``e = indices[..., j]`` (``gdn_expert_mlp``).
 
     x ``[..., H]``, gate_up ``[E, 2I, H]`` (per expert the gate's rows, then up's),
-    down ``[E, H, I]``, base ``[..., H]`` bf16; H and I multiples of 8; indices
-    ``[..., k]`` int32 and weights ``[..., k]`` fp32 as :func:`route_experts` returns
-    them.  A choice outside ``[0, E)`` adds nothing, one that stands twice is
+    down ``[E, H, I]``, base ``[..., H]`` bf16; H and I multiples of 8, the
+    experts' weights and ``out``'s rows 16-byte aligned; indices ``[..., k]`` int32 and
+    weights ``[..., k]`` fp32 as :func:`route_experts` returns them.  A choice outside ``[0, E)`` adds nothing, one that stands twice is
     added twice; a token without any is its base, or 0.  An expert's inner values
     are rounded to bf16, its result to 12 bits of significand or not at all (off by
     at most 2^-12 of itself), their fp32 sum once.

@@ -270,3 +270,8 @@ def test_the_tiles_calls_refuse_what_the_products_do():
     assert lib.gdn_expert_mlp_tile_rows(8, 12, 8, 4, 2) == _lib.ERR_INVALID
     assert lib.gdn_expert_mlp_tile_rows(1, 64, 32, 4, 2) == 0
     assert lib.gdn_expert_mlp_tile_rows(4096, 2048, 512, 256, 8) in (64, 128, 256)
+    # sizes that are refused for what they would span
+    assert lib.gdn_expert_mlp_tile_rows(300, 8, (1 << 22) + 8, 1, 1) == _lib.ERR_UNSUPPORTED
+    assert lib.gdn_expert_mlp_tile_rows(300, 1 << 16, 1 << 14, 1, 1) == _lib.ERR_UNSUPPORTED
+    assert lib.gdn_linear_act_tile(300, 8, 1 << 23, 0, tile) == _lib.ERR_UNSUPPORTED
+    assert lib.gdn_linear_act_tile(300, 1 << 24, 64, 5, tile) == _lib.ERR_UNSUPPORTED
